@@ -25,6 +25,9 @@ extern "C" {
 
 /* tensor dtypes, same codes as the reference's qm_dtype (src/qm_base.h:11-15) */
 enum { QMH_F32 = 0, QMH_Q8_0 = 2, QMH_Q4_0 = 3 };
+/* 16-bit element types of rows, pages and logits, for the ops of "several continuations of one prompt"
+ * below only: no weight and no file has them. No reference counterpart. */
+enum { QMH_F16 = 1, QMH_BF16 = 4 };
 
 /* ------------------------------------------------------------------ runtime */
 
@@ -88,6 +91,154 @@ int qmh_rope(float *v, int64_t n_heads, int64_t head_dim, int64_t pos, float the
 int qmh_swiglu(float *gate, const float *up, int64_t n, void *stream);
 /* *out = first index of the maximum. qm_argmax (src/sampler.c:27-32) */
 int qmh_argmax(const float *x, int32_t n, int32_t *out, void *stream);
+
+/* ------------------------------------------------------------------ several continuations of one prompt
+ * Op level, device pointers, as above: asynchronous on the stream (NULL = the library's), 0 or -1 with a
+ * message, nothing allocated. No reference counterpart (the reference runs one sequence), so these are not
+ * under the bitwise contract: sums and softmax statistics are held in 32 bits (64 where a choice hangs on
+ * them), results are rounded once to their type, and are the same from run to run. A step of a
+ * program that answers one prompt with several sequences: qmh_paged_append the new tokens,
+ * qmh_paged_attention in each layer, then for a beam search qmh_beam_select and one of the reorders.
+ * The calling thread's current device must be the library's. Calls that share a workspace must not overlap;
+ * graphs that may run at the same time need workspaces of their own. */
+
+/* Keys and values in pages on the device: k and v are [n_pages][n_kv_heads][page_size][head_dim] of dtype
+ * (QMH_F32, QMH_F16 or QMH_BF16), 16-byte aligned; page_size a power of two in [16, 1024], head_dim a
+ * multiple of 8 in [8, 256]. A table row of page numbers says where a sequence's positions lie: position
+ * t is row t % page_size of page table[t / page_size]. Entries behind a sequence's last page are not
+ * read. A page number outside [0, n_pages) is never followed (each op says what it does instead). */
+typedef struct {
+    int32_t dtype;
+    int32_t n_kv_heads, head_dim, page_size;
+    int64_t n_pages;
+    void *k, *v;
+} qmh_pages;
+
+/* The rotation of queries and keys: pairs of the first rot_dim elements of a head are turned by
+ * position * f_i radians, i < rot_dim / 2, and scaled by magnitude; the others stay. f_i = theta^(-2i / rot_dim),
+ * stretched for contexts longer than first_len by `scaling`:
+ *   QMH_ROTARY_LINEAR  f_i / factor
+ *   QMH_ROTARY_NTK     theta * factor^(rot_dim / (rot_dim - 2)) in theta's place (rot_dim > 2)
+ *   QMH_ROTARY_BANDS   f_i (w + (1 - w) / factor), w = (first_len f_i / 2 pi - low) / (high - low) held to [0, 1]: pairs
+ *                      that turn more than `high` times in first_len positions stay, fewer than `low` are slowed
+ *   QMH_ROTARY_YARN    the same with the ramp over pair numbers: w = 1 - (i - a) / (b - a) held to [0, 1], where
+ *                      c(n) = rot_dim ln(first_len / (2 pi n)) / (2 ln theta), a = max(floor c(high), 0),
+ *                      b = min(ceil c(low), rot_dim - 1), b - a at least 0.001
+ * Pairs are (2i, 2i + 1) (QMH_ROTARY_PAIRS, as qmh_rope) or (i, i + rot_dim / 2) (QMH_ROTARY_HALVES).
+ * Angles, their sines and cosines are computed in 64 bits for every position below max_pos (at most 2^24). */
+enum { QMH_ROTARY_PAIRS = 0, QMH_ROTARY_HALVES = 1 };
+enum { QMH_ROTARY_PLAIN = 0, QMH_ROTARY_LINEAR = 1, QMH_ROTARY_NTK = 2, QMH_ROTARY_BANDS = 3, QMH_ROTARY_YARN = 4 };
+typedef struct {
+    int32_t rot_dim, layout, scaling, max_pos, first_len;
+    float theta, factor, low, high, magnitude;
+} qmh_rotary_config;
+typedef struct qmh_rotary qmh_rotary;
+/* Tables of the rotation on the device (max_pos / 1024 + 1024 rows of rot_dim / 2 sine and cosine pairs in 64 bits).
+ * Synchronous. NULL on error. Free it when no call that uses it is under way. */
+qmh_rotary *qmh_rotary_create(const qmh_rotary_config *cfg);
+void qmh_rotary_free(qmh_rotary *r);
+
+/* New tokens into a paged cache, in one pass: queries and keys of each head normed (optional) and rotated
+ * (optional), keys and values written to the pages, queries to q_out. Rows are of the pages' dtype.
+ * Token t < n_tokens belongs to sequence seq[t] (a row of table [n_seq][table_stride]), is its position slot[t]
+ * in the pages, and is rotated by position pos[t] (NULL: slot[t]; they differ where a shared prefix lies before
+ * the sequence's own pages). With gains: x_i g_i / sqrt(mean x^2 + eps) over a head, g of head_dim floats.
+ * q: row t at q + t * q_stride elements, n_heads heads after one another; q_out alike (q_out = q with the same
+ * stride is allowed); both NULL: no queries. k, v: n_kv_heads heads a row; both NULL: queries only, and then
+ * pages->k, v, table, seq and (with pos) slot are not looked at. k, v and q may be parts of the same rows.
+ * A token whose seq, slot, page or pos is outside its range (slot < table_stride * page_size, pos < the rotary's
+ * max_pos) is left out, nothing of it is written: pos or slot -1 pads a batch. No two tokens of a call may name
+ * the same slot of the same sequence (the slot then holds a mixture of theirs). */
+typedef struct {
+    const qmh_pages *pages;
+    const qmh_rotary *rotary; /* NULL: no rotation */
+    int32_t n_tokens, n_heads;
+    const void *q;
+    int64_t q_stride;
+    void *q_out;
+    int64_t q_out_stride;
+    const void *k;
+    int64_t k_stride;
+    const void *v;
+    int64_t v_stride;
+    const float *q_gain, *k_gain; /* NULL: no norm */
+    float eps;
+    int32_t n_seq;
+    const int32_t *table;
+    int32_t table_stride;
+    const int32_t *seq, *slot, *pos;
+} qmh_append_args;
+int qmh_paged_append(const qmh_append_args *a, void *stream);
+
+/* Attention of n_seq sequences with q_len queries each, over a prefix that a group's sequences share and
+ * over each one's own pages: out = softmax(scale q k) v. Sequence i is in group i / (n_seq / n_groups) (n_groups divides n_seq). Its queries see
+ * the group's prefix, prefix_len[g] positions in the pages of prefix_table[g] [n_groups][prefix_stride], then its own
+ * pages, len[i] positions in table[i] [n_seq][table_stride]: the queries are the last q_len of these, query j
+ * sees positions below len[i] - q_len + 1 + j. The prefix's keys and values are read for all queries of a
+ * group together. Rows of q and out are of the pages' dtype: query j of sequence i is row i * q_len + j, n_heads
+ * heads after one another (n_heads a multiple of n_kv_heads: consecutive heads share a kv head); out must not
+ * overlap q. Lengths are read on the device; max_len and max_prefix are their upper bounds, from which the work
+ * is divided (0: no own pages / no prefix, the table and lengths then unused).
+ * Scores are held in 32 bits: products that pass their range are infinite. A query that sees nothing (or only scores of
+ * -inf) gives zeros. Where a sequence's len is outside [0, max_len] or a page it needs is outside
+ * the pool, its rows are NaN; a group's prefix does so for all its sequences. What lies in pages behind a length
+ * has no effect, whatever it holds. A position below len is the sequence's: an infinite or NaN value
+ * there may reach its queries that do not see it, too.
+ * ws: qmh_paged_attention_ws(a) bytes (0 for bad arguments), 16-byte aligned, any contents. */
+typedef struct {
+    const qmh_pages *pages;
+    int32_t n_heads, n_seq, q_len, n_groups;
+    const void *q;
+    int64_t q_stride;
+    void *out;
+    int64_t out_stride;
+    const int32_t *table, *len;
+    int32_t table_stride, max_len;
+    const int32_t *prefix_table, *prefix_len;
+    int32_t prefix_stride, max_prefix;
+    float scale;
+} qmh_attention_args;
+size_t qmh_paged_attention_ws(const qmh_attention_args *a);
+int qmh_paged_attention(const qmh_attention_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* A beam search's choice: the n_out best continuations of each group of n_beams rows of logits. Row b of a group
+ * continues with token t at score[b] + logits[b][t] - log sum exp logits[b], in 64 bits; the best come first, among
+ * equals the lower beam, then the lower token. logits: row r = group * n_beams + b at logits + r * stride elements of
+ * dtype (QMH_F32, QMH_F16, QMH_BF16). done (NULL or [rows]): a nonzero row is finished, its one continuation
+ * is token eos at score[b]. Continuations at -inf or NaN are none (a row of score -inf has none: a group's first
+ * step gives its other beams -inf; a row with a NaN or +inf logit has none); places that stay over get score -inf,
+ * parent -1 and token -1. out_*: [n_groups][n_out]; out_parent is b.
+ * n_beams and n_out at most 64, vocab at most 2^24. out_score may be score where n_out = n_beams.
+ * ws: qmh_beam_select_ws(a) bytes (0 for bad arguments), 16-byte aligned, any contents. */
+typedef struct {
+    int32_t dtype, n_groups, n_beams, vocab, n_out, eos;
+    const void *logits;
+    int64_t stride;
+    const float *score;
+    const int32_t *done;
+    float *out_score;
+    int32_t *out_parent, *out_token;
+} qmh_beam_args;
+size_t qmh_beam_select_ws(const qmh_beam_args *a);
+int qmh_beam_select(const qmh_beam_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* The states of surviving beams: dst's sequence j of each group takes src's sequence parent[j] of that group
+ * (parent [n_groups][n_beams] on the device, as qmh_beam_select gives them; outside [0, n_beams): its own).
+ * State of sequence i = group * n_beams + j: n_outer x n_rows pieces of `live` bytes, at outer_stride * o + seq_stride * i +
+ * row_stride * r; bytes between the pieces stay as they are. dst = src moves in place (any parents); otherwise
+ * the two must not overlap, nor may the pieces among themselves. n_beams at most 64. */
+typedef struct {
+    int64_t n_outer, outer_stride, seq_stride, n_rows, row_stride, live;
+} qmh_beam_state;
+int qmh_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const int32_t *parent, int32_t n_groups,
+                     int32_t n_beams, void *stream);
+/* The same for sequences' own pages, in place: positions below len[parent] of the parent's pages go to the
+ * same positions of the sequence's own (table [n_groups * n_beams][table_stride], len on the device, at most
+ * max_len, a longer one counts as max_len). Tables and lengths stay (beams of a group are usually equally long; a
+ * program that keeps them otherwise reorders len with qmh_beam_reorder). A page outside the pool is neither read nor written.
+ * No page may be in two rows of a group's tables. */
+int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t table_stride, const int32_t *len,
+                      int32_t max_len, const int32_t *parent, int32_t n_groups, int32_t n_beams, void *stream);
 
 /* ------------------------------------------------------------------ model level (host arguments) */
 

@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(_HERE, "libqmhip.so")
 INCLUDE = os.path.join(os.path.dirname(_HERE), "include", "qmhip.h")
 
 F32, Q8_0, Q4_0 = 0, 2, 3
+F16, BF16 = 1, 4  # rows, pages and logits of the ops for several continuations of one prompt
 DTYPES = {"f32": F32, "q8_0": Q8_0, "q4_0": Q4_0}
 
 
@@ -38,6 +39,54 @@ class TensorView(ctypes.Structure):
 
     _fields_ = [("dtype", ctypes.c_int32), ("ndim", ctypes.c_int32), ("ne", ctypes.c_int64 * 4),
                 ("data", ctypes.c_void_p)]
+
+
+def _fields(**kinds):
+    """ctypes fields from names by kind: p pointers, i int32, l int64, f float."""
+    c = {"p": ctypes.c_void_p, "i": ctypes.c_int32, "l": ctypes.c_int64, "f": ctypes.c_float}
+    return [(name, c[kind[0]]) for kind, names in kinds.items() for name in names.split()]
+
+
+class Pages(ctypes.Structure):
+    """qmh_pages: keys and values in pages on the device."""
+
+    _fields_ = _fields(i="dtype n_kv_heads head_dim page_size", l="n_pages", p="k v")
+
+
+class RotaryConfig(ctypes.Structure):
+    """qmh_rotary_config."""
+
+    _fields_ = _fields(i="rot_dim layout scaling max_pos first_len", f="theta factor low high magnitude")
+
+
+class AppendArgs(ctypes.Structure):
+    """qmh_append_args."""
+
+    _fields_ = ([("pages", ctypes.POINTER(Pages))] +
+                _fields(p="rotary", i="n_tokens n_heads", p1="q", l="q_stride", p2="q_out", l1="q_out_stride", p3="k",
+                        l2="k_stride", p4="v", l3="v_stride", p5="q_gain k_gain", f="eps", i1="n_seq", p6="table",
+                        i2="table_stride", p7="seq slot pos"))
+
+
+class AttentionArgs(ctypes.Structure):
+    """qmh_attention_args."""
+
+    _fields_ = ([("pages", ctypes.POINTER(Pages))] +
+                _fields(i="n_heads n_seq q_len n_groups", p="q", l="q_stride", p1="out", l1="out_stride", p2="table len",
+                        i1="table_stride max_len", p3="prefix_table prefix_len", i2="prefix_stride max_prefix", f="scale"))
+
+
+class BeamArgs(ctypes.Structure):
+    """qmh_beam_args."""
+
+    _fields_ = _fields(i="dtype n_groups n_beams vocab n_out eos", p="logits", l="stride",
+                       p1="score done out_score out_parent out_token")
+
+
+class BeamState(ctypes.Structure):
+    """qmh_beam_state."""
+
+    _fields_ = _fields(l="n_outer outer_stride seq_stride n_rows row_stride live")
 
 
 _lib = None
@@ -85,6 +134,15 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "qmh_rope": (ctypes.c_int, [vp, i64, i64, i64, f32, vp]),
         "qmh_swiglu": (ctypes.c_int, [vp, vp, i64, vp]),
         "qmh_argmax": (ctypes.c_int, [vp, i32, vp, vp]),
+        "qmh_rotary_create": (vp, [ctypes.POINTER(RotaryConfig)]),
+        "qmh_rotary_free": (None, [vp]),
+        "qmh_paged_append": (ctypes.c_int, [ctypes.POINTER(AppendArgs), vp]),
+        "qmh_paged_attention_ws": (sz, [ctypes.POINTER(AttentionArgs)]),
+        "qmh_paged_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), vp, sz, vp]),
+        "qmh_beam_select_ws": (sz, [ctypes.POINTER(BeamArgs)]),
+        "qmh_beam_select": (ctypes.c_int, [ctypes.POINTER(BeamArgs), vp, sz, vp]),
+        "qmh_beam_reorder": (ctypes.c_int, [ctypes.POINTER(BeamState), vp, vp, vp, i32, i32, vp]),
+        "qmh_paged_reorder": (ctypes.c_int, [ctypes.POINTER(Pages), vp, i32, vp, i32, vp, i32, i32, vp]),
         "qmh_model_create": (vp, [ctypes.POINTER(QmhConfig), ctypes.POINTER(TensorView), ctypes.POINTER(TensorView),
                                   ctypes.POINTER(TensorView), ctypes.POINTER(TensorView)]),
         "qmh_model_load": (vp, [ctypes.c_char_p, i32]),
@@ -195,6 +253,41 @@ class DeviceBuffer:
 
 def sync():
     _check(load_library().qmh_sync(), "qmh_sync")
+
+
+# ----------------------------------------------------------------------------- rotary positions
+
+class Rotary:
+    """The rotation of queries and keys that qmh_paged_append applies (qmh_rotary_create); pass its `handle`."""
+
+    LAYOUTS = {"pairs": 0, "halves": 1}
+    SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
+
+    def __init__(self, rot_dim: int, layout: str = "pairs", scaling: str = "none", max_pos: int = 131072,
+                 theta: float = 10000.0, factor: float = 1.0, low: float = 1.0, high: float = 4.0, first_len: int = 8192,
+                 magnitude: float = 1.0):
+        cfg = RotaryConfig(rot_dim, self.LAYOUTS[layout], self.SCALINGS[scaling], max_pos, first_len, theta, factor, low, high,
+                           magnitude)
+        self.handle = load_library().qmh_rotary_create(ctypes.byref(cfg))
+        if not self.handle:
+            raise QmhError(f"qmh_rotary_create: {last_error()}")
+
+    def close(self):
+        if getattr(self, "handle", None):
+            load_library().qmh_rotary_free(self.handle)
+            self.handle = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 # ----------------------------------------------------------------------------- model

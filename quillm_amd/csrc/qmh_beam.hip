@@ -1,0 +1,357 @@
+// gfx950 kernels of a beam search: qmh_beam_select (the best continuations over beams and vocabulary) and
+// qmh_beam_reorder (the surviving beams' dense states). No reference counterpart.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "qmh_device.h"
+#include "qmh_launch.h"
+#include "qmh_types.h"
+
+namespace {
+
+// --------------------------------------------------------------------------- select
+
+constexpr int SEL_T = 256;   // threads
+constexpr int SEL_CAP = 512; // candidates ranked in LDS
+
+// e^x in 64 bits for x <= 0 (and 0 far below): 2^k times the Taylor polynomial of 2^f, |f| <= 1/2, to degree 10,
+// whose remainder is below (ln 2 / 2)^11 / 11! = 2.2e-13 of the value: far inside the distance of scores that
+// decide a choice, at 10 multiply-adds.
+__device__ __forceinline__ double exp_neg(double x) {
+    double t = x * 1.4426950408889634074;
+    t = t < -1074.0 ? -1074.0 : t; // NaN stays
+    const double k = __builtin_rint(t), f = t - k;
+    double p = 7.0549116208011233299e-9;
+    p = __builtin_fma(p, f, 1.0178086009239699728e-7);
+    p = __builtin_fma(p, f, 1.3215486790144309488e-6);
+    p = __builtin_fma(p, f, 1.5252733804059840280e-5);
+    p = __builtin_fma(p, f, 1.5403530393381609954e-4);
+    p = __builtin_fma(p, f, 1.3333558146428443423e-3);
+    p = __builtin_fma(p, f, 9.6181291076284771619e-3);
+    p = __builtin_fma(p, f, 5.5504108664821579953e-2);
+    p = __builtin_fma(p, f, 2.4022650695910071233e-1);
+    p = __builtin_fma(p, f, 6.9314718055994530942e-1);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)k);
+}
+
+// the order of floats as unsigned numbers, -0 as 0; 0 for -inf and NaN, which are no continuations
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return x > -__builtin_inff() ? u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u) : 0u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((k >> 31) ? k ^ 0x80000000u : ~k); }
+
+// the same for doubles
+__device__ __forceinline__ uint64_t key_of_d(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+    return x > -__builtin_inf() ? u ^ ((u >> 63) ? ~0ull : 1ull << 63) : 0ull;
+}
+__device__ __forceinline__ double of_key_d(uint64_t k) {
+    return __longlong_as_double((long long)((k >> 63) ? k ^ (1ull << 63) : ~k));
+}
+
+// the sum of n over the workgroup
+__device__ __forceinline__ int block_total(int n, int *buf) {
+    for (int s = 1; s < 64; s <<= 1) n += __shfl_xor(n, s);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = n;
+    __syncthreads();
+    return buf[0] + buf[1] + buf[2] + buf[3];
+}
+
+struct scan_out { // of one chunk of one row
+    double sum;   // sum exp(x - max)
+    float max;
+    int count; // candidates that follow, best first
+};
+
+// Chunk blockIdx.x (SEL_T * EPT logits) of row blockIdx.y: its maximum, the sum of exponentials below it in 64 bits, and
+// its n_out best logits in order. The logits stay in registers. A bound below which nothing is among the best
+// is the n_out-th largest of the threads' own maxima; what reaches it (a few more than n_out, unless values repeat)
+// is ranked by counting. Where more than SEL_CAP reach it, the exact bound is searched bit by bit.
+template <typename T, int EPT, int VEC>
+__global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_out *heads, uint2 *cands,
+                                                     int row0) {
+    __shared__ uint32_t tmax[SEL_T];
+    __shared__ uint2 cand[SEL_CAP];
+    __shared__ double red[4];
+    __shared__ float redf[4];
+    __shared__ int cnt[4], ncand;
+    __shared__ uint32_t bound;
+    const int tid = threadIdx.x, row = row0 + blockIdx.y, n_out = a.n_out;
+    const int64_t slot = (int64_t)row * gridDim.x + blockIdx.x;
+    if ((a.done && a.done[row]) || !(a.score[row] > -__builtin_inff())) return; // the join does not look at it
+    const T *x = (const T *)a.logits + row * a.stride;
+    // vectors from the row's start rounded down to a vector: the ones that hold some element of the row
+    const int skew = VEC > 1 ? (int)(((uintptr_t)x / sizeof(T)) % VEC) : 0;
+    const int base = (int)blockIdx.x * SEL_T * EPT - skew;
+    uint32_t key[EPT];
+    float top = -__builtin_inff();
+    float xs[EPT];
+#pragma unroll
+    for (int k = 0; k < EPT / VEC; k++) {
+        const int i = base + (k * SEL_T + tid) * VEC;
+        qmh_vec<T, VEC> v;
+        const bool some = i + VEC > 0 && i < a.vocab;
+        if (some) v = *(const qmh_vec<T, VEC> *)(x + i);
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            xs[k * VEC + e] = some && i + e >= 0 && i + e < a.vocab ? qmh_to_f(v.e[e]) : -__builtin_inff();
+    }
+#pragma unroll
+    for (int k = 0; k < EPT; k++) top = fmaxf(top, xs[k]);
+    const float m = qmh_block_max(top, redf);
+    const float ref = m == -__builtin_inff() ? 0.0f : m;
+    double sum = 0.0;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < EPT; k++) {
+        sum += exp_neg((double)xs[k] - (double)ref); // NaN where x is NaN or +inf: the row then has no continuation
+        key[k] = key_of(xs[k]);
+        mine = key[k] > mine ? key[k] : mine;
+    }
+    sum = qmh_block_sum_d(sum, red);
+    auto index = [&](int k) { return base + ((k / VEC) * SEL_T + tid) * VEC + k % VEC; };
+    // the n_out-th largest of the threads' maxima (0: fewer have one)
+    tmax[tid] = mine;
+    if (tid == 0) ncand = 0;
+    __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < SEL_T; i++) rank += tmax[i] > mine || (tmax[i] == mine && i < tid);
+    if (rank == n_out - 1) bound = mine;
+    __syncthreads();
+    uint32_t from = bound ? bound : 1u;
+    int reach = 0;
+#pragma unroll
+    for (int k = 0; k < EPT; k++) reach += key[k] >= from;
+    int last = 0x7fffffff; // candidates equal to the bound: only up to this index
+    if (block_total(reach, cnt) > SEL_CAP) {
+        // the largest bound that n_out keys reach, then the lowest indexes among the keys equal to it
+        from = 0;
+        for (int b = 31; b >= 0; b--) {
+            const uint32_t t = from | 1u << b;
+            int n = 0;
+#pragma unroll
+            for (int k = 0; k < EPT; k++) n += key[k] >= t;
+            if (block_total(n, cnt) >= n_out) from = t;
+        }
+        int above = 0;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) above += key[k] > from;
+        above = block_total(above, cnt);
+        int lo = -1; // the largest index that leaves fewer than n_out
+        for (int b = 24; b >= 0; b--) {
+            const int t = lo + (1 << b);
+            int n = 0;
+#pragma unroll
+            for (int k = 0; k < EPT; k++) n += key[k] == from && index(k) <= t;
+            if (above + block_total(n, cnt) < n_out) lo = t;
+        }
+        last = lo + 1;
+    }
+#pragma unroll
+    for (int k = 0; k < EPT; k++)
+        if (key[k] > from || (key[k] == from && index(k) <= last)) cand[atomicAdd(&ncand, 1)] = make_uint2(key[k], (uint32_t)index(k));
+    __syncthreads();
+    const int n = ncand;
+    for (int c = tid; c < n; c += SEL_T) {
+        const uint2 v = cand[c];
+        int r = 0;
+        for (int i = 0; i < n; i++) r += cand[i].x > v.x || (cand[i].x == v.x && cand[i].y < v.y);
+        if (r < n_out) cands[slot * n_out + r] = v;
+    }
+    if (tid == 0) heads[slot] = scan_out{sum, m, n < n_out ? n : n_out};
+}
+
+// A group's choice from its rows' chunks: each row's log sum, then the n_out best totals, found one after another.
+__global__ __launch_bounds__(SEL_T) void k_beam_join(const qmh_beam_args a, const scan_out *heads, const uint2 *cands,
+                                                     int chunks) {
+    __shared__ double lse[64];
+    __shared__ uint64_t bk[4], chosen[64];
+    __shared__ uint32_t bf[4], where[64];
+    const int g = blockIdx.x, tid = threadIdx.x, K = a.n_beams, n_out = a.n_out;
+    auto alive = [&](int row) { return !(a.done && a.done[row]) && a.score[row] > -__builtin_inff(); };
+    for (int b = tid; b < K; b += SEL_T) {
+        const int row = g * K + b;
+        double s = __builtin_nan(""), m = 0.0;
+        if (alive(row)) {
+            const scan_out *h = heads + (int64_t)row * chunks;
+            float top = -__builtin_inff();
+            for (int c = 0; c < chunks; c++) top = fmaxf(top, h[c].max);
+            if (top > -__builtin_inff()) {
+                m = (double)top;
+                s = 0.0;
+                for (int c = 0; c < chunks; c++)
+                    if (h[c].max > -__builtin_inff() || h[c].sum != h[c].sum) s += h[c].sum * exp((double)h[c].max - m);
+            }
+        }
+        lse[b] = m + log(s);
+    }
+    __syncthreads();
+    uint64_t below = ~0ull; // what was chosen last: its total, then its place
+    int64_t place = -1;
+    for (int o = 0; o < n_out; o++) {
+        uint64_t best = 0;
+        uint32_t at = 0xffffffffu; // beam * vocab + token
+        auto offer = [&](double total, uint32_t p) {
+            const uint64_t k = key_of_d(total);
+            if (!k || k > below || (k == below && (int64_t)p <= place)) return;
+            if (k > best || (k == best && p < at)) {
+                best = k;
+                at = p;
+            }
+        };
+        const int per = chunks * n_out;
+        for (int i = tid; i < K * per; i += SEL_T) {
+            const int b = i / per, row = g * K + b;
+            if (!alive(row)) continue;
+            const int c = (i - b * per) / n_out, r = i % n_out;
+            if (r >= heads[(int64_t)row * chunks + c].count) continue;
+            const uint2 v = cands[((int64_t)row * chunks + c) * n_out + r];
+            offer((double)a.score[row] + ((double)of_key(v.x) - lse[b]), (uint32_t)(b * a.vocab) + v.y);
+        }
+        for (int b = tid; b < K; b += SEL_T)
+            if (a.done && a.done[g * K + b]) offer((double)a.score[g * K + b], (uint32_t)(b * a.vocab + a.eos));
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint64_t ok = __shfl_xor((unsigned long long)best, s);
+            const uint32_t op = __shfl_xor(at, s);
+            if (ok > best || (ok == best && op < at)) {
+                best = ok;
+                at = op;
+            }
+        }
+        __syncthreads();
+        if ((tid & 63) == 0) {
+            bk[tid >> 6] = best;
+            bf[tid >> 6] = at;
+        }
+        __syncthreads();
+        for (int w = 0; w < 4; w++)
+            if (bk[w] > best || (bk[w] == best && bf[w] < at)) {
+                best = bk[w];
+                at = bf[w];
+            }
+        below = best;
+        place = at;
+        if (tid == 0) {
+            chosen[o] = best;
+            where[o] = at;
+        }
+    }
+    __syncthreads(); // every score has been read: out_score may be score
+    if (tid < n_out) {
+        const uint64_t k = chosen[tid];
+        const int64_t o = (int64_t)g * n_out + tid;
+        a.out_score[o] = k ? (float)of_key_d(k) : -__builtin_inff();
+        a.out_parent[o] = k ? (int)(where[tid] / (uint32_t)a.vocab) : -1;
+        a.out_token[o] = k ? (int)(where[tid] % (uint32_t)a.vocab) : -1;
+    }
+}
+
+int scan_chunks(const qmh_beam_args *a, int ept) { return (a->vocab + 15 + SEL_T * ept - 1) / (SEL_T * ept); }
+// elements a thread holds: 8 spreads few rows over more workgroups, 32 leaves fewer candidates to the join
+int scan_ept(const qmh_beam_args *a) { return (int64_t)a->n_groups * a->n_beams * scan_chunks(a, 8) <= 1024 ? 8 : 32; }
+
+// --------------------------------------------------------------------------- reorder
+
+// V-sized pieces at `off` of every beam of a group that takes another's state: all are read before any is
+// written, so any parents move in place. own: beams without a parent keep (and out of place: take) their own.
+template <typename V, int BM>
+__device__ __forceinline__ void move_beams(uint8_t *dst, const uint8_t *src, const int32_t *par, int K, int64_t seq_stride,
+                                           int64_t off) {
+    V v[BM];
+#pragma unroll
+    for (int j = 0; j < BM; j++) {
+        if (j >= K) break;
+        const int p = par[j], from = p >= 0 && p < K ? p : j;
+        if (from != j || dst != src) v[j] = *(const V *)(src + from * seq_stride + off);
+    }
+#pragma unroll
+    for (int j = 0; j < BM; j++) {
+        if (j >= K) break;
+        const int p = par[j], from = p >= 0 && p < K ? p : j;
+        if (from != j || dst != src) *(V *)(dst + j * seq_stride + off) = v[j];
+    }
+}
+
+// Thread: one unit of U (the widest that every row is aligned to) of one row, for all beams of a group.
+template <typename U, int BM>
+__global__ __launch_bounds__(256) void k_beam_reorder(const qmh_beam_state s, uint8_t *dst, const uint8_t *src,
+                                                      const int32_t *__restrict__ parent, int n_groups, int K, uint32_t row_units,
+                                                      uint32_t blocks_per) {
+    const uint32_t og = blockIdx.x / blocks_per, ub = blockIdx.x - og * blocks_per;
+    const uint32_t o = og / (uint32_t)n_groups, g = og - o * n_groups;
+    const uint32_t u = ub * 256 + threadIdx.x, r = u / row_units, c = u - r * row_units;
+    if (r >= s.n_rows) return;
+    const int64_t base = o * s.outer_stride + (int64_t)g * K * s.seq_stride, row = base + r * s.row_stride;
+    const int32_t *par = parent + g * K;
+    int64_t at = (int64_t)c * sizeof(U);
+    if (at + (int64_t)sizeof(U) <= s.live) {
+        move_beams<U, BM>(dst, src, par, K, s.seq_stride, row + at);
+        return;
+    }
+    while (at < s.live) { // the row's end
+        if (sizeof(U) >= 4 && at + 4 <= s.live) {
+            move_beams<uint32_t, BM>(dst, src, par, K, s.seq_stride, row + at);
+            at += 4;
+        } else {
+            move_beams<uint8_t, BM>(dst, src, par, K, s.seq_stride, row + at);
+            at++;
+        }
+    }
+}
+
+} // namespace
+
+extern "C" size_t qmh_beam_ws_bytes(const qmh_beam_args *a) {
+    const size_t slots = (size_t)a->n_groups * a->n_beams * scan_chunks(a, scan_ept(a));
+    return slots * (sizeof(scan_out) + a->n_out * sizeof(uint2));
+}
+
+extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    const int rows = a->n_groups * a->n_beams, ept = scan_ept(a), chunks = scan_chunks(a, ept);
+    scan_out *heads = (scan_out *)ws;
+    uint2 *cands = (uint2 *)(heads + (size_t)rows * chunks);
+    qmh_for_type(a->dtype, [&](auto z) {
+        using T = decltype(z);
+        constexpr int VEC = 16 / sizeof(T);
+        // rows over y in passes of at most 65535
+        for (int r0 = 0; r0 < rows; r0 += 65535) {
+            const dim3 g(chunks, rows - r0 < 65535 ? rows - r0 : 65535), t(SEL_T);
+            if (ept == 8) hipLaunchKernelGGL((k_beam_scan<T, 8, VEC>), g, t, 0, st, *a, heads, cands, r0);
+            else hipLaunchKernelGGL((k_beam_scan<T, 32, VEC>), g, t, 0, st, *a, heads, cands, r0);
+        }
+    });
+    hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(SEL_T), 0, st, *a, heads, cands, chunks);
+    return (int)hipGetLastError();
+}
+
+template <typename U>
+static int reorder_as(const qmh_beam_state *s, void *dst, const void *src, const int32_t *parent, int n_groups, int K,
+                      hipStream_t st) {
+    const int64_t row_units = (s->live + (int64_t)sizeof(U) - 1) / (int64_t)sizeof(U), units = row_units * s->n_rows;
+    const int64_t per = (units + 255) / 256, blocks = per * n_groups * s->n_outer;
+    if (row_units > 0x7fffffff || units > 0x7fffff00 || blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+    const dim3 g((uint32_t)blocks), t(256);
+    uint8_t *d = (uint8_t *)dst;
+    const uint8_t *f = (const uint8_t *)src;
+    const uint32_t ru = (uint32_t)row_units, p = (uint32_t)per;
+    if (K <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 4>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
+    else if (K <= 8) hipLaunchKernelGGL((k_beam_reorder<U, 8>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
+    else if (K <= 16) hipLaunchKernelGGL((k_beam_reorder<U, 16>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
+    else if constexpr (sizeof(U) <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 64>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
+    return (int)hipGetLastError();
+}
+
+extern "C" int qmh_launch_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const int32_t *parent, int n_groups,
+                                       int n_beams, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    const uint64_t all = (uint64_t)(uintptr_t)dst | (uint64_t)(uintptr_t)src | (uint64_t)s->seq_stride |
+                         (s->n_outer > 1 ? (uint64_t)s->outer_stride : 0) | (s->n_rows > 1 ? (uint64_t)s->row_stride : 0);
+    // past 16 beams a thread's units of all beams take 4 bytes each, so that they stay in registers
+    if (all % 16 == 0 && n_beams <= 16) return reorder_as<uint4>(s, dst, src, parent, n_groups, n_beams, st);
+    if (all % 4 == 0) return reorder_as<uint32_t>(s, dst, src, parent, n_groups, n_beams, st);
+    return reorder_as<uint8_t>(s, dst, src, parent, n_groups, n_beams, st);
+}

@@ -7,6 +7,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/qmhip.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -230,6 +232,24 @@ int qmh_launch_sample_scratch(qmh_sample_args *a, void *base, void *stream);
 
 /* gate = silu(gate)*up over n (src/ops.c:128-133) */
 int qmh_launch_swiglu(float *gate, const float *up, int64_t n, void *stream);
+
+/* ---- several continuations of one prompt (qmh_paged.hip, qmh_beam.hip): arguments checked by the host code */
+/* rotation tables: position a = 1024 h + l; hi [rows][pairs] and lo [1024][pairs] of (cos, sin) */
+#define QMH_ROTARY_LO 1024
+typedef struct {
+    const double *hi, *lo;
+    int pairs, layout, max_pos;
+} qmh_rotary_tables;
+/* vw: elements per vector access (rot_dim / 2 and (head_dim - rot_dim) / 2 are multiples, all rows aligned) */
+int qmh_launch_paged_append(const qmh_append_args *a, const qmh_rotary_tables *r, int vw, void *stream);
+size_t qmh_attention_ws_bytes(const qmh_attention_args *a, int cus);
+int qmh_launch_paged_attention(const qmh_attention_args *a, int cus, void *ws, void *stream);
+size_t qmh_beam_ws_bytes(const qmh_beam_args *a);
+int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *stream);
+int qmh_launch_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const int32_t *parent, int n_groups,
+                            int n_beams, void *stream);
+int qmh_launch_paged_reorder(const qmh_pages *p, const int32_t *table, int table_stride, const int32_t *len, int max_len,
+                             const int32_t *parent, int n_groups, int n_beams, void *stream);
 
 /* op-level kernels */
 int qmh_launch_h2f(const uint16_t *h, float *f, int64_t n, void *stream);

@@ -207,6 +207,285 @@ int qmh_matmul_nt(const float *A, const float *B, float *C, int64_t M, int64_t N
     return 0;
 }
 
+/* ------------------------------------------------------------------ several continuations of one prompt */
+
+/* the library's device is the calling thread's: a launch from another one would fail or run elsewhere */
+static int on_device(const char *what) {
+    int d = -1;
+    if (ensure()) return -1;
+    HIPCHK(hipGetDevice(&d));
+    if (d != g_dev) return fail("%s: the current device is %d, the library's is %d", what, d, g_dev);
+    return 0;
+}
+static int elem_bytes(int dtype) { return dtype == QMH_F32 ? 4 : dtype == QMH_F16 || dtype == QMH_BF16 ? 2 : 0; }
+static int aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+/* kv: the arrays are used */
+static int check_pages(const qmh_pages *p, int kv, const char *what) {
+    if (!p) return fail("%s: NULL pages", what);
+    if (!elem_bytes(p->dtype)) return fail("%s: bad dtype %d", what, p->dtype);
+    if (p->head_dim < 8 || p->head_dim > 256 || p->head_dim % 8)
+        return fail("%s: head_dim %d is not a multiple of 8 in [8, 256]", what, p->head_dim);
+    if (p->n_kv_heads < 1 || p->n_kv_heads > 1024) return fail("%s: n_kv_heads %d outside [1, 1024]", what, p->n_kv_heads);
+    if (!kv) return 0;
+    if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+        return fail("%s: page_size %d is not a power of two in [16, 1024]", what, p->page_size);
+    if (p->n_pages < 1 || p->n_pages > 0x7fffffff) return fail("%s: n_pages outside [1, 2^31)", what);
+    if (!p->k || !p->v || !aligned(p->k, 16) || !aligned(p->v, 16)) return fail("%s: k, v NULL or not 16-byte aligned", what);
+    return 0;
+}
+
+struct qmh_rotary {
+    qmh_rotary_config cfg;
+    double *d_tab;
+    qmh_rotary_tables t;
+};
+
+void qmh_rotary_free(qmh_rotary *r) {
+    if (!r) return;
+    if (r->d_tab) (void)hipFree(r->d_tab);
+    free(r);
+}
+
+/* radians per position of pair i */
+static double rotary_freq(const qmh_rotary_config *c, int i) {
+    const double r = c->rot_dim, factor = c->factor, len = c->first_len, two_pi = 6.283185307179586476925;
+    double theta = c->theta;
+    if (c->scaling == QMH_ROTARY_NTK) theta *= pow(factor, r / (r - 2.0));
+    const double f = pow(theta, -2.0 * i / r);
+    double w = 1.0;
+    if (c->scaling == QMH_ROTARY_LINEAR) w = 0.0;
+    if (c->scaling == QMH_ROTARY_BANDS) w = (len * f / two_pi - c->low) / ((double)c->high - c->low);
+    if (c->scaling == QMH_ROTARY_YARN) {
+        double a = floor(r * log(len / (two_pi * c->high)) / (2.0 * log(theta)));
+        double b = ceil(r * log(len / (two_pi * c->low)) / (2.0 * log(theta)));
+        a = a > 0.0 ? a : 0.0;
+        b = b < r - 1.0 ? b : r - 1.0;
+        w = 1.0 - (i - a) / (b - a > 0.001 ? b - a : 0.001);
+    }
+    w = w < 0.0 ? 0.0 : w > 1.0 ? 1.0 : w;
+    return w == 1.0 ? f : f * w + f / factor * (1.0 - w);
+}
+
+static int check_rotary(const qmh_rotary_config *c) {
+    if (!c) return fail("rotary: NULL configuration");
+    if (c->rot_dim < 2 || c->rot_dim > 256 || c->rot_dim % 2) return fail("rotary: rot_dim %d is not even in [2, 256]", c->rot_dim);
+    if (c->layout != QMH_ROTARY_PAIRS && c->layout != QMH_ROTARY_HALVES) return fail("rotary: bad layout %d", c->layout);
+    if (c->scaling < QMH_ROTARY_PLAIN || c->scaling > QMH_ROTARY_YARN) return fail("rotary: bad scaling %d", c->scaling);
+    if (c->max_pos < 1 || c->max_pos > 1 << 24) return fail("rotary: max_pos %d outside [1, 2^24]", c->max_pos);
+    if (!(c->theta > 1.0f) || !isfinite(c->theta)) return fail("rotary: theta %g is not above 1", c->theta);
+    if (!isfinite(c->magnitude)) return fail("rotary: magnitude is not finite");
+    if (c->scaling != QMH_ROTARY_PLAIN && (!(c->factor > 0.0f) || !isfinite(c->factor))) return fail("rotary: bad factor %g", c->factor);
+    if (c->scaling == QMH_ROTARY_NTK && c->rot_dim == 2) return fail("rotary: this scaling needs rot_dim > 2");
+    if (c->scaling >= QMH_ROTARY_BANDS && (c->first_len < 1 || !(c->low > 0.0f) || !(c->high > c->low) || !isfinite(c->high)))
+        return fail("rotary: needs first_len > 0 and 0 < low < high");
+    return 0;
+}
+
+static int rotary_build(qmh_rotary *r, const qmh_rotary_config *c) {
+    const int np = c->rot_dim / 2, nh = (c->max_pos + QMH_ROTARY_LO - 1) / QMH_ROTARY_LO;
+    const size_t n = (size_t)(nh + QMH_ROTARY_LO) * np * 2;
+    double *h = malloc(n * sizeof(double));
+    if (!h) return fail("rotary: out of host memory");
+    for (int i = 0; i < np; i++) {
+        const double f = rotary_freq(c, i);
+        for (int a = 0; a < nh; a++) { /* the magnitude rides on one of the two factors */
+            const double ang = (double)a * QMH_ROTARY_LO * f;
+            h[2 * ((size_t)a * np + i)] = cos(ang) * c->magnitude;
+            h[2 * ((size_t)a * np + i) + 1] = sin(ang) * c->magnitude;
+        }
+        for (int l = 0; l < QMH_ROTARY_LO; l++) {
+            h[2 * ((size_t)(nh + l) * np + i)] = cos(l * f);
+            h[2 * ((size_t)(nh + l) * np + i) + 1] = sin(l * f);
+        }
+    }
+    hipError_t e = hipMalloc((void **)&r->d_tab, n * sizeof(double));
+    if (e == hipSuccess) e = hipMemcpyAsync(r->d_tab, h, n * sizeof(double), hipMemcpyHostToDevice, g_stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
+    free(h);
+    if (e != hipSuccess) return fail("rotary: %s", hipGetErrorString(e));
+    r->cfg = *c;
+    r->t.hi = r->d_tab;
+    r->t.lo = r->d_tab + (size_t)nh * np * 2;
+    r->t.pairs = np;
+    r->t.layout = c->layout;
+    r->t.max_pos = c->max_pos;
+    return 0;
+}
+
+qmh_rotary *qmh_rotary_create(const qmh_rotary_config *cfg) {
+    if (check_rotary(cfg) || on_device("rotary")) return NULL;
+    qmh_rotary *r = calloc(1, sizeof *r);
+    if (!r) {
+        fail("rotary: out of host memory");
+        return NULL;
+    }
+    if (rotary_build(r, cfg)) {
+        qmh_rotary_free(r);
+        return NULL;
+    }
+    return r;
+}
+
+/* a row array of the ops below: present, aligned to its elements, rows that do not overlap (n: elements a row) */
+static int check_rows(const char *what, const char *name, const void *p, int64_t stride, int64_t n, int es) {
+    if (!p) return fail("%s: NULL %s", what, name);
+    if (!aligned(p, (size_t)es)) return fail("%s: %s is not aligned to its elements", what, name);
+    if (stride < n || stride > (int64_t)1 << 40) return fail("%s: %s's rows of %lld elements overlap (stride %lld)", what, name, (long long)n, (long long)stride);
+    return 0;
+}
+
+int qmh_paged_append(const qmh_append_args *a, void *stream) {
+    static const char *me = "paged_append";
+    if (!a) return fail("%s: NULL arguments", me);
+    const int kv = a->k || a->v;
+    if (check_pages(a->pages, kv, me)) return -1;
+    const qmh_pages *p = a->pages;
+    const int es = elem_bytes(p->dtype), hd = p->head_dim;
+    if (a->n_tokens < 0) return fail("%s: n_tokens %d", me, a->n_tokens);
+    if (!a->q && !a->q_out && !kv) return fail("%s: neither queries nor keys and values", me);
+    if (a->q || a->q_out) {
+        if (a->n_heads < 1 || a->n_heads > 4096) return fail("%s: n_heads %d outside [1, 4096]", me, a->n_heads);
+        if (check_rows(me, "q", a->q, a->q_stride, (int64_t)a->n_heads * hd, es)) return -1;
+        if (check_rows(me, "q_out", a->q_out, a->q_out_stride, (int64_t)a->n_heads * hd, es)) return -1;
+        if (a->q_out == a->q && a->q_out_stride != a->q_stride) return fail("%s: q_out = q needs the same stride", me);
+    }
+    if (kv) {
+        if (check_rows(me, "k", a->k, a->k_stride, (int64_t)p->n_kv_heads * hd, es)) return -1;
+        if (check_rows(me, "v", a->v, a->v_stride, (int64_t)p->n_kv_heads * hd, es)) return -1;
+        if (!a->table || !a->seq || !a->slot) return fail("%s: NULL table, seq or slot", me);
+        if (a->n_seq < 1 || a->table_stride < 1) return fail("%s: a table of %d x %d", me, a->n_seq, a->table_stride);
+        if ((int64_t)a->table_stride * p->page_size > 0x7fffffff) return fail("%s: a table row of 2^31 positions", me);
+    }
+    const qmh_rotary *r = a->rotary;
+    if (r && !a->pos && !a->slot) return fail("%s: a rotation needs pos or slot", me);
+    if (r && r->cfg.rot_dim > hd) return fail("%s: rot_dim %d of a head of %d", me, r->cfg.rot_dim, hd);
+    if ((a->q_gain || a->k_gain) && !(a->eps >= 0.0f)) return fail("%s: eps %g", me, a->eps);
+    if (on_device(me)) return -1;
+    if (a->n_tokens == 0) return 0;
+    /* elements a vector access takes: both halves of the rotated part and of the rest divide into them, and every
+     * row starts at a multiple of them */
+    int vw = 16 / es;
+    const int half = r ? r->cfg.rot_dim / 2 : 0;
+    for (; vw > 1; vw >>= 1) {
+        const size_t b = (size_t)vw * es;
+        if (half % vw || (hd / 2 - half) % vw) continue;
+        if (a->q && (!aligned(a->q, b) || !aligned(a->q_out, b) || a->q_stride % vw || a->q_out_stride % vw)) continue;
+        if (kv && (!aligned(a->k, b) || !aligned(a->v, b) || a->k_stride % vw || a->v_stride % vw)) continue;
+        break;
+    }
+    LCHK(qmh_launch_paged_append(a, r ? &r->t : NULL, vw, S(stream)));
+    return 0;
+}
+
+static int check_attention(const qmh_attention_args *a, const char *me) {
+    if (!a) return fail("%s: NULL arguments", me);
+    if (check_pages(a->pages, 1, me)) return -1;
+    const qmh_pages *p = a->pages;
+    if (a->n_heads < 1 || a->n_heads > 4096 || a->n_heads % p->n_kv_heads)
+        return fail("%s: n_heads %d is not a multiple of n_kv_heads %d up to 4096", me, a->n_heads, p->n_kv_heads);
+    if (a->n_seq < 0 || a->q_len < 1 || (int64_t)a->n_seq * a->q_len > 1 << 20)
+        return fail("%s: %d sequences of %d queries (at most 2^20)", me, a->n_seq, a->q_len);
+    if (a->n_groups < 1 || (a->n_seq && a->n_seq % a->n_groups))
+        return fail("%s: %d sequences in %d groups", me, a->n_seq, a->n_groups);
+    const int64_t n = (int64_t)a->n_heads * p->head_dim;
+    /* 16-byte loads: every row starts at a multiple of 16 bytes */
+    const int es = elem_bytes(p->dtype), vw = 16 / es;
+    if (check_rows(me, "q", a->q, a->q_stride, n, es) || check_rows(me, "out", a->out, a->out_stride, n, es)) return -1;
+    if (!aligned(a->q, 16) || !aligned(a->out, 16) || a->q_stride % vw || a->out_stride % vw)
+        return fail("%s: rows of q and out must start at multiples of 16 bytes", me);
+    if (a->max_len < 0 || a->max_prefix < 0) return fail("%s: max_len %d, max_prefix %d", me, a->max_len, a->max_prefix);
+    if (a->max_len && (!a->table || !a->len || a->max_len > (int64_t)a->table_stride * p->page_size))
+        return fail("%s: max_len %d needs len and a table of that many positions", me, a->max_len);
+    if (a->max_prefix && (!a->prefix_table || !a->prefix_len || a->max_prefix > (int64_t)a->prefix_stride * p->page_size))
+        return fail("%s: max_prefix %d needs prefix_len and a table of that many positions", me, a->max_prefix);
+    if (!isfinite(a->scale)) return fail("%s: scale is not finite", me);
+    return 0;
+}
+
+size_t qmh_paged_attention_ws(const qmh_attention_args *a) {
+    if (check_attention(a, "paged_attention_ws") || ensure()) return 0;
+    return qmh_attention_ws_bytes(a, g_cus);
+}
+
+int qmh_paged_attention(const qmh_attention_args *a, void *ws, size_t ws_bytes, void *stream) {
+    static const char *me = "paged_attention";
+    if (check_attention(a, me) || on_device(me)) return -1;
+    if (a->n_seq == 0) return 0;
+    const size_t need = qmh_attention_ws_bytes(a, g_cus);
+    if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
+        return fail("%s: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", me, need, ws ? ws_bytes : 0);
+    LCHK(qmh_launch_paged_attention(a, g_cus, ws, S(stream)));
+    return 0;
+}
+
+static int check_beam(const qmh_beam_args *a, const char *me) {
+    if (!a) return fail("%s: NULL arguments", me);
+    const int es = elem_bytes(a->dtype);
+    if (!es) return fail("%s: bad dtype %d", me, a->dtype);
+    if (a->n_groups < 0 || a->n_groups > 65535) return fail("%s: n_groups %d outside [0, 65535]", me, a->n_groups);
+    if (a->n_beams < 1 || a->n_beams > 64) return fail("%s: n_beams %d outside [1, 64]", me, a->n_beams);
+    if (a->n_out < 1 || a->n_out > 64) return fail("%s: n_out %d outside [1, 64]", me, a->n_out);
+    if (a->vocab < 1 || a->vocab > 1 << 24) return fail("%s: vocab %d outside [1, 2^24]", me, a->vocab);
+    if (check_rows(me, "logits", a->logits, a->stride, a->vocab, es)) return -1;
+    if (!a->score || !a->out_score || !a->out_parent || !a->out_token) return fail("%s: NULL score or output", me);
+    if (a->out_score == a->score && a->n_out != a->n_beams) return fail("%s: out_score = score needs n_out = n_beams", me);
+    if (a->done && (a->eos < 0 || a->eos >= a->vocab)) return fail("%s: eos %d outside the vocabulary", me, a->eos);
+    return 0;
+}
+
+size_t qmh_beam_select_ws(const qmh_beam_args *a) {
+    if (check_beam(a, "beam_select_ws")) return 0;
+    return qmh_beam_ws_bytes(a);
+}
+
+int qmh_beam_select(const qmh_beam_args *a, void *ws, size_t ws_bytes, void *stream) {
+    static const char *me = "beam_select";
+    if (check_beam(a, me) || on_device(me)) return -1;
+    if (a->n_groups == 0) return 0;
+    const size_t need = qmh_beam_ws_bytes(a);
+    if (!ws || ws_bytes < need || !aligned(ws, 16))
+        return fail("%s: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", me, need, ws ? ws_bytes : 0);
+    LCHK(qmh_launch_beam_select(a, ws, S(stream)));
+    return 0;
+}
+
+static int check_parents(const char *me, const int32_t *parent, int32_t n_groups, int32_t n_beams) {
+    if (n_groups < 0 || n_groups > 65535) return fail("%s: n_groups %d outside [0, 65535]", me, n_groups);
+    if (n_beams < 1 || n_beams > 64) return fail("%s: n_beams %d outside [1, 64]", me, n_beams);
+    if (!parent) return fail("%s: NULL parent", me);
+    return 0;
+}
+
+int qmh_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const int32_t *parent, int32_t n_groups,
+                     int32_t n_beams, void *stream) {
+    static const char *me = "beam_reorder";
+    if (!s || !dst || !src) return fail("%s: NULL argument", me);
+    if (check_parents(me, parent, n_groups, n_beams)) return -1;
+    const int64_t top = (int64_t)1 << 46;
+    if (s->n_outer < 0 || s->n_rows < 0 || s->live < 0 || s->n_outer > 1 << 24 || s->n_rows > 1 << 30 || s->live > (int64_t)1 << 40 ||
+        s->outer_stride < 0 || s->seq_stride < 0 || s->row_stride < 0 || s->outer_stride > top || s->seq_stride > top || s->row_stride > top)
+        return fail("%s: a size or stride is negative or too large", me);
+    if (s->n_rows > 1 && s->row_stride < s->live) return fail("%s: rows of %lld bytes overlap", me, (long long)s->live);
+    if (on_device(me)) return -1;
+    if (!n_groups || !s->n_outer || !s->n_rows || !s->live) return 0;
+    LCHK(qmh_launch_beam_reorder(s, dst, src, parent, n_groups, n_beams, S(stream)));
+    return 0;
+}
+
+int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t table_stride, const int32_t *len,
+                      int32_t max_len, const int32_t *parent, int32_t n_groups, int32_t n_beams, void *stream) {
+    static const char *me = "paged_reorder";
+    if (check_pages(pages, 1, me) || check_parents(me, parent, n_groups, n_beams)) return -1;
+    if (max_len < 0) return fail("%s: max_len %d", me, max_len);
+    if (max_len && (!table || !len || max_len > (int64_t)table_stride * pages->page_size))
+        return fail("%s: max_len %d needs len and a table of that many positions", me, max_len);
+    if (on_device(me)) return -1;
+    if (!n_groups || !max_len) return 0;
+    LCHK(qmh_launch_paged_reorder(pages, table, table_stride, len, max_len, parent, n_groups, n_beams, S(stream)));
+    return 0;
+}
+
 /* ------------------------------------------------------------------ device weights */
 
 struct qmh_weight {
