@@ -136,60 +136,484 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
 }
 
 // --------------------------------------------------------------------------- attention
+//
+// A wave holds 16 NR rows of queries (a row: one query of one head; rows that share keys lie together: a group's
+// sequences for the prefix, a sequence's queries and the heads of its kv head for its own pages) and walks positions, KS at a time,
+// with the running maximum and sum of a softmax. Both products are MFMAs on registers alone, no LDS:
+//   S^T = K Q^T   16x16 tiles: lane (i = lane & 15, g = lane >> 4) gives row i of K, 16 bytes of each 64; it gets the scores
+//                 of query i at positions 4 g + e
+//   O^T = V^T P^T the probabilities are where the product wants them: its k index is numbered so that lane group g
+//                 holds positions 4 g + e (and 16 + 4 g + e). For V^T a lane loads HDP / 16 neighbouring values of
+//                 the rows it holds, whole rows per 16 lanes, and takes the d-th tile's row i to be d = i HDP / 16 + tile;
+//                 16-bit pairs are turned by byte permutes.
+// Rows behind a list's end are out of the loads' range and read as zero, whatever lies there. The four waves
+// of a workgroup take the steps of one chunk of positions in turn and are joined through LDS; chunks are joined by
+// k_attention_join.
 
-// One wave per (row of queries, head): 64 positions at a time, a lane's score each, then the lanes over head_dim.
-template <typename T>
-__global__ __launch_bounds__(256) void k_paged_attention(const qmh_attention_args a, const qmh_pages p) {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6))), lane = threadIdx.x & 63;
-    const int row = wave / a.n_heads, h = wave - row * a.n_heads;
-    if (row >= a.n_seq * a.q_len) return;
-    const int hd = p.head_dim, ps = p.page_size, KV = p.n_kv_heads, kvh = h / (a.n_heads / KV);
-    const int sq = row / a.q_len, j = row - sq * a.q_len, g = sq / (a.n_seq / a.n_groups);
-    const T *q = (const T *)a.q + row * a.q_stride + h * hd;
-    float m = -__builtin_inff(), l = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    bool bad = false;
-    for (int own = 0; own < 2; own++) {
-        const int most = own ? a.max_len : a.max_prefix;
-        if (!most) continue;
-        const int all = own ? a.len[sq] : a.prefix_len[g];
-        if (all < 0 || all > most) {
-            bad = true;
-            continue;
-        }
-        const int n = own ? all - a.q_len + 1 + j : all;
-        const int32_t *tab = own ? a.table + (int64_t)sq * a.table_stride : a.prefix_table + (int64_t)g * a.prefix_stride;
-        for (int t0 = 0; t0 < n; t0 += 64) {
-            const int t = t0 + lane < n ? t0 + lane : n - 1;
-            int page = tab[t / ps];
-            if (page < 0 || page >= p.n_pages) {
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef qmh_f16 v8h __attribute__((ext_vector_type(8)));
+typedef qmh_f16 v2h __attribute__((ext_vector_type(2)));
+typedef qmh_bf16 v8b __attribute__((ext_vector_type(8)));
+typedef qmh_bf16 v2b __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ v4f mma32(qmh_f16, v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mma32(qmh_bf16, v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+}
+// two floats rounded to nearest into 16 bits each
+__device__ __forceinline__ uint32_t pack2(qmh_f16, float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){x, y}, v2h));
+}
+__device__ __forceinline__ uint32_t pack2(qmh_bf16, float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){x, y}, v2b));
+}
+
+typedef const __attribute__((address_space(4))) int32_t *const_i32; // scalar loads
+__device__ __forceinline__ const_i32 as_const(const int32_t *p) { return (const_i32)(uintptr_t)p; }
+
+// how the work is divided (the same for the workspace's size and the launch)
+struct attn_plan {
+    int joint;       // prefix and own pages in one pass of each sequence, no parts
+    int G;           // heads per kv head
+    int per;         // sequences per group
+    int nrp, nro;    // 16-row tiles of a wave: prefix, own
+    int pt, ps, pc;  // prefix: row tiles, splits, positions of a split
+    int ot, os, oc;  // own
+    int64_t pre_blocks, blocks;
+    int64_t rows;    // all rows of queries (query x head)
+};
+
+struct attn_args {
+    qmh_attention_args a;
+    qmh_pages p;
+    attn_plan n;
+    int lg_ps;
+    float *part; // [parts][rows][head_dim], unnormalised
+    float2 *ml;  // [parts][rows]: maximum and sum
+};
+
+struct attn_list {
+    const int32_t *tab;
+    int own;      // a sequence's own pages: its queries see different numbers of positions
+    int n;        // positions
+    int from, to; // this chunk's; to <= n
+};
+
+template <typename T, int HDP, int NR>
+struct attn_wave {
+    static constexpr bool F = sizeof(T) == 4;
+    static constexpr int KS = F ? 16 : 32;            // positions a step
+    static constexpr int RT = KS / 16;                // 16-row blocks of K a step
+    static constexpr int KC = HDP * (int)sizeof(T) / 64; // 16-byte loads of a K row per lane
+    static constexpr int VE = HDP / 16;               // values of a V row per lane
+    static constexpr int VB = VE * (int)sizeof(T);    // their bytes
+    static constexpr int VW = VB / 4;                 // and words
+    static constexpr int LDS_COL = HDP + 4;
+    static constexpr int LDS_FLOATS = 4 * 16 * NR * LDS_COL + 4 * 16 * NR * 2;
+
+    v4u Q[NR][KC];
+    v4f O[NR][VE];
+    float m[NR], l[NR];
+    int lim[NR];
+    struct step {
+        v4u k[RT][KC];
+        uint32_t v[RT * 4][VW];
+    };
+
+    __device__ __forceinline__ void load(step &x, const attn_args &s, const attn_list &L, int base, int kvh, bool &bad) const {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = s.p.head_dim;
+        const int rb = hd * (int)sizeof(T);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const int at = base + 16 * r, left = L.to - at; // positions from L.to on are nobody's here
+            const int rows = left < 0 ? 0 : left > 16 ? 16 : left;
+            const int safe = rows ? at : 0;
+            int page = rows ? as_const(L.tab)[safe >> s.lg_ps] : 0;
+            if ((uint32_t)page >= (uint64_t)s.p.n_pages) {
                 bad = true;
                 page = 0;
             }
-            const int64_t at = (((int64_t)page * KV + kvh) * ps + t % ps) * hd;
-            const T *k = (const T *)p.k + at;
-            float s = 0.0f;
-            for (int d = 0; d < hd; d++) s = __builtin_fmaf(qmh_to_f(q[d]), qmh_to_f(k[d]), s);
-            s = t0 + lane < n ? s * a.scale : -__builtin_inff();
-            float mn = fmaxf(m, qmh_wave_max(s));
-            const float ref = mn == -__builtin_inff() ? 0.0f : mn;
-            const float e = expf(s - ref), f = expf(m - ref);
-            m = mn;
-            l *= f;
-            for (int i = 0; i < 4; i++) acc[i] *= f;
-            for (int i = 0; i < 64 && t0 + i < n; i++) {
-                const float pi = __shfl(e, i);
-                const int64_t ai = __shfl(at, i);
-                l += pi;
-                for (int c = 0; c < 4; c++)
-                    if (lane + 64 * c < hd) acc[c] = __builtin_fmaf(pi, qmh_to_f(((const T *)p.v)[ai + lane + 64 * c]), acc[c]);
+            page = __builtin_amdgcn_readfirstlane(page);
+            const int64_t off = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (safe & (s.p.page_size - 1))) * rb;
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.k + off, (short)0, rows * rb, 0x00020000);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.v + off, (short)0, rows * rb, 0x00020000);
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const int b = (4 * c + g) * 16;
+                x.k[r][c] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rk, b < rb ? i * rb + b : 0x7ffffff0, 0, 0));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int c = 0; c < (VB + 15) / 16; c++) {
+                    const int b = i * VB + 16 * c, o = b < rb ? (4 * g + e) * rb + b : 0x7ffffff0;
+                    if constexpr (VB >= 16) {
+                        const v4u w = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, 0));
+#pragma unroll
+                        for (int d = 0; d < 4; d++) x.v[4 * r + e][4 * c + d] = w[d];
+                    } else {
+                        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 0);
+                        x.v[4 * r + e][0] = w[0];
+                        x.v[4 * r + e][1] = w[1];
+                    }
+                }
+        }
+    }
+
+    // masked: some row of the tile does not see all of the step
+    __device__ __forceinline__ void use(const step &x, int base, float sc, bool masked) {
+        const int g = (threadIdx.x & 63) >> 4;
+        v4f S[NR][RT];
+#pragma unroll
+        for (int c = 0; c < NR; c++)
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KC; k++) {
+                    if constexpr (F) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[r][k][j]), __uint_as_float(Q[c][k][j]), acc, 0, 0, 0);
+                    } else {
+                        acc = mma32(T{}, x.k[r][k], Q[c][k], acc);
+                    }
+                }
+                S[c][r] = acc;
+            }
+        if (masked) {
+#pragma unroll
+            for (int c = 0; c < NR; c++)
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (base + 16 * r + 4 * g + e >= lim[c]) S[c][r][e] = -__builtin_inff();
+        }
+        // The reference value of a row's exponentials is raised only when a score passes it by 2^8: the sums stay exact
+        // floats either way, and the rescaling of O is rare
+        bool up = false;
+        float mx[NR];
+#pragma unroll
+        for (int c = 0; c < NR; c++) {
+            float v = S[c][0][0];
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) v = fmaxf(v, S[c][r][e]);
+            mx[c] = v;
+            up |= m[c] == -__builtin_inff() ? v > m[c] : (v - m[c]) * sc > 8.0f;
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (int c = 0; c < NR; c++) {
+                float v = mx[c];
+                v = fmaxf(v, __uint_as_float(qmh_xor16_u(__float_as_uint(v))));
+                v = fmaxf(v, __uint_as_float(qmh_xor32_u(__float_as_uint(v))));
+                if (v > m[c]) {
+                    const float f = m[c] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[c] - v) * sc);
+                    m[c] = v;
+                    l[c] *= f;
+#pragma unroll
+                    for (int t = 0; t < VE; t++) O[c][t] = O[c][t] * f;
+                }
+            }
+        }
+        v4u P[NR];   // 16-bit: positions 4 g + e, then 16 + 4 g + e
+#pragma unroll
+        for (int c = 0; c < NR; c++) {
+            const float off = m[c] == -__builtin_inff() ? 0.0f : -m[c] * sc;
+            float pr[4 * RT];
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[c][r][e], sc, off));
+                    if (masked && base + 16 * r + 4 * g + e >= lim[c]) v = 0.0f;
+                    pr[4 * r + e] = v;
+                }
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4 * RT; e++) sum += pr[e];
+            l[c] += sum;
+            if constexpr (F) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) P[c][e] = __float_as_uint(pr[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) P[c][e] = pack2(T{}, pr[(2 * e) % (4 * RT)], pr[(2 * e + 1) % (4 * RT)]);
+            }
+        }
+        if constexpr (F) {
+#pragma unroll
+            for (int t = 0; t < VE; t++)
+#pragma unroll
+                for (int c = 0; c < NR; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        O[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[e][t]), __uint_as_float(P[c][e]), O[c][t], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int u = 0; u < VW; u++) {
+                v4u lo, hi; // tiles 2 u and 2 u + 1
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t a = x.v[(2 * j) % (4 * RT)][u], b = x.v[(2 * j + 1) % (4 * RT)][u];
+                    lo[j] = __builtin_amdgcn_perm(b, a, 0x05040100);
+                    hi[j] = __builtin_amdgcn_perm(b, a, 0x07060302);
+                }
+#pragma unroll
+                for (int c = 0; c < NR; c++) {
+                    O[c][(2 * u) % VE] = mma32(T{}, lo, P[c], O[c][(2 * u) % VE]);
+                    O[c][(2 * u + 1) % VE] = mma32(T{}, hi, P[c], O[c][(2 * u + 1) % VE]);
+                }
             }
         }
     }
-    if (__any(bad)) l = __builtin_nanf("");
+
+    // this wave's steps of the list's chunk; full: positions that every row sees
+    __device__ __forceinline__ void walk(const attn_args &s, const attn_list &L, int kvh, float sc, int full, bool &bad) {
+        const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        int base = L.from + w * KS;
+        if (base >= L.to) return;
+        step A, B;
+        load(A, s, L, base, kvh, bad);
+        for (;;) {
+            load(B, s, L, base + 4 * KS, kvh, bad);
+            use(A, base, sc, base + KS > full);
+            base += 4 * KS;
+            if (base >= L.to) break;
+            load(A, s, L, base + 4 * KS, kvh, bad);
+            use(B, base, sc, base + KS > full);
+            base += 4 * KS;
+            if (base >= L.to) break;
+        }
+    }
+};
+
+// Rows [row0, row0 + 16 NR) of the R that share a kv head's keys: row r is token t0 + r / G, head r % G of it. They see
+// the chunk of the shared prefix and then the chunk of own pages. part < 0: the result goes out, else it is part `part`.
+template <typename T, int HDP, int NR>
+__device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0, int R, int t0, int kvh, const attn_list &shared,
+                                       const attn_list &own, bool bad, int part) {
+    using W = attn_wave<T, HDP, NR>;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, G = s.n.G, hd = s.p.head_dim;
+    const int H = s.a.n_heads, h0 = kvh * G;
+    const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f; // exponentials are powers of two
+    W x;
+#pragma unroll
+    for (int c = 0; c < NR; c++) {
+        int r = row0 + 16 * c + i;
+        r = r < R ? r : R - 1; // rows past the last are computed with its queries and not written
+        const T *q = (const T *)s.a.q + (int64_t)(t0 + r / G) * s.a.q_stride + (int64_t)(h0 + r % G) * hd;
+        const uint32_t flip = s.a.scale < 0.0f ? (W::F ? 0x80000000u : 0x80008000u) : 0u; // the scale's sign
+#pragma unroll
+        for (int k = 0; k < W::KC; k++) {
+            const int e = (4 * k + g) * (16 / (int)sizeof(T));
+            v4u v = {0, 0, 0, 0};
+            if (e < hd) v = *(const v4u *)(q + e) ^ flip;
+            x.Q[c][k] = v;
+        }
+        x.m[c] = -__builtin_inff();
+        x.l[c] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < W::VE; t++) x.O[c][t] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll 1
+    for (int k = 0; k < 2; k++) {
+        attn_list L = k ? own : shared;
+        int full = L.to;
+#pragma unroll
+        for (int c = 0; c < NR; c++) x.lim[c] = L.n;
+        if (L.own) {
+            const int first = L.n - s.a.q_len + 1, last = row0 + 16 * NR < R ? row0 + 16 * NR - 1 : R - 1;
+            L.to = min(L.to, first + last / G);
+            full = min(L.to, first + row0 / G);
+#pragma unroll
+            for (int c = 0; c < NR; c++) {
+                const int r = row0 + 16 * c + i;
+                x.lim[c] = first + (r < R ? r : R - 1) / G;
+            }
+        }
+        x.walk(s, L, kvh, sc, full, bad);
+    }
+    // join the waves
+    float *ob = lds;                                           // [wave][16 NR][LDS_COL]
+    float2 *mb = (float2 *)(lds + 4 * 16 * NR * W::LDS_COL);   // [wave][16 NR]
+    if (bad) // a page or length that is none
+#pragma unroll
+        for (int c = 0; c < NR; c++) x.l[c] = __builtin_nanf("");
+#pragma unroll
+    for (int c = 0; c < NR; c++) {
+        float l = x.l[c];
+        l += __uint_as_float(qmh_xor16_u(__float_as_uint(l)));
+        l += __uint_as_float(qmh_xor32_u(__float_as_uint(l)));
+        if (g == 0) mb[w * 16 * NR + 16 * c + i] = make_float2(x.m[c], l);
+        float *o = ob + (w * 16 * NR + 16 * c + i) * W::LDS_COL + 4 * g * W::VE;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int t = 0; t < W::VE; t += 4)
+                *(v4f *)(o + e * W::VE + t) = (v4f){x.O[c][t][e], x.O[c][t + 1][e], x.O[c][t + 2][e], x.O[c][t + 3][e]};
+    }
+    __syncthreads();
+    constexpr int D4 = HDP / 4;
+    for (int u = threadIdx.x; u < 16 * NR * D4; u += 256) {
+        const int col = u / D4, d = 4 * (u % D4), r = row0 + col;
+        if (r >= R || d >= hd) continue;
+        float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) m = fmaxf(m, mb[k * 16 * NR + col].x);
+        v4f o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 a = mb[k * 16 * NR + col];
+            const float f = a.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((a.x - m) * sc); // a wave without steps: sums of 0 (or NaN)
+            l = __builtin_fmaf(a.y, f, l);
+            o += *(const v4f *)(ob + (k * 16 * NR + col) * W::LDS_COL + d) * f;
+        }
+        const int token = t0 + r / G, h = h0 + r % G;
+        if (part < 0) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            qmh_vec<T, 4> y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y.e[e] = (T)(o[e] * inv);
+            *(qmh_vec<T, 4> *)((T *)s.a.out + (int64_t)token * s.a.out_stride + (int64_t)h * hd + d) = y;
+        } else {
+            const int64_t at = (int64_t)part * s.n.rows + (int64_t)token * H + h;
+            if (d == 0) s.ml[at] = make_float2(m, l);
+            *(v4f *)(s.part + at * hd + d) = o;
+        }
+    }
+}
+
+template <typename T, int HDP, int NRP, int NRO>
+__global__ __launch_bounds__(256) void k_paged_attention(const attn_args s) {
+    __shared__ __align__(16) float lds[attn_wave<T, HDP, (NRP > NRO ? NRP : NRO)>::LDS_FLOATS];
+    const attn_plan &n = s.n;
+    const int KV = s.p.n_kv_heads, Q = s.a.q_len;
+    int64_t b = blockIdx.x;
+    const attn_list none = {nullptr, 0, 0, 0, 0};
+    if (b < n.pre_blocks) { // (group, kv head, split), row tile: tiles of the same keys 8 blocks apart, on one XCD's cache
+        const int64_t units = (int64_t)s.a.n_groups * KV * n.ps;
+        const int64_t line = b / (8 * n.pt), in = b - line * 8 * n.pt;
+        const int64_t unit = line * 8 + (in & 7);
+        const int tile = (int)(in >> 3);
+        if (unit >= units) return;
+        const int split = (int)(unit / ((int64_t)s.a.n_groups * KV)), gk = (int)(unit - (int64_t)split * s.a.n_groups * KV);
+        const int g = gk / KV, kvh = gk - g * KV;
+        int len = s.a.prefix_len[g];
+        const bool bad = len < 0 || len > s.a.max_prefix;
+        if (bad) len = 0;
+        const attn_list L = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, len, split * n.pc, min(len, (split + 1) * n.pc)};
+        attend<T, HDP, NRP>(s, lds, tile * 16 * NRP, n.per * Q * n.G, g * n.per * Q, kvh, L, none, bad, split);
+        return;
+    }
+    b -= n.pre_blocks;
+    const int64_t units = (int64_t)s.a.n_seq * KV;
+    const int64_t st = b / units, unit = b - st * units;
+    const int split = (int)(st % n.os), tile = (int)(st / n.os), sq = (int)(unit / KV), kvh = (int)(unit - (int64_t)sq * KV);
+    int len = s.a.max_len ? s.a.len[sq] : 0, plen = 0;
+    bool bad = len < 0 || len > s.a.max_len;
+    if (bad) len = 0;
+    const int g = sq / n.per;
+    if (n.joint && s.a.max_prefix) {
+        plen = s.a.prefix_len[g];
+        if (plen < 0 || plen > s.a.max_prefix) {
+            bad = true;
+            plen = 0;
+        }
+    }
+    const attn_list S = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, plen, 0, plen};
+    const attn_list L = {s.a.table + (int64_t)sq * s.a.table_stride, 1, len, split * n.oc, min(len, (split + 1) * n.oc)};
+    attend<T, HDP, NRO>(s, lds, tile * 16 * NRO, Q * n.G, sq * Q, kvh, S, L, bad, n.ps + n.os > 1 ? n.ps + split : -1);
+}
+
+// out = the parts of each row joined: 64 / D4 rows a wave, 4 values a lane
+template <typename T, int D4>
+__global__ __launch_bounds__(256) void k_attention_join(const attn_args s, int parts) {
+    const int hd = s.p.head_dim, d = 4 * (threadIdx.x % D4);
+    const int64_t row = (int64_t)blockIdx.x * (256 / D4) + threadIdx.x / D4;
+    if (row >= s.n.rows || d >= hd) return;
+    const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f;
+    float m = -__builtin_inff(), l = 0.0f;
+    for (int k = 0; k < parts; k++) m = fmaxf(m, s.ml[(int64_t)k * s.n.rows + row].x);
+    v4f o = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < parts; k++) {
+        const float2 a = s.ml[(int64_t)k * s.n.rows + row];
+        const float f = a.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((a.x - m) * sc);
+        l = __builtin_fmaf(a.y, f, l);
+        o += *(const v4f *)(s.part + ((int64_t)k * s.n.rows + row) * hd + d) * f;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T *out = (T *)a.out + row * a.out_stride + h * hd;
-    for (int c = 0; c < 4; c++)
-        if (lane + 64 * c < hd) out[lane + 64 * c] = (T)(acc[c] * inv);
+    const int64_t token = row / s.a.n_heads;
+    const int h = (int)(row - token * s.a.n_heads);
+    qmh_vec<T, 4> y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y.e[e] = (T)(o[e] * inv);
+    *(qmh_vec<T, 4> *)((T *)s.a.out + token * s.a.out_stride + (int64_t)h * hd + d) = y;
+}
+
+attn_plan plan_attention(const qmh_attention_args *a, int cus) {
+    attn_plan n = {};
+    const qmh_pages *p = a->pages;
+    const int KV = p->n_kv_heads;
+    const int most = p->head_dim > 128 ? 1 : p->head_dim > 64 ? 2 : 4; // what the registers hold
+    n.G = a->n_heads / KV;
+    n.per = a->n_seq / a->n_groups;
+    n.rows = (int64_t)a->n_seq * a->q_len * a->n_heads;
+    const int64_t ro = (int64_t)a->q_len * n.G, rp = a->max_prefix ? ro * n.per : ro;
+    auto tiles = [&](int64_t r) { return r <= 16 || most == 1 ? 1 : r <= 32 || most == 2 ? 2 : 4; };
+    n.nrp = tiles(rp);
+    n.nro = ro <= 16 ? 1 : n.nrp;
+    n.pt = (int)((rp + 16 * n.nrp - 1) / (16 * n.nrp));
+    n.ot = (int)((ro + 16 * n.nro - 1) / (16 * n.nro));
+    const int64_t up = (int64_t)a->n_groups * KV * n.pt, uo = (int64_t)a->n_seq * KV * n.ot;
+    n.os = 1;
+    n.oc = a->max_len ? a->max_len : 1;
+    // short sequences: each reads the prefix itself, which costs less than another launch
+    n.joint = a->max_prefix == 0 ? a->max_len <= 512 : a->max_prefix + a->max_len <= 256;
+    if (!n.joint) {
+        // chunks of positions, the same for both, that give each CU a few workgroups
+        const int64_t all = up * a->max_prefix + uo * a->max_len;
+        int64_t c = (all / (4 * cus) + 127) / 128 * 128;
+        c = c < 128 ? 128 : c > 4096 ? 4096 : c;
+        if (a->max_prefix) {
+            n.ps = (int)((a->max_prefix + c - 1) / c);
+            n.pc = (int)c;
+            n.pre_blocks = ((int64_t)a->n_groups * KV * n.ps + 7) / 8 * 8 * n.pt;
+        }
+        if (a->max_len) {
+            n.os = (int)((a->max_len + c - 1) / c);
+            n.oc = (int)c;
+        }
+    }
+    n.blocks = n.pre_blocks + uo * n.os;
+    return n;
+}
+
+template <typename T, int HDP>
+void launch_attention(const attn_args &s, hipStream_t st) {
+    const dim3 g((uint32_t)s.n.blocks), t(256);
+    const int p = s.n.nrp, o = s.n.nro;
+    if (p == 1) hipLaunchKernelGGL((k_paged_attention<T, HDP, 1, 1>), g, t, 0, st, s);
+    else if constexpr (HDP <= 128) {
+        if (p == 2 && o == 1) hipLaunchKernelGGL((k_paged_attention<T, HDP, 2, 1>), g, t, 0, st, s);
+        else if (p == 2) hipLaunchKernelGGL((k_paged_attention<T, HDP, 2, 2>), g, t, 0, st, s);
+    }
+    if constexpr (HDP <= 64) {
+        if (p == 4 && o == 1) hipLaunchKernelGGL((k_paged_attention<T, HDP, 4, 1>), g, t, 0, st, s);
+        else if (p == 4) hipLaunchKernelGGL((k_paged_attention<T, HDP, 4, 4>), g, t, 0, st, s);
+    }
+    const int parts = s.n.ps + s.n.os;
+    if (parts > 1) {
+        constexpr int per = 256 / (HDP / 4);
+        hipLaunchKernelGGL((k_attention_join<T, HDP / 4>), dim3((uint32_t)((s.n.rows + per - 1) / per)), t, 0, st, s, parts);
+    }
 }
 
 // --------------------------------------------------------------------------- reorder
@@ -268,19 +692,26 @@ extern "C" int qmh_launch_paged_append(const qmh_append_args *a, const qmh_rotar
 }
 
 extern "C" size_t qmh_attention_ws_bytes(const qmh_attention_args *a, int cus) {
-    (void)a;
-    (void)cus;
-    return 0;
+    if (a->n_seq == 0) return 0;
+    const attn_plan n = plan_attention(a, cus);
+    const size_t parts = n.ps + n.os;
+    return parts > 1 ? parts * n.rows * (a->pages->head_dim * sizeof(float) + sizeof(float2)) : 0;
 }
 
 extern "C" int qmh_launch_paged_attention(const qmh_attention_args *a, int cus, void *ws, void *stream) {
-    (void)cus;
-    (void)ws;
-    const int64_t waves = (int64_t)a->n_seq * a->q_len * a->n_heads;
-    if (waves > 0x7fffffff - 4) return (int)hipErrorInvalidValue;
-    qmh_for_type(a->pages->dtype, [&](auto z) {
-        hipLaunchKernelGGL((k_paged_attention<decltype(z)>), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, (hipStream_t)stream,
-                           *a, *a->pages);
+    attn_args s;
+    s.a = *a;
+    s.p = *a->pages;
+    s.n = plan_attention(a, cus);
+    s.lg_ps = __builtin_ctz(s.p.page_size);
+    s.part = (float *)ws;
+    s.ml = (float2 *)(s.part + (size_t)(s.n.ps + s.n.os) * s.n.rows * s.p.head_dim);
+    if (s.n.blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+    qmh_for_type(s.p.dtype, [&](auto z) {
+        using T = decltype(z);
+        if (s.p.head_dim <= 64) launch_attention<T, 64>(s, (hipStream_t)stream);
+        else if (s.p.head_dim <= 128) launch_attention<T, 128>(s, (hipStream_t)stream);
+        else launch_attention<T, 256>(s, (hipStream_t)stream);
     });
     return (int)hipGetLastError();
 }
