@@ -175,6 +175,8 @@ __device__ __forceinline__ uint32_t pack2(qmh_bf16, float x, float y) {
 typedef const __attribute__((address_space(4))) int32_t *const_i32; // scalar loads
 __device__ __forceinline__ const_i32 as_const(const int32_t *p) { return (const_i32)(uintptr_t)p; }
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // how the work is divided (the same for the workspace's size and the launch)
 struct attn_plan {
     int joint;       // prefix and own pages in one pass of each sequence, no parts
@@ -183,7 +185,8 @@ struct attn_plan {
     int nrp, nro;    // 16-row tiles of a wave: prefix, own
     int pt, ps, pc;  // prefix: row tiles, splits, positions of a split
     int ot, os, oc;  // own
-    int64_t pre_blocks, blocks;
+    uint32_t pre_blocks;
+    int64_t blocks;  // below 2^31
     int64_t rows;    // all rows of queries (query x head)
 };
 
@@ -201,6 +204,7 @@ struct attn_list {
     int own;      // a sequence's own pages: its queries see different numbers of positions
     int n;        // positions
     int from, to; // this chunk's; to <= n
+    int cap;      // the table has pages (of whatever kind) up to this position
 };
 
 template <typename T, int HDP, int NR>
@@ -213,39 +217,67 @@ struct attn_wave {
     static constexpr int VB = VE * (int)sizeof(T);    // their bytes
     static constexpr int VW = VB / 4;                 // and words
     static constexpr int LDS_COL = HDP + 4;
-    static constexpr int LDS_FLOATS = 4 * 16 * NR * LDS_COL + 4 * 16 * NR * 2;
+    static constexpr int LDS_FLOATS = 4 * 16 * NR * LDS_COL + 4 * 16 * NR * 2 + 16 * NR * 2;
 
     v4u Q[NR][KC];
     v4f O[NR][VE];
-    float m[NR], l[NR];
+    // l: the sum of a row's probabilities: a lane's own positions in l[0], or (16 bit) all of them in every element, by a
+    // product with ones
+    v4f l[NR];
+    float m[NR], off[NR], pass[NR]; // the reference, its negative in powers of two, the score that raises it
     int lim[NR];
-    struct step {
-        v4u k[RT][KC];
-        uint32_t v[RT * 4][VW];
-    };
+    v4u k[RT][KC];
+    uint32_t v[RT * 4][VW];
 
-    __device__ __forceinline__ void load(step &x, const attn_args &s, const attn_list &L, int base, int kvh, bool &bad) const {
-        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = s.p.head_dim;
-        const int rb = hd * (int)sizeof(T);
+    // page numbers of a step, fetched one step before its loads go out (the first ones without waiting for the
+    // list's length)
+    struct pages {
+        int page[RT];
+    };
+    __device__ __forceinline__ pages fetch(const attn_args &s, const attn_list &L, int base) const {
+        pages x;
+#pragma unroll
+        for (int r = 0; r < RT; r++) x.page[r] = as_const(L.tab)[min(base + 16 * r, L.cap) >> s.lg_ps];
+        return x;
+    }
+
+    // where a step's blocks of 16 positions lie in the pools, and their bytes in rows that are somebody's: rows from L.to
+    // on are out of range
+    struct blocks {
+        int64_t off[RT];
+        int bytes[RT];
+    };
+    __device__ __forceinline__ blocks locate(const attn_args &s, const attn_list &L, const pages &pg, int base, int kvh, bool &bad) const {
+        blocks x;
+        const int rb = s.p.head_dim * (int)sizeof(T);
 #pragma unroll
         for (int r = 0; r < RT; r++) {
-            const int at = base + 16 * r, left = L.to - at; // positions from L.to on are nobody's here
-            const int rows = left < 0 ? 0 : left > 16 ? 16 : left;
-            const int safe = rows ? at : 0;
-            int page = rows ? as_const(L.tab)[safe >> s.lg_ps] : 0;
-            if ((uint32_t)page >= (uint64_t)s.p.n_pages) {
-                bad = true;
-                page = 0;
-            }
-            page = __builtin_amdgcn_readfirstlane(page);
-            const int64_t off = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (safe & (s.p.page_size - 1))) * rb;
-            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.k + off, (short)0, rows * rb, 0x00020000);
-            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.v + off, (short)0, rows * rb, 0x00020000);
+            const int at = base + 16 * r, left = L.to - at, page = pg.page[r];
+            const int rows = uniform(left < 0 ? 0 : left > 16 ? 16 : left);
+            const bool none = (uint32_t)page >= (uint32_t)s.p.n_pages;
+            bad |= none && rows > 0;
+            x.off[r] = (((int64_t)uniform(none ? 0 : page) * s.p.n_kv_heads + kvh) * s.p.page_size + (at & (s.p.page_size - 1))) * rb;
+            x.bytes[r] = rows * rb;
+        }
+        return x;
+    }
+    __device__ __forceinline__ void load_k(const attn_args &s, const blocks &bl) {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, rb = s.p.head_dim * (int)sizeof(T);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.k + bl.off[r], (short)0, bl.bytes[r], 0x00020000);
 #pragma unroll
             for (int c = 0; c < KC; c++) {
                 const int b = (4 * c + g) * 16;
-                x.k[r][c] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rk, b < rb ? i * rb + b : 0x7ffffff0, 0, 0));
+                k[r][c] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rk, b < rb ? i * rb + b : 0x7ffffff0, 0, 0));
             }
+        }
+    }
+    __device__ __forceinline__ void load_v(const attn_args &s, const blocks &bl) {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, rb = s.p.head_dim * (int)sizeof(T);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.v + bl.off[r], (short)0, bl.bytes[r], 0x00020000);
 #pragma unroll
             for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -254,37 +286,39 @@ struct attn_wave {
                     if constexpr (VB >= 16) {
                         const v4u w = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, 0));
 #pragma unroll
-                        for (int d = 0; d < 4; d++) x.v[4 * r + e][4 * c + d] = w[d];
+                        for (int d = 0; d < 4; d++) v[4 * r + e][4 * c + d] = w[d];
                     } else {
                         const auto w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 0);
-                        x.v[4 * r + e][0] = w[0];
-                        x.v[4 * r + e][1] = w[1];
+                        v[4 * r + e][0] = w[0];
+                        v[4 * r + e][1] = w[1];
                     }
                 }
         }
     }
 
-    // masked: some row of the tile does not see all of the step
-    __device__ __forceinline__ void use(const step &x, int base, float sc, bool masked) {
-        const int g = (threadIdx.x & 63) >> 4;
-        v4f S[NR][RT];
+    __device__ __forceinline__ void scores(v4f (&S)[NR][RT]) const {
 #pragma unroll
         for (int c = 0; c < NR; c++)
 #pragma unroll
             for (int r = 0; r < RT; r++) {
                 v4f acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < KC; k++) {
+                for (int x = 0; x < KC; x++) {
                     if constexpr (F) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[r][k][j]), __uint_as_float(Q[c][k][j]), acc, 0, 0, 0);
+                            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[r][x][j]), __uint_as_float(Q[c][x][j]), acc, 0, 0, 0);
                     } else {
-                        acc = mma32(T{}, x.k[r][k], Q[c][k], acc);
+                        acc = mma32(T{}, k[r][x], Q[c][x], acc);
                     }
                 }
                 S[c][r] = acc;
             }
+    }
+
+    // the probabilities of a step's scores, packed for the product with V; masked: some row does not see all of it
+    __device__ __forceinline__ void weigh(v4f (&S)[NR][RT], v4u (&P)[NR], int base, float sc, bool masked) {
+        const int g = (threadIdx.x & 63) >> 4;
         if (masked) {
 #pragma unroll
             for (int c = 0; c < NR; c++)
@@ -295,59 +329,71 @@ struct attn_wave {
                         if (base + 16 * r + 4 * g + e >= lim[c]) S[c][r][e] = -__builtin_inff();
         }
         // The reference value of a row's exponentials is raised only when a score passes it by 2^8: the sums stay exact
-        // floats either way, and the rescaling of O is rare
+        // floats either way, and the rescaling of O is rare. (maximum: NaN wins, and needs no canonical operands.)
         bool up = false;
         float mx[NR];
 #pragma unroll
         for (int c = 0; c < NR; c++) {
-            float v = S[c][0][0];
+            float x = S[c][0][0];
 #pragma unroll
             for (int r = 0; r < RT; r++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) v = fmaxf(v, S[c][r][e]);
-            mx[c] = v;
-            up |= m[c] == -__builtin_inff() ? v > m[c] : (v - m[c]) * sc > 8.0f;
+                for (int e = 0; e < 4; e++) x = __builtin_elementwise_maximum(x, S[c][r][e]);
+            mx[c] = x;
+            up |= x > pass[c];
         }
         if (__any(up)) {
 #pragma unroll
             for (int c = 0; c < NR; c++) {
-                float v = mx[c];
-                v = fmaxf(v, __uint_as_float(qmh_xor16_u(__float_as_uint(v))));
-                v = fmaxf(v, __uint_as_float(qmh_xor32_u(__float_as_uint(v))));
-                if (v > m[c]) {
-                    const float f = m[c] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[c] - v) * sc);
-                    m[c] = v;
-                    l[c] *= f;
+                float x = mx[c];
+                x = fmaxf(x, __uint_as_float(qmh_xor16_u(__float_as_uint(x))));
+                x = fmaxf(x, __uint_as_float(qmh_xor32_u(__float_as_uint(x))));
+                if (x > m[c]) {
+                    const float f = m[c] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[c] - x) * sc);
+                    m[c] = x;
+                    off[c] = -x * sc;
+                    pass[c] = x + 8.0f / sc;
+                    l[c] = l[c] * f;
 #pragma unroll
                     for (int t = 0; t < VE; t++) O[c][t] = O[c][t] * f;
                 }
             }
         }
-        v4u P[NR];   // 16-bit: positions 4 g + e, then 16 + 4 g + e
 #pragma unroll
         for (int c = 0; c < NR; c++) {
-            const float off = m[c] == -__builtin_inff() ? 0.0f : -m[c] * sc;
-            float pr[4 * RT];
 #pragma unroll
             for (int r = 0; r < RT; r++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[c][r][e], sc, off));
-                    if (masked && base + 16 * r + 4 * g + e >= lim[c]) v = 0.0f;
-                    pr[4 * r + e] = v;
-                }
-            float sum = 0.0f;
+                for (int e = 0; e < 4; e++) S[c][r][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[c][r][e], sc, off[c]));
+        }
+        if (masked) { // also where the scale is 0
+            asm volatile(""); // a branch: no selects in the other steps
 #pragma unroll
-            for (int e = 0; e < 4 * RT; e++) sum += pr[e];
-            l[c] += sum;
+            for (int c = 0; c < NR; c++)
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (base + 16 * r + 4 * g + e >= lim[c]) S[c][r][e] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < NR; c++) {
             if constexpr (F) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) P[c][e] = __float_as_uint(pr[e]);
+                for (int e = 0; e < 4; e++) {
+                    l[c][0] += S[c][0][e];
+                    P[c][e] = __float_as_uint(S[c][0][e]);
+                }
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) P[c][e] = pack2(T{}, pr[(2 * e) % (4 * RT)], pr[(2 * e + 1) % (4 * RT)]);
+                for (int e = 0; e < 4; e++) P[c][e] = pack2(T{}, S[c][e / 2][(2 * e) % 4], S[c][e / 2][(2 * e + 1) % 4]);
+                const uint32_t one = pack2(T{}, 1.0f, 1.0f);
+                l[c] = mma32(T{}, (v4u){one, one, one, one}, P[c], l[c]);
             }
         }
+    }
+
+    __device__ __forceinline__ void add_values(const v4u (&P)[NR]) {
         if constexpr (F) {
 #pragma unroll
             for (int t = 0; t < VE; t++)
@@ -355,14 +401,14 @@ struct attn_wave {
                 for (int c = 0; c < NR; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        O[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.v[e][t]), __uint_as_float(P[c][e]), O[c][t], 0, 0, 0);
+                        O[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[e][t]), __uint_as_float(P[c][e]), O[c][t], 0, 0, 0);
         } else {
 #pragma unroll
             for (int u = 0; u < VW; u++) {
                 v4u lo, hi; // tiles 2 u and 2 u + 1
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t a = x.v[(2 * j) % (4 * RT)][u], b = x.v[(2 * j + 1) % (4 * RT)][u];
+                    const uint32_t a = v[(2 * j) % (4 * RT)][u], b = v[(2 * j + 1) % (4 * RT)][u];
                     lo[j] = __builtin_amdgcn_perm(b, a, 0x05040100);
                     hi[j] = __builtin_amdgcn_perm(b, a, 0x07060302);
                 }
@@ -375,20 +421,27 @@ struct attn_wave {
         }
     }
 
-    // this wave's steps of the list's chunk; full: positions that every row sees
+    // This wave's steps of the list's chunk; full: positions that every row sees. The next step's keys are loaded as soon
+    // as the scores are made, its values as soon as the step's are used: each has the other's work to arrive in.
     __device__ __forceinline__ void walk(const attn_args &s, const attn_list &L, int kvh, float sc, int full, bool &bad) {
-        const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        const int w = uniform((int)(threadIdx.x >> 6));
         int base = L.from + w * KS;
+        pages pg = fetch(s, L, base);
         if (base >= L.to) return;
-        step A, B;
-        load(A, s, L, base, kvh, bad);
+        blocks bl = locate(s, L, pg, base, kvh, bad);
+        load_k(s, bl);
+        load_v(s, bl);
+        pg = fetch(s, L, base + 4 * KS);
         for (;;) {
-            load(B, s, L, base + 4 * KS, kvh, bad);
-            use(A, base, sc, base + KS > full);
-            base += 4 * KS;
-            if (base >= L.to) break;
-            load(A, s, L, base + 4 * KS, kvh, bad);
-            use(B, base, sc, base + KS > full);
+            v4f S[NR][RT];
+            v4u P[NR];
+            scores(S);
+            bl = locate(s, L, pg, base + 4 * KS, kvh, bad);
+            load_k(s, bl);
+            weigh(S, P, base, sc, base + KS > full);
+            add_values(P);
+            load_v(s, bl);
+            pg = fetch(s, L, base + 8 * KS);
             base += 4 * KS;
             if (base >= L.to) break;
         }
@@ -418,8 +471,9 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             if (e < hd) v = *(const v4u *)(q + e) ^ flip;
             x.Q[c][k] = v;
         }
-        x.m[c] = -__builtin_inff();
-        x.l[c] = 0.0f;
+        x.m[c] = x.pass[c] = -__builtin_inff();
+        x.off[c] = 0.0f;
+        x.l[c] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < W::VE; t++) x.O[c][t] = (v4f){0.f, 0.f, 0.f, 0.f};
     }
@@ -444,15 +498,20 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     // join the waves
     float *ob = lds;                                           // [wave][16 NR][LDS_COL]
     float2 *mb = (float2 *)(lds + 4 * 16 * NR * W::LDS_COL);   // [wave][16 NR]
-    if (bad) // a page or length that is none
-#pragma unroll
-        for (int c = 0; c < NR; c++) x.l[c] = __builtin_nanf("");
+    int2 *where = (int2 *)(mb + 4 * 16 * NR);                  // [16 NR]: token, head
 #pragma unroll
     for (int c = 0; c < NR; c++) {
-        float l = x.l[c];
-        l += __uint_as_float(qmh_xor16_u(__float_as_uint(l)));
-        l += __uint_as_float(qmh_xor32_u(__float_as_uint(l)));
-        if (g == 0) mb[w * 16 * NR + 16 * c + i] = make_float2(x.m[c], l);
+        float l = x.l[c][0];
+        if constexpr (W::F) {
+            l += __uint_as_float(qmh_xor16_u(__float_as_uint(l)));
+            l += __uint_as_float(qmh_xor32_u(__float_as_uint(l)));
+        }
+        if (bad) l = __builtin_nanf(""); // a page or length that is none
+        if (g == 0) {
+            mb[w * 16 * NR + 16 * c + i] = make_float2(x.m[c], l);
+            const int r = row0 + 16 * c + i;
+            if (w == 0) where[16 * c + i] = make_int2(t0 + r / G, h0 + r % G);
+        }
         float *o = ob + (w * 16 * NR + 16 * c + i) * W::LDS_COL + 4 * g * W::VE;
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -462,9 +521,9 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     }
     __syncthreads();
     constexpr int D4 = HDP / 4;
-    for (int u = threadIdx.x; u < 16 * NR * D4; u += 256) {
-        const int col = u / D4, d = 4 * (u % D4), r = row0 + col;
-        if (r >= R || d >= hd) continue;
+    const int d = 4 * (threadIdx.x % D4); // 256 is a multiple of D4
+    if (d >= hd) return;
+    for (int col = threadIdx.x / D4; col < 16 * NR && row0 + col < R; col += 256 / D4) {
         float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; k++) m = fmaxf(m, mb[k * 16 * NR + col].x);
@@ -476,15 +535,15 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             l = __builtin_fmaf(a.y, f, l);
             o += *(const v4f *)(ob + (k * 16 * NR + col) * W::LDS_COL + d) * f;
         }
-        const int token = t0 + r / G, h = h0 + r % G;
+        const int2 th = where[col];
         if (part < 0) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             qmh_vec<T, 4> y;
 #pragma unroll
             for (int e = 0; e < 4; e++) y.e[e] = (T)(o[e] * inv);
-            *(qmh_vec<T, 4> *)((T *)s.a.out + (int64_t)token * s.a.out_stride + (int64_t)h * hd + d) = y;
+            *(qmh_vec<T, 4> *)((T *)s.a.out + (int64_t)th.x * s.a.out_stride + (int64_t)th.y * hd + d) = y;
         } else {
-            const int64_t at = (int64_t)part * s.n.rows + (int64_t)token * H + h;
+            const int64_t at = (int64_t)part * s.n.rows + (int64_t)th.x * H + th.y;
             if (d == 0) s.ml[at] = make_float2(m, l);
             *(v4f *)(s.part + at * hd + d) = o;
         }
@@ -492,66 +551,80 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
 }
 
 template <typename T, int HDP, int NRP, int NRO>
-__global__ __launch_bounds__(256) void k_paged_attention(const attn_args s) {
+__global__ __launch_bounds__(256, 2) void k_paged_attention(const attn_args s) {
     __shared__ __align__(16) float lds[attn_wave<T, HDP, (NRP > NRO ? NRP : NRO)>::LDS_FLOATS];
     const attn_plan &n = s.n;
     const int KV = s.p.n_kv_heads, Q = s.a.q_len;
-    int64_t b = blockIdx.x;
-    const attn_list none = {nullptr, 0, 0, 0, 0};
-    if (b < n.pre_blocks) { // (group, kv head, split), row tile: tiles of the same keys 8 blocks apart, on one XCD's cache
-        const int64_t units = (int64_t)s.a.n_groups * KV * n.ps;
-        const int64_t line = b / (8 * n.pt), in = b - line * 8 * n.pt;
-        const int64_t unit = line * 8 + (in & 7);
-        const int tile = (int)(in >> 3);
-        if (unit >= units) return;
-        const int split = (int)(unit / ((int64_t)s.a.n_groups * KV)), gk = (int)(unit - (int64_t)split * s.a.n_groups * KV);
-        const int g = gk / KV, kvh = gk - g * KV;
-        int len = s.a.prefix_len[g];
+    uint32_t b = blockIdx.x;
+    const attn_list none = {nullptr, 0, 0, 0, 0, 0};
+    if (b < n.pre_blocks) { // split, (group, kv head); row tile: tiles of the same keys 8 blocks apart, on one XCD's cache
+        const uint32_t gks = (uint32_t)s.a.n_groups * KV, line = b / (8 * n.pt), in = b - line * 8 * n.pt, unit = line * 8 + (in & 7);
+        const int tile = (int)(in >> 3), split = (int)(unit / gks);
+        if (split >= n.ps) return;
+        const uint32_t gk = unit - split * gks, g = gk / KV, kvh = gk - g * KV;
+        int len = uniform(as_const(s.a.prefix_len)[g]);
         const bool bad = len < 0 || len > s.a.max_prefix;
         if (bad) len = 0;
-        const attn_list L = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, len, split * n.pc, min(len, (split + 1) * n.pc)};
+        const attn_list L = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, len, split * n.pc, min(len, (split + 1) * n.pc), s.a.max_prefix - 1};
         attend<T, HDP, NRP>(s, lds, tile * 16 * NRP, n.per * Q * n.G, g * n.per * Q, kvh, L, none, bad, split);
         return;
     }
     b -= n.pre_blocks;
-    const int64_t units = (int64_t)s.a.n_seq * KV;
-    const int64_t st = b / units, unit = b - st * units;
-    const int split = (int)(st % n.os), tile = (int)(st / n.os), sq = (int)(unit / KV), kvh = (int)(unit - (int64_t)sq * KV);
-    int len = s.a.max_len ? s.a.len[sq] : 0, plen = 0;
+    const uint32_t units = (uint32_t)s.a.n_seq * KV, st = b / units, unit = b - st * units;
+    const uint32_t tile = st / n.os, split = st - tile * n.os, sq = unit / KV, kvh = unit - sq * KV, g = sq / n.per;
+    int len = s.a.max_len ? uniform(as_const(s.a.len)[sq]) : 0, plen = 0;
     bool bad = len < 0 || len > s.a.max_len;
     if (bad) len = 0;
-    const int g = sq / n.per;
     if (n.joint && s.a.max_prefix) {
-        plen = s.a.prefix_len[g];
+        plen = uniform(as_const(s.a.prefix_len)[g]);
         if (plen < 0 || plen > s.a.max_prefix) {
             bad = true;
             plen = 0;
         }
     }
-    const attn_list S = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, plen, 0, plen};
-    const attn_list L = {s.a.table + (int64_t)sq * s.a.table_stride, 1, len, split * n.oc, min(len, (split + 1) * n.oc)};
-    attend<T, HDP, NRO>(s, lds, tile * 16 * NRO, Q * n.G, sq * Q, kvh, S, L, bad, n.ps + n.os > 1 ? n.ps + split : -1);
+    const attn_list S = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, plen, 0, plen, s.a.max_prefix - 1};
+    const attn_list L = {s.a.table + (int64_t)sq * s.a.table_stride, 1, len, (int)split * n.oc, min(len, ((int)split + 1) * n.oc), s.a.max_len - 1};
+    attend<T, HDP, NRO>(s, lds, tile * 16 * NRO, Q * n.G, sq * Q, kvh, S, L, bad, n.ps + n.os > 1 ? n.ps + (int)split : -1);
 }
 
-// out = the parts of each row joined: 64 / D4 rows a wave, 4 values a lane
+// out = the parts of a row joined, a wave a row (parts at most 64: lane k weighs part k). 64 / D4 parts are read at
+// once, 4 values a lane.
 template <typename T, int D4>
 __global__ __launch_bounds__(256) void k_attention_join(const attn_args s, int parts) {
-    const int hd = s.p.head_dim, d = 4 * (threadIdx.x % D4);
-    const int64_t row = (int64_t)blockIdx.x * (256 / D4) + threadIdx.x / D4;
-    if (row >= s.n.rows || d >= hd) return;
+    constexpr int PG = 64 / D4;
+    const int lane = threadIdx.x & 63, hd = s.p.head_dim, d = 4 * (lane % D4);
+    const uint32_t row = (uint32_t)uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    if (row >= s.n.rows) return;
     const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f;
-    float m = -__builtin_inff(), l = 0.0f;
-    for (int k = 0; k < parts; k++) m = fmaxf(m, s.ml[(int64_t)k * s.n.rows + row].x);
+    float2 a = make_float2(-__builtin_inff(), 0.0f);
+    if (lane < parts) a = s.ml[(int64_t)lane * s.n.rows + row];
+    const float m = qmh_wave_max(a.x);
+    const float f = a.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((a.x - m) * sc); // without a score: sums of 0 (or NaN)
+    float l = a.y * f;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) l += __shfl_xor(l, k);
     v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < parts; k++) {
-        const float2 a = s.ml[(int64_t)k * s.n.rows + row];
-        const float f = a.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((a.x - m) * sc);
-        l = __builtin_fmaf(a.y, f, l);
-        o += *(const v4f *)(s.part + ((int64_t)k * s.n.rows + row) * hd + d) * f;
+    const float *part = s.part + (int64_t)row * hd + (d < hd ? d : 0);
+    const int64_t step = s.n.rows * hd;
+    int k = lane / D4;
+    for (; k + 3 * PG < parts; k += 4 * PG) {
+        v4f v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = *(const v4f *)(part + (k + j * PG) * step);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o += v[j] * __shfl(f, k + j * PG);
     }
+    for (int j = 0; j < 4; j++, k += PG) { // __shfl by all lanes
+        const float fk = __shfl(f, k & 63);
+        if (k < parts) o += *(const v4f *)(part + k * step) * fk;
+    }
+#pragma unroll
+    for (int x = D4; x < 64; x <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], x);
+    if (lane >= D4 || d >= hd) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t token = row / s.a.n_heads;
-    const int h = (int)(row - token * s.a.n_heads);
+    const uint32_t token = row / s.a.n_heads, h = row - token * s.a.n_heads;
     qmh_vec<T, 4> y;
 #pragma unroll
     for (int e = 0; e < 4; e++) y.e[e] = (T)(o[e] * inv);
@@ -573,26 +646,30 @@ attn_plan plan_attention(const qmh_attention_args *a, int cus) {
     n.pt = (int)((rp + 16 * n.nrp - 1) / (16 * n.nrp));
     n.ot = (int)((ro + 16 * n.nro - 1) / (16 * n.nro));
     const int64_t up = (int64_t)a->n_groups * KV * n.pt, uo = (int64_t)a->n_seq * KV * n.ot;
+    int64_t pre = 0;
     n.os = 1;
     n.oc = a->max_len ? a->max_len : 1;
     // short sequences: each reads the prefix itself, which costs less than another launch
     n.joint = a->max_prefix == 0 ? a->max_len <= 512 : a->max_prefix + a->max_len <= 256;
     if (!n.joint) {
-        // chunks of positions, the same for both, that give each CU a few workgroups
+        // chunks of positions, about the same for both, that fill the chip's workgroups (two per CU) once
         const int64_t all = up * a->max_prefix + uo * a->max_len;
-        int64_t c = (all / (4 * cus) + 127) / 128 * 128;
-        c = c < 128 ? 128 : c > 4096 ? 4096 : c;
+        const int unit = 4 * (p->dtype == QMH_F32 ? 16 : 32); // a step of every wave
+        const double c = (double)all / (2 * cus);
+        auto split = [&](int len, int most, int *chunk) {
+            int k = (int)(len / c + 0.5);
+            k = k < 1 ? 1 : k > most ? most : k;
+            *chunk = ((len + k - 1) / k + unit - 1) / unit * unit;
+            return (len + *chunk - 1) / *chunk;
+        };
         if (a->max_prefix) {
-            n.ps = (int)((a->max_prefix + c - 1) / c);
-            n.pc = (int)c;
-            n.pre_blocks = ((int64_t)a->n_groups * KV * n.ps + 7) / 8 * 8 * n.pt;
+            n.ps = split(a->max_prefix, 40, &n.pc);
+            pre = ((int64_t)a->n_groups * KV * n.ps + 7) / 8 * 8 * n.pt;
         }
-        if (a->max_len) {
-            n.os = (int)((a->max_len + c - 1) / c);
-            n.oc = (int)c;
-        }
+        if (a->max_len) n.os = split(a->max_len, 24, &n.oc);
     }
-    n.blocks = n.pre_blocks + uo * n.os;
+    n.pre_blocks = (uint32_t)(pre < 0x7fffffff ? pre : 0x7fffffff);
+    n.blocks = pre + uo * n.os;
     return n;
 }
 
@@ -611,8 +688,7 @@ void launch_attention(const attn_args &s, hipStream_t st) {
     }
     const int parts = s.n.ps + s.n.os;
     if (parts > 1) {
-        constexpr int per = 256 / (HDP / 4);
-        hipLaunchKernelGGL((k_attention_join<T, HDP / 4>), dim3((uint32_t)((s.n.rows + per - 1) / per)), t, 0, st, s, parts);
+        hipLaunchKernelGGL((k_attention_join<T, HDP / 4>), dim3((uint32_t)((s.n.rows + 3) / 4)), t, 0, st, s, parts);
     }
 }
 
@@ -706,7 +782,7 @@ extern "C" int qmh_launch_paged_attention(const qmh_attention_args *a, int cus, 
     s.lg_ps = __builtin_ctz(s.p.page_size);
     s.part = (float *)ws;
     s.ml = (float2 *)(s.part + (size_t)(s.n.ps + s.n.os) * s.n.rows * s.p.head_dim);
-    if (s.n.blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+    if (s.n.blocks > 0x7fffffff || s.n.rows > 0x7fffffff) return (int)hipErrorInvalidValue;
     qmh_for_type(s.p.dtype, [&](auto z) {
         using T = decltype(z);
         if (s.p.head_dim <= 64) launch_attention<T, 64>(s, (hipStream_t)stream);
