@@ -255,50 +255,89 @@ int scan_ept(const qmh_beam_args *a) { return (int64_t)a->n_groups * a->n_beams 
 
 // --------------------------------------------------------------------------- reorder
 
-// V-sized pieces at `off` of every beam of a group that takes another's state: all are read before any is
-// written, so any parents move in place. own: beams without a parent keep (and out of place: take) their own.
-template <typename V, int BM>
-__device__ __forceinline__ void move_beams(uint8_t *dst, const uint8_t *src, const int32_t *par, int K, int64_t seq_stride,
-                                           int64_t off) {
-    V v[BM];
-#pragma unroll
-    for (int j = 0; j < BM; j++) {
-        if (j >= K) break;
-        const int p = par[j], from = p >= 0 && p < K ? p : j;
-        if (from != j || dst != src) v[j] = *(const V *)(src + from * seq_stride + off);
-    }
-#pragma unroll
-    for (int j = 0; j < BM; j++) {
-        if (j >= K) break;
-        const int p = par[j], from = p >= 0 && p < K ? p : j;
-        if (from != j || dst != src) *(V *)(dst + j * seq_stride + off) = v[j];
-    }
-}
-
-// Thread: one unit of U (the widest that every row is aligned to) of one row, for all beams of a group.
+// Thread: one unit of U (the widest that every row is aligned to) of one row, for all beams of a group. Every beam that
+// takes another's state is read before any is written, so any parents move in place; a row's last bytes go in 4-byte
+// pieces, read together too, and single bytes. parents: uniform, by scalar loads.
+typedef const __attribute__((address_space(4))) int32_t *const_i32;
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 template <typename U, int BM>
-__global__ __launch_bounds__(256) void k_beam_reorder(const qmh_beam_state s, uint8_t *dst, const uint8_t *src,
-                                                      const int32_t *__restrict__ parent, int n_groups, int K, uint32_t row_units,
-                                                      uint32_t blocks_per) {
+__global__ __launch_bounds__(256, BM > 16 ? 2 : 4) void k_beam_reorder(const qmh_beam_state s, uint8_t *dst, const uint8_t *src, const int32_t *parent,
+                                                      uint32_t n_groups, int K, uint32_t row_units, uint32_t blocks_per) {
     const uint32_t og = blockIdx.x / blocks_per, ub = blockIdx.x - og * blocks_per;
-    const uint32_t o = og / (uint32_t)n_groups, g = og - o * n_groups;
+    const uint32_t o = og / n_groups, g = og - o * n_groups;
     const uint32_t u = ub * 256 + threadIdx.x, r = u / row_units, c = u - r * row_units;
-    if (r >= s.n_rows) return;
-    const int64_t base = o * s.outer_stride + (int64_t)g * K * s.seq_stride, row = base + r * s.row_stride;
-    const int32_t *par = parent + g * K;
-    int64_t at = (int64_t)c * sizeof(U);
-    if (at + (int64_t)sizeof(U) <= s.live) {
-        move_beams<U, BM>(dst, src, par, K, s.seq_stride, row + at);
+    const_i32 par = (const_i32)(uintptr_t)(parent + g * K);
+    if constexpr (BM > 16) { // U is 1 or 4 bytes: a row's last bytes singly
+        __shared__ U keep[64 * 256];
+        if (r >= s.n_rows) return;
+        const int64_t at = (int64_t)c * sizeof(U), base = o * s.outer_stride + (int64_t)g * K * s.seq_stride + r * s.row_stride + at;
+        auto source = [&](int j) { return par[j] >= 0 && par[j] < K ? par[j] : j; };
+        auto move = [&](auto z, U *slot, int64_t b) {
+            using V = decltype(z);
+            qmh_move_many(
+                (V *)slot, K,
+                [&](int j, V &u) {
+                    if (source(j) == j && dst == src) return false;
+                    u = *(const V *)(src + b + source(j) * s.seq_stride);
+                    return true;
+                },
+                [&](int j, V u) {
+                    if (source(j) != j || dst != src) *(V *)(dst + b + j * s.seq_stride) = u;
+                });
+        };
+        if (at + (int64_t)sizeof(U) <= s.live) move(U{}, keep + threadIdx.x, base);
+        else
+            for (int64_t k = 0; at + k < s.live; k++) move(uint8_t{}, (U *)((uint8_t *)keep + threadIdx.x), base + k);
         return;
     }
-    while (at < s.live) { // the row's end
-        if (sizeof(U) >= 4 && at + 4 <= s.live) {
-            move_beams<uint32_t, BM>(dst, src, par, K, s.seq_stride, row + at);
-            at += 4;
-        } else {
-            move_beams<uint8_t, BM>(dst, src, par, K, s.seq_stride, row + at);
-            at++;
-        }
+    int from[BM]; // -1: nothing to do
+#pragma unroll
+    for (int j = 0; j < BM; j++) {
+        const int p = par[j < K ? j : 0], f = p >= 0 && p < K ? p : j;
+        from[j] = j >= K || (f == j && dst == src) ? -1 : f;
+    }
+    if (r >= s.n_rows) return;
+    int64_t at = (int64_t)c * sizeof(U);
+    const int64_t base = o * s.outer_stride + (int64_t)g * K * s.seq_stride + r * s.row_stride + at;
+    const uint8_t *f = src + base;
+    uint8_t *t = dst + base;
+    const int64_t left = s.live - at;
+    if (left >= (int64_t)sizeof(U)) {
+        U v[BM];
+#pragma unroll
+        for (int j = 0; j < BM; j++)
+            if (from[j] >= 0) v[j] = *(const U *)(f + from[j] * s.seq_stride);
+#pragma unroll
+        for (int j = 0; j < BM; j++)
+            if (from[j] >= 0) *(U *)(t + j * s.seq_stride) = v[j];
+        return;
+    }
+    int done = 0;
+    if constexpr (sizeof(U) == 16) { // 1 to 3 words
+        const int words = (int)(left >> 2);
+        uint32_t v[BM][3];
+#pragma unroll
+        for (int j = 0; j < BM; j++)
+            if (from[j] >= 0)
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    if (k < words) v[j][k] = *(const uint32_t *)(f + from[j] * s.seq_stride + 4 * k);
+#pragma unroll
+        for (int j = 0; j < BM; j++)
+            if (from[j] >= 0)
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    if (k < words) *(uint32_t *)(t + j * s.seq_stride + 4 * k) = v[j][k];
+        done = 4 * words;
+    }
+    for (; done < left; done++) {
+        uint8_t v[BM];
+#pragma unroll
+        for (int j = 0; j < BM; j++)
+            if (from[j] >= 0) v[j] = f[from[j] * s.seq_stride + done];
+#pragma unroll
+        for (int j = 0; j < BM; j++)
+            if (from[j] >= 0) t[j * s.seq_stride + done] = v[j];
     }
 }
 
@@ -350,8 +389,8 @@ extern "C" int qmh_launch_beam_reorder(const qmh_beam_state *s, void *dst, const
     hipStream_t st = (hipStream_t)stream;
     const uint64_t all = (uint64_t)(uintptr_t)dst | (uint64_t)(uintptr_t)src | (uint64_t)s->seq_stride |
                          (s->n_outer > 1 ? (uint64_t)s->outer_stride : 0) | (s->n_rows > 1 ? (uint64_t)s->row_stride : 0);
-    // past 16 beams a thread's units of all beams take 4 bytes each, so that they stay in registers
-    if (all % 16 == 0 && n_beams <= 16) return reorder_as<uint4>(s, dst, src, parent, n_groups, n_beams, st);
+    // past 16 beams units are of 4 bytes, kept in LDS
+    if (all % 16 == 0 && n_beams <= 16) return reorder_as<v4u>(s, dst, src, parent, n_groups, n_beams, st);
     if (all % 4 == 0) return reorder_as<uint32_t>(s, dst, src, parent, n_groups, n_beams, st);
     return reorder_as<uint8_t>(s, dst, src, parent, n_groups, n_beams, st);
 }

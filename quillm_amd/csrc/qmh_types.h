@@ -24,3 +24,19 @@ static inline void qmh_for_type(int dtype, F body) {
     else if (dtype == QMH_F16) body(qmh_f16{});
     else body(qmh_bf16{});
 }
+
+// Past 16 beams a thread's unit of every beam goes through LDS (slot m * blockDim.x of keep, the thread's own: no barrier),
+// eight loads under way at a time: get(m, u) loads beam m's unit, or says that it does not move, put(m, u) stores it.
+template <typename U, typename G, typename P>
+__device__ __forceinline__ void qmh_move_many(U *keep, int n, G get, P put) {
+    for (int m0 = 0; m0 < n; m0 += 8) {
+        U v[8];
+        bool moves[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) moves[k] = m0 + k < n && get(m0 + k, v[k]);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (moves[k]) keep[(m0 + k) * 256] = v[k];
+    }
+    for (int m = 0; m < n; m++) put(m, keep[m * 256]);
+}
