@@ -11,16 +11,18 @@ namespace {
 
 // --------------------------------------------------------------------------- select
 
-constexpr int SEL_T = 256;   // threads
-constexpr int SEL_CAP = 512; // candidates ranked in LDS
+constexpr int SEL_T = 256;    // threads of the scan
+constexpr int SEL_CAP = 512;  // candidates it ranks in LDS
+constexpr int JOIN_T = 512;   // threads of the join
+constexpr int JOIN_CAP = 1024;
 
-// e^x in 64 bits for x <= 0 (and 0 far below): 2^k times the Taylor polynomial of 2^f, |f| <= 1/2, to degree 10,
-// whose remainder is below (ln 2 / 2)^11 / 11! = 2.2e-13 of the value: far inside the distance of scores that
-// decide a choice, at 10 multiply-adds.
-__device__ __forceinline__ double exp_neg(double x) {
-    double t = x * 1.4426950408889634074;
-    t = t < -1074.0 ? -1074.0 : t; // NaN stays
-    const double k = __builtin_rint(t), f = t - k;
+// e^(x - ref) in 64 bits for x <= ref, both floats, ref finite: x log2 e - ref log2 e = k + f, |f| <= 1/2, and 2^k times the
+// Taylor polynomial of 2^f to degree 10, whose remainder is below (ln 2 / 2)^11 / 11! = 2.2e-13 of the value: far
+// inside the distance of scores that decide a choice. Adding 1.5 2^52 rounds to k and leaves it in the low word. Values
+// below ref - 700 count as that.
+__device__ __forceinline__ double exp_below(float x, float low, double ref2) {
+    const double t = __builtin_fma((double)fmaxf(x, low), 1.4426950408889634074, -ref2);
+    const double s = t + 0x1.8p52, f = t - (s - 0x1.8p52);
     double p = 7.0549116208011233299e-9;
     p = __builtin_fma(p, f, 1.0178086009239699728e-7);
     p = __builtin_fma(p, f, 1.3215486790144309488e-6);
@@ -32,7 +34,7 @@ __device__ __forceinline__ double exp_neg(double x) {
     p = __builtin_fma(p, f, 2.4022650695910071233e-1);
     p = __builtin_fma(p, f, 6.9314718055994530942e-1);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, (int)k);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(s) << 20), __double2loint(p));
 }
 
 // the order of floats as unsigned numbers, -0 as 0; 0 for -inf and NaN, which are no continuations
@@ -60,193 +62,274 @@ __device__ __forceinline__ int block_total(int n, int *buf) {
     return buf[0] + buf[1] + buf[2] + buf[3];
 }
 
-struct scan_out { // of one chunk of one row
-    double sum;   // sum exp(x - max)
+struct scan_head { // a wave's part of a chunk of a row: its maximum and the sum of exp(x - max); NaN: the row has none
+    double sum;
     float max;
-    int count; // candidates that follow, best first
+    int count; // of the chunk (its first wave): candidates that follow, best first
 };
 
-// Chunk blockIdx.x (SEL_T * EPT logits) of row blockIdx.y: its maximum, the sum of exponentials below it in 64 bits, and
-// its n_out best logits in order. The logits stay in registers. A bound below which nothing is among the best
-// is the n_out-th largest of the threads' own maxima; what reaches it (a few more than n_out, unless values repeat)
-// is ranked by counting. Where more than SEL_CAP reach it, the exact bound is searched bit by bit.
+// The largest t that at least n <= 64 of a wave's values reach, 0 if there is none above: bit by bit, by ballots.
+__device__ __forceinline__ uint32_t wave_nth(uint32_t v, int n) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t u = t | 1u << b;
+        t = __popcll(__ballot(v >= u)) >= n ? u : t;
+    }
+    return t;
+}
+
+// Chunk blockIdx.x (SEL_T * EPT logits) of a row: each wave's maximum and sum of exponentials below it, in 64 bits,
+// and the chunk's n_out best logits in order. The logits stay in registers. Below the n_out-th largest of the lanes'
+// own maxima in a wave nothing is among the best; what reaches the largest such bound of the four waves (a few times n_out,
+// unless values repeat) is ranked by counting. Where more than SEL_CAP reach it, the exact bound is searched bit by bit.
 template <typename T, int EPT, int VEC>
-__global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_out *heads, uint2 *cands,
-                                                     int row0) {
-    __shared__ uint32_t tmax[SEL_T];
+__global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_head *heads, uint2 *cands, int row0) {
     __shared__ uint2 cand[SEL_CAP];
-    __shared__ double red[4];
-    __shared__ float redf[4];
     __shared__ int cnt[4], ncand;
-    __shared__ uint32_t bound;
-    const int tid = threadIdx.x, row = row0 + blockIdx.y, n_out = a.n_out;
+    __shared__ uint32_t bounds[4];
+    const int tid = threadIdx.x, w = tid >> 6, row = row0 + blockIdx.y, n_out = a.n_out;
     const int64_t slot = (int64_t)row * gridDim.x + blockIdx.x;
     if ((a.done && a.done[row]) || !(a.score[row] > -__builtin_inff())) return; // the join does not look at it
     const T *x = (const T *)a.logits + row * a.stride;
     // vectors from the row's start rounded down to a vector: the ones that hold some element of the row
     const int skew = VEC > 1 ? (int)(((uintptr_t)x / sizeof(T)) % VEC) : 0;
     const int base = (int)blockIdx.x * SEL_T * EPT - skew;
-    uint32_t key[EPT];
-    float top = -__builtin_inff();
     float xs[EPT];
+    {
+        qmh_vec<T, VEC> v[EPT / VEC];
 #pragma unroll
-    for (int k = 0; k < EPT / VEC; k++) {
-        const int i = base + (k * SEL_T + tid) * VEC;
-        qmh_vec<T, VEC> v;
-        const bool some = i + VEC > 0 && i < a.vocab;
-        if (some) v = *(const qmh_vec<T, VEC> *)(x + i);
+        for (int k = 0; k < EPT / VEC; k++) {
+            const int i = base + (k * SEL_T + tid) * VEC;
+            if (i + VEC > 0 && i < a.vocab) v[k] = *(const qmh_vec<T, VEC> *)(x + i);
+        }
 #pragma unroll
-        for (int e = 0; e < VEC; e++)
-            xs[k * VEC + e] = some && i + e >= 0 && i + e < a.vocab ? qmh_to_f(v.e[e]) : -__builtin_inff();
+        for (int k = 0; k < EPT / VEC; k++) {
+            const int i = base + (k * SEL_T + tid) * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) xs[k * VEC + e] = (uint32_t)(i + e) < (uint32_t)a.vocab ? qmh_to_f(v[k].e[e]) : -__builtin_inff();
+        }
     }
-#pragma unroll
-    for (int k = 0; k < EPT; k++) top = fmaxf(top, xs[k]);
-    const float m = qmh_block_max(top, redf);
-    const float ref = m == -__builtin_inff() ? 0.0f : m;
-    double sum = 0.0;
-    uint32_t mine = 0;
-#pragma unroll
-    for (int k = 0; k < EPT; k++) {
-        sum += exp_neg((double)xs[k] - (double)ref); // NaN where x is NaN or +inf: the row then has no continuation
-        key[k] = key_of(xs[k]);
-        mine = key[k] > mine ? key[k] : mine;
-    }
-    sum = qmh_block_sum_d(sum, red);
-    auto index = [&](int k) { return base + ((k / VEC) * SEL_T + tid) * VEC + k % VEC; };
-    // the n_out-th largest of the threads' maxima (0: fewer have one)
-    tmax[tid] = mine;
     if (tid == 0) ncand = 0;
+    float top = xs[0];
+#pragma unroll
+    for (int k = 1; k < EPT; k++) top = __builtin_elementwise_maximum(top, xs[k]); // NaN if one is
+    const bool bad = __any(!(top < __builtin_inff()));
+    const float m = qmh_wave_max(top), ref = m > -__builtin_inff() && m < __builtin_inff() ? m : 0.0f;
+    // the bound first: it is short and the sums' latency hides in it
+    uint32_t mine = key_of(top);
+    if (bad) { // NaN hides the lane's maximum
+        mine = 0;
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            const uint32_t q = key_of(xs[k]);
+            mine = q > mine ? q : mine;
+        }
+    }
+    const uint32_t bw = wave_nth(mine, n_out);
+    if ((tid & 63) == 0) bounds[w] = bw;
+    const double ref2 = (double)ref * 1.4426950408889634074;
+    const float low = ref - 700.0f;
+    double sum = 0.0, sum2 = 0.0;
+#pragma unroll
+    for (int k = 0; k < EPT; k += 2) {
+        sum += exp_below(xs[k], low, ref2);
+        sum2 += exp_below(xs[k + 1], low, ref2);
+    }
+    sum = qmh_wave_sum_d(sum + sum2);
     __syncthreads();
-    int rank = 0;
-    for (int i = 0; i < SEL_T; i++) rank += tmax[i] > mine || (tmax[i] == mine && i < tid);
-    if (rank == n_out - 1) bound = mine;
-    __syncthreads();
-    uint32_t from = bound ? bound : 1u;
+    uint32_t from = bounds[0];
+#pragma unroll
+    for (int k = 1; k < 4; k++) from = bounds[k] > from ? bounds[k] : from;
+    from = from ? from : 1u;
+    auto index = [&](int k) { return base + ((k / VEC) * SEL_T + tid) * VEC + k % VEC; };
     int reach = 0;
 #pragma unroll
-    for (int k = 0; k < EPT; k++) reach += key[k] >= from;
+    for (int k = 0; k < EPT; k++) reach += key_of(xs[k]) >= from;
+    int at = reach ? atomicAdd(&ncand, reach) : 0;
+    __syncthreads();
     int last = 0x7fffffff; // candidates equal to the bound: only up to this index
-    if (block_total(reach, cnt) > SEL_CAP) {
+    if (ncand > SEL_CAP) {
         // the largest bound that n_out keys reach, then the lowest indexes among the keys equal to it
         from = 0;
         for (int b = 31; b >= 0; b--) {
             const uint32_t t = from | 1u << b;
             int n = 0;
 #pragma unroll
-            for (int k = 0; k < EPT; k++) n += key[k] >= t;
+            for (int k = 0; k < EPT; k++) n += key_of(xs[k]) >= t;
             if (block_total(n, cnt) >= n_out) from = t;
         }
         int above = 0;
 #pragma unroll
-        for (int k = 0; k < EPT; k++) above += key[k] > from;
+        for (int k = 0; k < EPT; k++) above += key_of(xs[k]) > from;
         above = block_total(above, cnt);
         int lo = -1; // the largest index that leaves fewer than n_out
         for (int b = 24; b >= 0; b--) {
             const int t = lo + (1 << b);
             int n = 0;
 #pragma unroll
-            for (int k = 0; k < EPT; k++) n += key[k] == from && index(k) <= t;
+            for (int k = 0; k < EPT; k++) n += key_of(xs[k]) == from && index(k) <= t;
             if (above + block_total(n, cnt) < n_out) lo = t;
         }
         last = lo + 1;
-    }
+        if (tid == 0) ncand = 0;
+        __syncthreads();
+        reach = 0;
 #pragma unroll
-    for (int k = 0; k < EPT; k++)
-        if (key[k] > from || (key[k] == from && index(k) <= last)) cand[atomicAdd(&ncand, 1)] = make_uint2(key[k], (uint32_t)index(k));
+        for (int k = 0; k < EPT; k++) reach += key_of(xs[k]) > from || (key_of(xs[k]) == from && index(k) <= last);
+        at = reach ? atomicAdd(&ncand, reach) : 0;
+        __syncthreads();
+    }
+    if (reach)
+#pragma unroll
+        for (int k = 0; k < EPT; k++) {
+            const uint32_t q = key_of(xs[k]);
+            if (q > from || (q == from && index(k) <= last)) cand[at++] = make_uint2(q, (uint32_t)index(k));
+        }
     __syncthreads();
     const int n = ncand;
     for (int c = tid; c < n; c += SEL_T) {
         const uint2 v = cand[c];
         int r = 0;
-        for (int i = 0; i < n; i++) r += cand[i].x > v.x || (cand[i].x == v.x && cand[i].y < v.y);
+        for (int i = 0; i < n; i++) {
+            const uint2 u = cand[i];
+            r += u.x > v.x || (u.x == v.x && u.y < v.y);
+        }
         if (r < n_out) cands[slot * n_out + r] = v;
     }
-    if (tid == 0) heads[slot] = scan_out{sum, m, n < n_out ? n : n_out};
+    if ((tid & 63) == 0) heads[slot * 4 + w] = scan_head{bad ? __builtin_nan("") : m > -__builtin_inff() ? sum : 0.0, m, n < n_out ? n : n_out};
 }
 
-// A group's choice from its rows' chunks: each row's log sum, then the n_out best totals, found one after another.
-__global__ __launch_bounds__(SEL_T) void k_beam_join(const qmh_beam_args a, const scan_out *heads, const uint2 *cands,
-                                                     int chunks) {
-    __shared__ double lse[64];
-    __shared__ uint64_t bk[4], chosen[64];
-    __shared__ uint32_t bf[4], where[64];
-    const int g = blockIdx.x, tid = threadIdx.x, K = a.n_beams, n_out = a.n_out;
-    auto alive = [&](int row) { return !(a.done && a.done[row]) && a.score[row] > -__builtin_inff(); };
-    for (int b = tid; b < K; b += SEL_T) {
+// A group's choice from its rows' chunks: each row's log sum (a wave a row), then the n_out best totals as in the scan:
+// a bound from the lanes' best, what reaches it ranked in LDS. Where more than JOIN_CAP reach it, one after another.
+__global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int chunks) {
+    constexpr int NW = JOIN_T / 64;
+    __shared__ double lse[64], score[64];
+    __shared__ uint64_t ckey[JOIN_CAP], bk[NW];
+    __shared__ uint32_t cplace[JOIN_CAP], bounds[NW], bf[NW];
+    __shared__ int ncand;
+    const int g = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63, K = a.n_beams, n_out = a.n_out;
+    if (tid == 0) ncand = 0;
+    for (int b = w; b < K; b += NW) {
         const int row = g * K + b;
-        double s = __builtin_nan(""), m = 0.0;
-        if (alive(row)) {
-            const scan_out *h = heads + (int64_t)row * chunks;
-            float top = -__builtin_inff();
-            for (int c = 0; c < chunks; c++) top = fmaxf(top, h[c].max);
-            if (top > -__builtin_inff()) {
-                m = (double)top;
-                s = 0.0;
-                for (int c = 0; c < chunks; c++)
-                    if (h[c].max > -__builtin_inff() || h[c].sum != h[c].sum) s += h[c].sum * exp((double)h[c].max - m);
-            }
+        const float sc = a.score[row];
+        const bool done = a.done && a.done[row];
+        double s = __builtin_nan("");
+        if (!done && sc > -__builtin_inff()) {
+            const scan_head *h = heads + (int64_t)row * chunks * 4;
+            float m = -__builtin_inff();
+            for (int c = lane; c < chunks * 4; c += 64) m = fmaxf(m, h[c].max);
+            m = qmh_wave_max(m);
+            s = 0.0;
+            const double ref2 = (double)m * 1.4426950408889634074;
+            for (int c = lane; c < chunks * 4; c += 64) s = __builtin_fma(h[c].sum, exp_below(h[c].max, m - 700.0f, ref2), s);
+            s = (double)m + log(qmh_wave_sum_d(s)); // a row without a logit: NaN or -inf, and no continuation
         }
-        lse[b] = m + log(s);
+        if (lane == 0) {
+            lse[b] = s;
+            score[b] = done ? -(double)sc : (double)sc;
+            if (done) lse[b] = __builtin_inf(); // marks a finished row
+        }
     }
     __syncthreads();
+    const int per = chunks * n_out, all = K * per;
+    // candidate i's total as an ordered key (0: none) and its place, beam * vocab + token
+    auto key_at = [&](int i, uint32_t &place) -> uint64_t {
+        const int b = i / per, row = g * K + b, j = i - b * per, c = j / n_out, r = j - c * n_out;
+        const double L = lse[b];
+        if (L == __builtin_inf()) { // finished: one continuation
+            place = (uint32_t)(b * a.vocab + a.eos);
+            return j == 0 ? key_of_d(-score[b]) : 0ull;
+        }
+        if (L != L || r >= heads[((int64_t)row * chunks + c) * 4].count) return 0ull;
+        const uint2 v = cands[((int64_t)row * chunks + c) * n_out + r];
+        place = (uint32_t)(b * a.vocab) + v.y;
+        return key_of_d(score[b] + ((double)of_key(v.x) - L));
+    };
+    uint32_t mine = 0, place = 0;
+    for (int i = tid; i < all; i += JOIN_T) {
+        const uint32_t q = (uint32_t)(key_at(i, place) >> 32);
+        mine = q > mine ? q : mine;
+    }
+    const uint32_t bw = wave_nth(mine, n_out);
+    if (lane == 0) bounds[w] = bw;
+    __syncthreads();
+    uint32_t from = 1;
+#pragma unroll
+    for (int k = 0; k < NW; k++) from = bounds[k] > from ? bounds[k] : from;
+    for (int i = tid; i < all; i += JOIN_T) {
+        const uint64_t q = key_at(i, place);
+        if ((uint32_t)(q >> 32) >= from) {
+            const int at = atomicAdd(&ncand, 1);
+            if (at < JOIN_CAP) {
+                ckey[at] = q;
+                cplace[at] = place;
+            }
+        }
+    }
+    __syncthreads();
+    auto write = [&](int o, uint64_t k, uint32_t p) {
+        const int64_t at = (int64_t)g * n_out + o;
+        a.out_score[at] = k ? (float)of_key_d(k) : -__builtin_inff();
+        a.out_parent[at] = k ? (int)(p / (uint32_t)a.vocab) : -1;
+        a.out_token[at] = k ? (int)(p % (uint32_t)a.vocab) : -1;
+    };
+    const int n = ncand;
+    if (n <= JOIN_CAP) { // every score has been read: out_score may be score
+        for (int c = tid; c < n; c += JOIN_T) {
+            const uint64_t q = ckey[c];
+            const uint32_t p = cplace[c];
+            int r = 0;
+            for (int i = 0; i < n; i++) {
+                const uint64_t u = ckey[i];
+                r += u > q || (u == q && cplace[i] < p);
+            }
+            if (r < n_out) write(r, q, p);
+        }
+        if (tid >= n && tid < n_out) write(tid, 0, 0);
+        return;
+    }
     uint64_t below = ~0ull; // what was chosen last: its total, then its place
-    int64_t place = -1;
+    int64_t after = -1;
     for (int o = 0; o < n_out; o++) {
         uint64_t best = 0;
-        uint32_t at = 0xffffffffu; // beam * vocab + token
-        auto offer = [&](double total, uint32_t p) {
-            const uint64_t k = key_of_d(total);
-            if (!k || k > below || (k == below && (int64_t)p <= place)) return;
-            if (k > best || (k == best && p < at)) {
-                best = k;
-                at = p;
+        uint32_t at = 0xffffffffu;
+        for (int i = tid; i < all; i += JOIN_T) {
+            const uint64_t q = key_at(i, place);
+            if (!q || q > below || (q == below && (int64_t)place <= after)) continue;
+            if (q > best || (q == best && place < at)) {
+                best = q;
+                at = place;
             }
-        };
-        const int per = chunks * n_out;
-        for (int i = tid; i < K * per; i += SEL_T) {
-            const int b = i / per, row = g * K + b;
-            if (!alive(row)) continue;
-            const int c = (i - b * per) / n_out, r = i % n_out;
-            if (r >= heads[(int64_t)row * chunks + c].count) continue;
-            const uint2 v = cands[((int64_t)row * chunks + c) * n_out + r];
-            offer((double)a.score[row] + ((double)of_key(v.x) - lse[b]), (uint32_t)(b * a.vocab) + v.y);
         }
-        for (int b = tid; b < K; b += SEL_T)
-            if (a.done && a.done[g * K + b]) offer((double)a.score[g * K + b], (uint32_t)(b * a.vocab + a.eos));
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint64_t ok = __shfl_xor((unsigned long long)best, s);
-            const uint32_t op = __shfl_xor(at, s);
-            if (ok > best || (ok == best && op < at)) {
-                best = ok;
+        for (int x = 1; x < 64; x <<= 1) {
+            const uint64_t oq = __shfl_xor((unsigned long long)best, x);
+            const uint32_t op = __shfl_xor(at, x);
+            if (oq > best || (oq == best && op < at)) {
+                best = oq;
                 at = op;
             }
         }
         __syncthreads();
-        if ((tid & 63) == 0) {
-            bk[tid >> 6] = best;
-            bf[tid >> 6] = at;
+        if (lane == 0) {
+            bk[w] = best;
+            bf[w] = at;
         }
         __syncthreads();
-        for (int w = 0; w < 4; w++)
-            if (bk[w] > best || (bk[w] == best && bf[w] < at)) {
-                best = bk[w];
-                at = bf[w];
+        for (int k = 0; k < NW; k++)
+            if (bk[k] > best || (bk[k] == best && bf[k] < at)) {
+                best = bk[k];
+                at = bf[k];
             }
         below = best;
-        place = at;
+        after = at;
         if (tid == 0) {
-            chosen[o] = best;
-            where[o] = at;
+            ckey[o] = best;
+            cplace[o] = at;
         }
     }
-    __syncthreads(); // every score has been read: out_score may be score
-    if (tid < n_out) {
-        const uint64_t k = chosen[tid];
-        const int64_t o = (int64_t)g * n_out + tid;
-        a.out_score[o] = k ? (float)of_key_d(k) : -__builtin_inff();
-        a.out_parent[o] = k ? (int)(where[tid] / (uint32_t)a.vocab) : -1;
-        a.out_token[o] = k ? (int)(where[tid] % (uint32_t)a.vocab) : -1;
-    }
+    __syncthreads();
+    if (tid < n_out) write(tid, ckey[tid], cplace[tid]);
 }
 
 int scan_chunks(const qmh_beam_args *a, int ept) { return (a->vocab + 15 + SEL_T * ept - 1) / (SEL_T * ept); }
@@ -345,14 +428,14 @@ __global__ __launch_bounds__(256, BM > 16 ? 2 : 4) void k_beam_reorder(const qmh
 
 extern "C" size_t qmh_beam_ws_bytes(const qmh_beam_args *a) {
     const size_t slots = (size_t)a->n_groups * a->n_beams * scan_chunks(a, scan_ept(a));
-    return slots * (sizeof(scan_out) + a->n_out * sizeof(uint2));
+    return slots * (4 * sizeof(scan_head) + a->n_out * sizeof(uint2));
 }
 
 extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *stream) {
     hipStream_t st = (hipStream_t)stream;
     const int rows = a->n_groups * a->n_beams, ept = scan_ept(a), chunks = scan_chunks(a, ept);
-    scan_out *heads = (scan_out *)ws;
-    uint2 *cands = (uint2 *)(heads + (size_t)rows * chunks);
+    scan_head *heads = (scan_head *)ws;
+    uint2 *cands = (uint2 *)(heads + (size_t)rows * chunks * 4);
     qmh_for_type(a->dtype, [&](auto z) {
         using T = decltype(z);
         constexpr int VEC = 16 / sizeof(T);
@@ -363,7 +446,7 @@ extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *st
             else hipLaunchKernelGGL((k_beam_scan<T, 32, VEC>), g, t, 0, st, *a, heads, cands, r0);
         }
     });
-    hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(SEL_T), 0, st, *a, heads, cands, chunks);
+    hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, chunks);
     return (int)hipGetLastError();
 }
 
