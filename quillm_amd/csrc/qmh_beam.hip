@@ -64,8 +64,7 @@ __device__ __forceinline__ int block_total(int n, int *buf) {
 
 struct scan_head { // a wave's part of a chunk of a row: its maximum and the sum of exp(x - max); NaN: the row has none
     double sum;
-    float max;
-    int count; // of the chunk (its first wave): candidates that follow, best first
+    float max, pad;
 };
 
 // The largest t that at least n <= 64 of a wave's values reach, 0 if there is none above: bit by bit, by ballots.
@@ -77,6 +76,23 @@ __device__ __forceinline__ uint32_t wave_nth(uint32_t v, int n) {
         t = __popcll(__ballot(v >= u)) >= n ? u : t;
     }
     return t;
+}
+
+// done(c, rank) for each of n candidates: its rank is how many others are before(i, c) it, counted by as many neighbouring
+// threads as there are for each (a power of two up to 64). All threads of the workgroup take part.
+template <typename B, typename D>
+__device__ __forceinline__ void rank_all(int n, int threads, B before, D done) {
+    int per = 1;
+    while (per < 64 && 2 * per * n <= threads) per *= 2;
+    const int tid = threadIdx.x, part = tid & (per - 1);
+    for (int c0 = 0; c0 < n; c0 += threads / per) {
+        const int c = c0 + tid / per;
+        int r = 0;
+        if (c < n)
+            for (int i = part; i < n; i += per) r += before(i, c);
+        for (int x = 1; x < per; x *= 2) r += __shfl_xor(r, x);
+        if (c < n && part == 0) done(c, r);
+    }
 }
 
 // Chunk blockIdx.x (SEL_T * EPT logits) of a row: each wave's maximum and sum of exponentials below it, in 64 bits,
@@ -104,12 +120,13 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
             if (i + VEC > 0 && i < a.vocab) v[k] = *(const qmh_vec<T, VEC> *)(x + i);
         }
 #pragma unroll
-        for (int k = 0; k < EPT / VEC; k++) {
-            const int i = base + (k * SEL_T + tid) * VEC;
-#pragma unroll
-            for (int e = 0; e < VEC; e++) xs[k * VEC + e] = (uint32_t)(i + e) < (uint32_t)a.vocab ? qmh_to_f(v[k].e[e]) : -__builtin_inff();
-        }
+        for (int k = 0; k < EPT; k++) xs[k] = qmh_to_f(v[k / VEC].e[k % VEC]);
     }
+    auto index = [&](int k) { return base + ((k / VEC) * SEL_T + tid) * VEC + k % VEC; };
+    if (base < 0 || base + SEL_T * EPT > a.vocab) // the row's ends
+#pragma unroll
+        for (int k = 0; k < EPT; k++)
+            if ((uint32_t)index(k) >= (uint32_t)a.vocab) xs[k] = -__builtin_inff();
     if (tid == 0) ncand = 0;
     float top = xs[0];
 #pragma unroll
@@ -141,11 +158,11 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
     uint32_t from = bounds[0];
 #pragma unroll
     for (int k = 1; k < 4; k++) from = bounds[k] > from ? bounds[k] : from;
-    from = from ? from : 1u;
-    auto index = [&](int k) { return base + ((k / VEC) * SEL_T + tid) * VEC + k % VEC; };
+    // as a float (at least the lowest finite one): -inf and NaN never reach it
+    float at_least = of_key(from ? from : 0x00800000u);
     int reach = 0;
 #pragma unroll
-    for (int k = 0; k < EPT; k++) reach += key_of(xs[k]) >= from;
+    for (int k = 0; k < EPT; k++) reach += xs[k] >= at_least;
     int at = reach ? atomicAdd(&ncand, reach) : 0;
     __syncthreads();
     int last = 0x7fffffff; // candidates equal to the bound: only up to this index
@@ -172,6 +189,7 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
             if (above + block_total(n, cnt) < n_out) lo = t;
         }
         last = lo + 1;
+        at_least = of_key(from);
         if (tid == 0) ncand = 0;
         __syncthreads();
         reach = 0;
@@ -182,22 +200,17 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
     }
     if (reach)
 #pragma unroll
-        for (int k = 0; k < EPT; k++) {
-            const uint32_t q = key_of(xs[k]);
-            if (q > from || (q == from && index(k) <= last)) cand[at++] = make_uint2(q, (uint32_t)index(k));
-        }
+        for (int k = 0; k < EPT; k++)
+            if (xs[k] > at_least || (xs[k] == at_least && index(k) <= last)) cand[at++] = make_uint2(key_of(xs[k]), (uint32_t)index(k));
     __syncthreads();
     const int n = ncand;
-    for (int c = tid; c < n; c += SEL_T) {
-        const uint2 v = cand[c];
-        int r = 0;
-        for (int i = 0; i < n; i++) {
-            const uint2 u = cand[i];
-            r += u.x > v.x || (u.x == v.x && u.y < v.y);
-        }
-        if (r < n_out) cands[slot * n_out + r] = v;
-    }
-    if ((tid & 63) == 0) heads[slot * 4 + w] = scan_head{bad ? __builtin_nan("") : m > -__builtin_inff() ? sum : 0.0, m, n < n_out ? n : n_out};
+    rank_all(
+        n, SEL_T, [&](int i, int c) { return cand[i].x > cand[c].x || (cand[i].x == cand[c].x && cand[i].y < cand[c].y); },
+        [&](int c, int r) {
+            if (r < n_out) cands[slot * n_out + r] = cand[c];
+        });
+    if (tid >= n && tid < n_out) cands[slot * n_out + tid] = make_uint2(0, 0);
+    if ((tid & 63) == 0) heads[slot * 4 + w] = scan_head{bad ? __builtin_nan("") : m > -__builtin_inff() ? sum : 0.0, m, 0.0f};
 }
 
 // A group's choice from its rows' chunks: each row's log sum (a wave a row), then the n_out best totals as in the scan:
@@ -232,41 +245,43 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
         }
     }
     __syncthreads();
-    const int per = chunks * n_out, all = K * per;
-    // candidate i's total as an ordered key (0: none) and its place, beam * vocab + token
-    auto key_at = [&](int i, uint32_t &place) -> uint64_t {
-        const int b = i / per, row = g * K + b, j = i - b * per, c = j / n_out, r = j - c * n_out;
+    // a wave's own rows: lane's j-th candidate of row b as an ordered key (0: none), its place beam * vocab + token
+    const int per = chunks * n_out;
+    auto key_at = [&](int b, int j, uint32_t &place) -> uint64_t {
         const double L = lse[b];
         if (L == __builtin_inf()) { // finished: one continuation
             place = (uint32_t)(b * a.vocab + a.eos);
             return j == 0 ? key_of_d(-score[b]) : 0ull;
         }
-        if (L != L || r >= heads[((int64_t)row * chunks + c) * 4].count) return 0ull;
-        const uint2 v = cands[((int64_t)row * chunks + c) * n_out + r];
+        const uint2 v = cands[(int64_t)(g * K + b) * per + j];
         place = (uint32_t)(b * a.vocab) + v.y;
-        return key_of_d(score[b] + ((double)of_key(v.x) - L));
+        return v.x && L == L ? key_of_d(score[b] + ((double)of_key(v.x) - L)) : 0ull;
     };
-    uint32_t mine = 0, place = 0;
-    for (int i = tid; i < all; i += JOIN_T) {
-        const uint32_t q = (uint32_t)(key_at(i, place) >> 32);
-        mine = q > mine ? q : mine;
-    }
+    auto each = [&](auto body) {
+        uint32_t place = 0;
+        for (int b = w; b < K; b += NW) {
+            for (int j = lane; j < per; j += 64) {
+                const uint64_t q = key_at(b, j, place);
+                if (q) body(q, place);
+            }
+        }
+    };
+    uint32_t mine = 0;
+    each([&](uint64_t q, uint32_t) { mine = (uint32_t)(q >> 32) > mine ? (uint32_t)(q >> 32) : mine; });
     const uint32_t bw = wave_nth(mine, n_out);
     if (lane == 0) bounds[w] = bw;
     __syncthreads();
     uint32_t from = 1;
 #pragma unroll
     for (int k = 0; k < NW; k++) from = bounds[k] > from ? bounds[k] : from;
-    for (int i = tid; i < all; i += JOIN_T) {
-        const uint64_t q = key_at(i, place);
-        if ((uint32_t)(q >> 32) >= from) {
-            const int at = atomicAdd(&ncand, 1);
-            if (at < JOIN_CAP) {
-                ckey[at] = q;
-                cplace[at] = place;
-            }
+    each([&](uint64_t q, uint32_t place) {
+        if ((uint32_t)(q >> 32) < from) return;
+        const int at = atomicAdd(&ncand, 1);
+        if (at < JOIN_CAP) {
+            ckey[at] = q;
+            cplace[at] = place;
         }
-    }
+    });
     __syncthreads();
     auto write = [&](int o, uint64_t k, uint32_t p) {
         const int64_t at = (int64_t)g * n_out + o;
@@ -276,16 +291,11 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     };
     const int n = ncand;
     if (n <= JOIN_CAP) { // every score has been read: out_score may be score
-        for (int c = tid; c < n; c += JOIN_T) {
-            const uint64_t q = ckey[c];
-            const uint32_t p = cplace[c];
-            int r = 0;
-            for (int i = 0; i < n; i++) {
-                const uint64_t u = ckey[i];
-                r += u > q || (u == q && cplace[i] < p);
-            }
-            if (r < n_out) write(r, q, p);
-        }
+        rank_all(
+            n, JOIN_T, [&](int i, int c) { return ckey[i] > ckey[c] || (ckey[i] == ckey[c] && cplace[i] < cplace[c]); },
+            [&](int c, int r) {
+                if (r < n_out) write(r, ckey[c], cplace[c]);
+            });
         if (tid >= n && tid < n_out) write(tid, 0, 0);
         return;
     }
@@ -294,14 +304,13 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     for (int o = 0; o < n_out; o++) {
         uint64_t best = 0;
         uint32_t at = 0xffffffffu;
-        for (int i = tid; i < all; i += JOIN_T) {
-            const uint64_t q = key_at(i, place);
-            if (!q || q > below || (q == below && (int64_t)place <= after)) continue;
+        each([&](uint64_t q, uint32_t place) {
+            if (q > below || (q == below && (int64_t)place <= after)) return;
             if (q > best || (q == best && place < at)) {
                 best = q;
                 at = place;
             }
-        }
+        });
         for (int x = 1; x < 64; x <<= 1) {
             const uint64_t oq = __shfl_xor((unsigned long long)best, x);
             const uint32_t op = __shfl_xor(at, x);
