@@ -12,29 +12,39 @@ namespace {
 // --------------------------------------------------------------------------- select
 
 constexpr int SEL_T = 256;    // threads of the scan
-constexpr int SEL_CAP = 512;  // candidates it ranks in LDS
+constexpr int SEL_CAP = 256;  // candidates a wave of it lists
 constexpr int JOIN_T = 512;   // threads of the join
 constexpr int JOIN_CAP = 1024;
 
-// e^(x - ref) in 64 bits for x <= ref, both floats, ref finite: x log2 e - ref log2 e = k + f, |f| <= 1/2, and 2^k times the
-// Taylor polynomial of 2^f to degree 10, whose remainder is below (ln 2 / 2)^11 / 11! = 2.2e-13 of the value: far
-// inside the distance of scores that decide a choice. Adding 1.5 2^52 rounds to k and leaves it in the low word. Values
-// below ref - 700 count as that.
-__device__ __forceinline__ double exp_below(float x, float low, double ref2) {
-    const double t = __builtin_fma((double)fmaxf(x, low), 1.4426950408889634074, -ref2);
-    const double s = t + 0x1.8p52, f = t - (s - 0x1.8p52);
-    double p = 7.0549116208011233299e-9;
-    p = __builtin_fma(p, f, 1.0178086009239699728e-7);
-    p = __builtin_fma(p, f, 1.3215486790144309488e-6);
-    p = __builtin_fma(p, f, 1.5252733804059840280e-5);
-    p = __builtin_fma(p, f, 1.5403530393381609954e-4);
-    p = __builtin_fma(p, f, 1.3333558146428443423e-3);
-    p = __builtin_fma(p, f, 9.6181291076284771619e-3);
-    p = __builtin_fma(p, f, 5.5504108664821579953e-2);
-    p = __builtin_fma(p, f, 2.4022650695910071233e-1);
-    p = __builtin_fma(p, f, 6.9314718055994530942e-1);
-    p = __builtin_fma(p, f, 1.0);
-    return __hiloint2double(__double2hiint(p) + (__double2loint(s) << 20), __double2loint(p));
+// The sum of e^(x - ref) over N floats, in 64 bits, x at most 600 above ref (finite): x log2 e - ref log2 e = k + f,
+// |f| <= 1/2, and 2^k times the Taylor polynomial of 2^f to degree 10, whose remainder is below
+// (ln 2 / 2)^11 / 11! = 2.2e-13 of the value: far inside the distance of scores that decide a choice. Adding 1.5 2^52
+// rounds to k and leaves it in the low word. Values below low = ref - 700 count as that. The N chains run side by side.
+template <int N>
+__device__ __forceinline__ double exp_sum(const float *x, float low, double ref2) {
+    constexpr double c[10] = {1.0178086009239699728e-7, 1.3215486790144309488e-6, 1.5252733804059840280e-5, 1.5403530393381609954e-4,
+                              1.3333558146428443423e-3, 9.6181291076284771619e-3, 5.5504108664821579953e-2, 2.4022650695910071233e-1,
+                              6.9314718055994530942e-1, 1.0};
+    double t[N], s[N], p[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) t[j] = __builtin_fma((double)fmaxf(x[j], low), 1.4426950408889634074, -ref2);
+#pragma unroll
+    for (int j = 0; j < N; j++) s[j] = t[j] + 0x1.8p52;
+#pragma unroll
+    for (int j = 0; j < N; j++) t[j] = t[j] - (s[j] - 0x1.8p52);
+#pragma unroll
+    for (int j = 0; j < N; j++) p[j] = 7.0549116208011233299e-9;
+#pragma unroll
+    for (int k = 0; k < 10; k++)
+#pragma unroll
+        for (int j = 0; j < N; j++) p[j] = __builtin_fma(p[j], t[j], c[k]);
+#pragma unroll
+    for (int j = 0; j < N; j++) p[j] = __hiloint2double(__double2hiint(p[j]) + (__double2loint(s[j]) << 20), __double2loint(p[j]));
+#pragma unroll
+    for (int n = N; n > 1; n /= 2)
+#pragma unroll
+        for (int j = 0; j < n / 2; j++) p[j] += p[j + n / 2];
+    return p[0];
 }
 
 // the order of floats as unsigned numbers, -0 as 0; 0 for -inf and NaN, which are no continuations
@@ -53,18 +63,9 @@ __device__ __forceinline__ double of_key_d(uint64_t k) {
     return __longlong_as_double((long long)((k >> 63) ? k ^ (1ull << 63) : ~k));
 }
 
-// the sum of n over the workgroup
-__device__ __forceinline__ int block_total(int n, int *buf) {
-    for (int s = 1; s < 64; s <<= 1) n += __shfl_xor(n, s);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = n;
-    __syncthreads();
-    return buf[0] + buf[1] + buf[2] + buf[3];
-}
-
-struct scan_head { // a wave's part of a chunk of a row: its maximum and the sum of exp(x - max); NaN: the row has none
+struct scan_head { // a wave's part of a segment of a row: the sum of exp(x - ref); NaN: the row has no continuation
     double sum;
-    float max, pad;
+    float ref, pad;
 };
 
 // The largest t that at least n <= 64 of a wave's values reach, 0 if there is none above: bit by bit, by ballots.
@@ -95,127 +96,206 @@ __device__ __forceinline__ void rank_all(int n, int threads, B before, D done) {
     }
 }
 
-// Chunk blockIdx.x (SEL_T * EPT logits) of a row: each wave's maximum and sum of exponentials below it, in 64 bits,
-// and the chunk's n_out best logits in order. The logits stay in registers. Below the n_out-th largest of the lanes'
-// own maxima in a wave nothing is among the best; what reaches the largest such bound of the four waves (a few times n_out,
-// unless values repeat) is ranked by counting. Where more than SEL_CAP reach it, the exact bound is searched bit by bit.
+// what a wave wrote to LDS is there for all its lanes
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wave takes a segment of a row, iters pieces of 64 EPT logits, in one pass with no word to the other waves: the sum of
+// exponentials in 64 bits, and the segment's n_out best logits. A piece is in registers while the next one's loads are
+// under way. Candidates go to a list in LDS, placed by ballots. What may be one is told by a bound: at first the
+// n_out-th largest of the lanes' own maxima (below it nothing is among the best); when the list is cut down to its
+// n_out best, the least of them, which only larger logits pass, since later ones lose a tie. Where a piece brings
+// more than the list holds (a rising row, repeated values) its own lane maxima raise the bound, and if that does not help
+// the exact bound of the piece is searched bit by bit.
 template <typename T, int EPT, int VEC>
-__global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_head *heads, uint2 *cands, int row0) {
-    __shared__ uint2 cand[SEL_CAP];
-    __shared__ int cnt[4], ncand;
-    __shared__ uint32_t bounds[4];
-    const int tid = threadIdx.x, w = tid >> 6, row = row0 + blockIdx.y, n_out = a.n_out;
-    const int64_t slot = (int64_t)row * gridDim.x + blockIdx.x;
+__global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_head *heads, uint2 *cands, int row0, int iters) {
+    constexpr int PIECE = 64 * EPT;
+    __shared__ uint2 lists[SEL_T / 64][SEL_CAP];
+    const int lane = threadIdx.x & 63, row = row0 + blockIdx.y, n_out = a.n_out;
+    const int seg = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (SEL_T / 64) + (threadIdx.x >> 6)));
     if ((a.done && a.done[row]) || !(a.score[row] > -__builtin_inff())) return; // the join does not look at it
+    uint2 *list = lists[threadIdx.x >> 6];
+    const int64_t slot = (int64_t)row * (gridDim.x * (SEL_T / 64)) + seg;
     const T *x = (const T *)a.logits + row * a.stride;
     // vectors from the row's start rounded down to a vector: the ones that hold some element of the row
     const int skew = VEC > 1 ? (int)(((uintptr_t)x / sizeof(T)) % VEC) : 0;
-    const int base = (int)blockIdx.x * SEL_T * EPT - skew;
-    float xs[EPT];
-    {
-        qmh_vec<T, VEC> v[EPT / VEC];
+    const int64_t first = (int64_t)seg * iters * PIECE - skew;
+    int base = first < a.vocab ? (int)first : a.vocab;
+    qmh_vec<T, VEC> v[EPT / VEC];
+    auto load = [&](int from) {
 #pragma unroll
         for (int k = 0; k < EPT / VEC; k++) {
-            const int i = base + (k * SEL_T + tid) * VEC;
+            const int i = from + (k * 64 + lane) * VEC;
             if (i + VEC > 0 && i < a.vocab) v[k] = *(const qmh_vec<T, VEC> *)(x + i);
         }
+    };
+    load(base);
+    float xs[EPT];
+    float max = -__builtin_inff(), ref = 0.0f; // the segment's maximum; what its exponentials are taken below
+    double sum = 0.0, ref2 = 0.0;
+    float bound = -__builtin_inff(); // logits above it are candidates
+    bool bad = false, none = true;
+    int n = 0; // candidates in the list
+    auto before = [](uint2 u, uint2 v) { return u.x > v.x || (u.x == v.x && u.y < v.y); };
+    auto place = [&](uint64_t all) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0)); };
+    // the list's n_out best, in any order
+    auto cut = [&]() {
+        constexpr int E = SEL_CAP / 64;
+        wave_sync();
+        if (n > 64) { // what the n_out-th largest of the lanes' best leaves
+            uint2 e[E];
+            uint32_t best = 0;
+#pragma unroll
+            for (int j = 0; j < E; j++) {
+                e[j] = lane + 64 * j < n ? list[lane + 64 * j] : make_uint2(0, 0);
+                best = e[j].x > best ? e[j].x : best;
+            }
+            const uint32_t t = wave_nth(best, n_out);
+            wave_sync();
+            n = 0;
+#pragma unroll
+            for (int j = 0; j < E; j++) {
+                const uint64_t all = __ballot(e[j].x >= t && e[j].x);
+                if (e[j].x >= t && e[j].x) list[n + place(all)] = e[j];
+                n += __popcll(all);
+            }
+            wave_sync();
+        }
+        if (n < n_out) return;
+        uint32_t t;
+        if (n <= 64) {
+            const uint2 e = lane < n ? list[lane] : make_uint2(0, 0);
+            t = wave_nth(e.x, n_out);
+            bool keep = e.x >= t; // t is not 0: n entries have keys
+            if (__popcll(__ballot(keep)) > n_out) { // equal values
+                int r = 0;
+                for (int i = 0; i < n; i++) r += before(list[i], e);
+                keep = lane < n && r < n_out;
+            }
+            const uint64_t all = __ballot(keep);
+            wave_sync();
+            if (keep) list[place(all)] = e;
+        } else {
+            uint2 e[E];
+            int r[E] = {};
+#pragma unroll
+            for (int j = 0; j < E; j++) e[j] = list[lane + 64 * j];
+            for (int i = 0; i < n; i++) {
+                const uint2 u = list[i];
+#pragma unroll
+                for (int j = 0; j < E; j++) r[j] += before(u, e[j]);
+            }
+            wave_sync();
+#pragma unroll
+            for (int j = 0; j < E; j++)
+                if (lane + 64 * j < n && r[j] < n_out) list[r[j]] = e[j];
+            wave_sync();
+            t = __builtin_amdgcn_readfirstlane(list[n_out - 1].x);
+        }
+        wave_sync();
+        n = n_out;
+        bound = fmaxf(bound, of_key(t));
+    };
+    for (int it = 0; it < iters && base < a.vocab; it++, base += PIECE) {
 #pragma unroll
         for (int k = 0; k < EPT; k++) xs[k] = qmh_to_f(v[k / VEC].e[k % VEC]);
-    }
-    auto index = [&](int k) { return base + ((k / VEC) * SEL_T + tid) * VEC + k % VEC; };
-    if (base < 0 || base + SEL_T * EPT > a.vocab) // the row's ends
+        if (it + 1 < iters && base + PIECE < a.vocab) load(base + PIECE);
+        auto index = [&](int k) { return base + ((k / VEC) * 64 + lane) * VEC + k % VEC; };
+        if (base < 0 || base + PIECE > a.vocab) // the row's ends
 #pragma unroll
-        for (int k = 0; k < EPT; k++)
-            if ((uint32_t)index(k) >= (uint32_t)a.vocab) xs[k] = -__builtin_inff();
-    if (tid == 0) ncand = 0;
-    float top = xs[0];
+            for (int k = 0; k < EPT; k++)
+                if ((uint32_t)index(k) >= (uint32_t)a.vocab) xs[k] = -__builtin_inff();
+        float top = xs[0];
 #pragma unroll
-    for (int k = 1; k < EPT; k++) top = __builtin_elementwise_maximum(top, xs[k]); // NaN if one is
-    const bool bad = __any(!(top < __builtin_inff()));
-    const float m = qmh_wave_max(top), ref = m > -__builtin_inff() && m < __builtin_inff() ? m : 0.0f;
-    // the bound first: it is short and the sums' latency hides in it
-    uint32_t mine = key_of(top);
-    if (bad) { // NaN hides the lane's maximum
-        mine = 0;
-#pragma unroll
-        for (int k = 0; k < EPT; k++) {
-            const uint32_t q = key_of(xs[k]);
-            mine = q > mine ? q : mine;
+        for (int k = 1; k < EPT; k++) top = __builtin_elementwise_maximum(top, xs[k]); // NaN if one is
+        bad = bad || __any(!(top < __builtin_inff()));
+        if (__any(top > max)) {
+            // a new maximum: the sums stay in range as long as it is within 600 of the reference
+            max = fmaxf(max, qmh_wave_max(top));
+            if (max < __builtin_inff() && (none || max > ref + 600.0f)) {
+                sum *= none ? 0.0 : exp_sum<1>(&ref, max - 700.0f, (double)max * 1.4426950408889634074);
+                ref = max;
+                ref2 = (double)ref * 1.4426950408889634074;
+                none = false;
+            }
         }
-    }
-    const uint32_t bw = wave_nth(mine, n_out);
-    if ((tid & 63) == 0) bounds[w] = bw;
-    const double ref2 = (double)ref * 1.4426950408889634074;
-    const float low = ref - 700.0f;
-    double sum = 0.0, sum2 = 0.0;
 #pragma unroll
-    for (int k = 0; k < EPT; k += 2) {
-        sum += exp_below(xs[k], low, ref2);
-        sum2 += exp_below(xs[k + 1], low, ref2);
-    }
-    sum = qmh_wave_sum_d(sum + sum2);
-    __syncthreads();
-    uint32_t from = bounds[0];
+        for (int k = 0; k < EPT; k += 4) sum += exp_sum<4>(xs + k, ref - 700.0f, ref2);
+        // the largest float below the n_out-th largest of the lanes' maxima, if that is more than the bound
+        auto raise = [&]() {
+            uint32_t mine = 0;
+            if (!bad) {
+                mine = key_of(top);
+            } else { // NaN hides the lane's maximum
 #pragma unroll
-    for (int k = 1; k < 4; k++) from = bounds[k] > from ? bounds[k] : from;
-    // as a float (at least the lowest finite one): -inf and NaN never reach it
-    float at_least = of_key(from ? from : 0x00800000u);
-    int reach = 0;
+                for (int k = 0; k < EPT; k++) {
+                    const uint32_t q = key_of(xs[k]);
+                    mine = q > mine ? q : mine;
+                }
+            }
+            const uint32_t t = wave_nth(mine, n_out);
+            if (t > 1) bound = fmaxf(bound, of_key(t - (t == 0x80000000u ? 2 : 1))); // below 0 is not -0
+        };
+        auto passing = [&]() {
+            int c = 0;
 #pragma unroll
-    for (int k = 0; k < EPT; k++) reach += xs[k] >= at_least;
-    int at = reach ? atomicAdd(&ncand, reach) : 0;
-    __syncthreads();
-    int last = 0x7fffffff; // candidates equal to the bound: only up to this index
-    if (ncand > SEL_CAP) {
-        // the largest bound that n_out keys reach, then the lowest indexes among the keys equal to it
-        from = 0;
-        for (int b = 31; b >= 0; b--) {
-            const uint32_t t = from | 1u << b;
-            int n = 0;
-#pragma unroll
-            for (int k = 0; k < EPT; k++) n += key_of(xs[k]) >= t;
-            if (block_total(n, cnt) >= n_out) from = t;
+            for (int k = 0; k < EPT; k++) c += __popcll(__ballot(xs[k] > bound));
+            return c;
+        };
+        auto append = [&](int k, bool take) {
+            const uint64_t all = __ballot(take);
+            if (all) {
+                if (take) list[n + place(all)] = make_uint2(key_of(xs[k]), (uint32_t)index(k));
+                n += __popcll(all);
+            }
+        };
+        if (it == 0) raise();
+        if (!__any(top > bound) && !bad) continue;
+        bool searched = false;
+        if (n + passing() > SEL_CAP) {
+            cut();
+            raise();
+            searched = n + passing() > SEL_CAP;
         }
-        int above = 0;
+        if (!searched) {
 #pragma unroll
-        for (int k = 0; k < EPT; k++) above += key_of(xs[k]) > from;
-        above = block_total(above, cnt);
-        int lo = -1; // the largest index that leaves fewer than n_out
-        for (int b = 24; b >= 0; b--) {
-            const int t = lo + (1 << b);
-            int n = 0;
+            for (int k = 0; k < EPT; k++) append(k, xs[k] > bound);
+        } else {
+            // the largest key that n_out of the piece's reach, then the lowest indexes among those equal to it
+            uint32_t from = 0;
+            for (int b = 31; b >= 0; b--) {
+                const uint32_t t = from | 1u << b;
+                int c = 0;
 #pragma unroll
-            for (int k = 0; k < EPT; k++) n += key_of(xs[k]) == from && index(k) <= t;
-            if (above + block_total(n, cnt) < n_out) lo = t;
+                for (int k = 0; k < EPT; k++) c += __popcll(__ballot(key_of(xs[k]) >= t));
+                if (c >= n_out) from = t;
+            }
+            const float exact = of_key(from);
+            int last = -1; // the largest index that leaves fewer than n_out, and then the next one
+            for (int b = 24; b >= 0; b--) {
+                const int t = last + (1 << b);
+                int c = 0;
+#pragma unroll
+                for (int k = 0; k < EPT; k++) c += __popcll(__ballot(xs[k] > exact || (xs[k] == exact && index(k) <= t)));
+                if (c < n_out) last = t;
+            }
+            last++;
+#pragma unroll
+            for (int k = 0; k < EPT; k++) append(k, xs[k] > exact || (xs[k] == exact && index(k) <= last));
         }
-        last = lo + 1;
-        at_least = of_key(from);
-        if (tid == 0) ncand = 0;
-        __syncthreads();
-        reach = 0;
-#pragma unroll
-        for (int k = 0; k < EPT; k++) reach += key_of(xs[k]) > from || (key_of(xs[k]) == from && index(k) <= last);
-        at = reach ? atomicAdd(&ncand, reach) : 0;
-        __syncthreads();
+        if (n > SEL_CAP / 2) cut();
     }
-    if (reach)
-#pragma unroll
-        for (int k = 0; k < EPT; k++)
-            if (xs[k] > at_least || (xs[k] == at_least && index(k) <= last)) cand[at++] = make_uint2(key_of(xs[k]), (uint32_t)index(k));
-    __syncthreads();
-    const int n = ncand;
-    rank_all(
-        n, SEL_T, [&](int i, int c) { return cand[i].x > cand[c].x || (cand[i].x == cand[c].x && cand[i].y < cand[c].y); },
-        [&](int c, int r) {
-            if (r < n_out) cands[slot * n_out + r] = cand[c];
-        });
-    if (tid >= n && tid < n_out) cands[slot * n_out + tid] = make_uint2(0, 0);
-    if ((tid & 63) == 0) heads[slot * 4 + w] = scan_head{bad ? __builtin_nan("") : m > -__builtin_inff() ? sum : 0.0, m, 0.0f};
+    cut();
+    if (lane < n_out) cands[slot * n_out + lane] = lane < n ? list[lane] : make_uint2(0, 0);
+    sum = qmh_wave_sum_d(sum);
+    if (lane == 0) heads[slot] = scan_head{bad ? __builtin_nan("") : none ? 0.0 : sum, ref, 0.0f};
 }
 
 // A group's choice from its rows' chunks: each row's log sum (a wave a row), then the n_out best totals as in the scan:
 // a bound from the lanes' best, what reaches it ranked in LDS. Where more than JOIN_CAP reach it, one after another.
-__global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int chunks) {
+__global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int segs) {
     constexpr int NW = JOIN_T / 64;
     __shared__ double lse[64], score[64];
     __shared__ uint64_t ckey[JOIN_CAP], bk[NW];
@@ -223,46 +303,51 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     __shared__ int ncand;
     const int g = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63, K = a.n_beams, n_out = a.n_out;
     if (tid == 0) ncand = 0;
-    for (int b = w; b < K; b += NW) {
+    // few beams: several waves a row, each with the row's log sum for itself
+    const int share = K < NW ? NW / K : 1, per = segs * n_out;
+    for (int b = w / share; b < K; b += NW / share) {
+        if (w / share >= NW / share) break;
         const int row = g * K + b;
         const float sc = a.score[row];
         const bool done = a.done && a.done[row];
         double s = __builtin_nan("");
         if (!done && sc > -__builtin_inff()) {
-            const scan_head *h = heads + (int64_t)row * chunks * 4;
+            const scan_head *h = heads + (int64_t)row * segs;
             float m = -__builtin_inff();
-            for (int c = lane; c < chunks * 4; c += 64) m = fmaxf(m, h[c].max);
+            for (int c = lane; c < segs; c += 64) m = h[c].sum == 0.0 ? m : fmaxf(m, h[c].ref);
             m = qmh_wave_max(m);
             s = 0.0;
             const double ref2 = (double)m * 1.4426950408889634074;
-            for (int c = lane; c < chunks * 4; c += 64) s = __builtin_fma(h[c].sum, exp_below(h[c].max, m - 700.0f, ref2), s);
-            s = (double)m + log(qmh_wave_sum_d(s)); // a row without a logit: NaN or -inf, and no continuation
+            for (int c = lane; c < segs; c += 64) s = __builtin_fma(h[c].sum, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
+            s = (double)m + log(qmh_wave_sum_d(s)); // a row without a logit: NaN, and no continuation
         }
-        if (lane == 0) {
-            lse[b] = s;
-            score[b] = done ? -(double)sc : (double)sc;
-            if (done) lse[b] = __builtin_inf(); // marks a finished row
+        if (lane == 0 && w % share == 0) {
+            lse[b] = done ? __builtin_inf() : s; // marks a finished row
+            score[b] = (double)sc;
         }
     }
     __syncthreads();
-    // a wave's own rows: lane's j-th candidate of row b as an ordered key (0: none), its place beam * vocab + token
-    const int per = chunks * n_out;
-    auto key_at = [&](int b, int j, uint32_t &place) -> uint64_t {
-        const double L = lse[b];
-        if (L == __builtin_inf()) { // finished: one continuation
-            place = (uint32_t)(b * a.vocab + a.eos);
-            return j == 0 ? key_of_d(-score[b]) : 0ull;
-        }
-        const uint2 v = cands[(int64_t)(g * K + b) * per + j];
-        place = (uint32_t)(b * a.vocab) + v.y;
-        return v.x && L == L ? key_of_d(score[b] + ((double)of_key(v.x) - L)) : 0ull;
-    };
+    // body(ordered key of the total, place = beam * vocab + token) for each candidate of the wave's rows
     auto each = [&](auto body) {
-        uint32_t place = 0;
-        for (int b = w; b < K; b += NW) {
-            for (int j = lane; j < per; j += 64) {
-                const uint64_t q = key_at(b, j, place);
-                if (q) body(q, place);
+        if (w / share >= NW / share) return;
+        for (int b = w / share; b < K; b += NW / share) {
+            const double L = lse[b], sc = score[b];
+            if (L == __builtin_inf()) { // finished: one continuation
+                const uint64_t q = key_of_d(sc);
+                if (lane == 0 && w % share == 0 && q) body(q, (uint32_t)(b * a.vocab + a.eos));
+                continue;
+            }
+            if (L != L) continue;
+            const uint2 *c = cands + (int64_t)(g * K + b) * per;
+            for (int j0 = (w % share) * 64 + lane; j0 < per; j0 += 256 * share) {
+                uint2 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = j0 + 64 * share * k < per ? c[j0 + 64 * share * k] : make_uint2(0, 0);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint64_t q = v[k].x ? key_of_d(sc + ((double)of_key(v[k].x) - L)) : 0ull;
+                    if (q) body(q, (uint32_t)(b * a.vocab) + v[k].y);
+                }
             }
         }
     };
@@ -341,9 +426,28 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     if (tid < n_out) write(tid, ckey[tid], cplace[tid]);
 }
 
-int scan_chunks(const qmh_beam_args *a, int ept) { return (a->vocab + 15 + SEL_T * ept - 1) / (SEL_T * ept); }
-// elements a thread holds: 8 spreads few rows over more workgroups, 32 leaves fewer candidates to the join
-int scan_ept(const qmh_beam_args *a) { return (int64_t)a->n_groups * a->n_beams * scan_chunks(a, 8) <= 1024 ? 8 : 32; }
+#ifndef SC_WAVES
+#define SC_WAVES 3072
+#endif
+#ifndef SC_EPT
+#define SC_EPT 16
+#endif
+// How a row is cut: into segments of whole pieces, one a wave, as many as give the chip about SC_WAVES waves.
+struct scan_plan {
+    int ept, iters, segs; // segs: of a row, a multiple of a workgroup's waves
+};
+scan_plan plan_scan(const qmh_beam_args *a) {
+    constexpr int W = SEL_T / 64;
+    const int64_t rows = (int64_t)a->n_groups * a->n_beams, len = (int64_t)a->vocab + 15; // 15: a row that starts inside a vector
+    scan_plan p;
+    p.ept = rows * len <= (int64_t)SC_WAVES * 64 * 8 ? 8 : SC_EPT;
+    const int64_t piece = 64 * p.ept, pieces = (len + piece - 1) / piece;
+    int64_t segs = SC_WAVES / rows / W * W;
+    segs = segs < W ? W : segs;
+    p.iters = (int)((pieces + segs - 1) / segs);
+    p.segs = (int)((pieces + (int64_t)p.iters * W - 1) / ((int64_t)p.iters * W)) * W;
+    return p;
+}
 
 // --------------------------------------------------------------------------- reorder
 
@@ -436,26 +540,27 @@ __global__ __launch_bounds__(256, BM > 16 ? 2 : 4) void k_beam_reorder(const qmh
 } // namespace
 
 extern "C" size_t qmh_beam_ws_bytes(const qmh_beam_args *a) {
-    const size_t slots = (size_t)a->n_groups * a->n_beams * scan_chunks(a, scan_ept(a));
-    return slots * (4 * sizeof(scan_head) + a->n_out * sizeof(uint2));
+    const size_t lists = (size_t)a->n_groups * a->n_beams * plan_scan(a).segs;
+    return lists * (sizeof(scan_head) + a->n_out * sizeof(uint2));
 }
 
 extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *stream) {
     hipStream_t st = (hipStream_t)stream;
-    const int rows = a->n_groups * a->n_beams, ept = scan_ept(a), chunks = scan_chunks(a, ept);
+    const scan_plan p = plan_scan(a);
+    const int rows = a->n_groups * a->n_beams;
     scan_head *heads = (scan_head *)ws;
-    uint2 *cands = (uint2 *)(heads + (size_t)rows * chunks * 4);
+    uint2 *cands = (uint2 *)(heads + (size_t)rows * p.segs);
     qmh_for_type(a->dtype, [&](auto z) {
         using T = decltype(z);
         constexpr int VEC = 16 / sizeof(T);
         // rows over y in passes of at most 65535
         for (int r0 = 0; r0 < rows; r0 += 65535) {
-            const dim3 g(chunks, rows - r0 < 65535 ? rows - r0 : 65535), t(SEL_T);
-            if (ept == 8) hipLaunchKernelGGL((k_beam_scan<T, 8, VEC>), g, t, 0, st, *a, heads, cands, r0);
-            else hipLaunchKernelGGL((k_beam_scan<T, 32, VEC>), g, t, 0, st, *a, heads, cands, r0);
+            const dim3 g(p.segs / (SEL_T / 64), rows - r0 < 65535 ? rows - r0 : 65535);
+            if (p.ept == 8) hipLaunchKernelGGL((k_beam_scan<T, 8, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
+            else hipLaunchKernelGGL((k_beam_scan<T, SC_EPT, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
         }
     });
-    hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, chunks);
+    hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);
     return (int)hipGetLastError();
 }
 
