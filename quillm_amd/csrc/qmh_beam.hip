@@ -17,14 +17,13 @@ constexpr int JOIN_T = 512;   // threads of the join
 constexpr int JOIN_CAP = 1024;
 
 // The sum of e^(x - ref) over N floats, in 64 bits, x at most 600 above ref (finite): x log2 e - ref log2 e = k + f,
-// |f| <= 1/2, and 2^k times the Taylor polynomial of 2^f to degree 10, whose remainder is below
-// (ln 2 / 2)^11 / 11! = 2.2e-13 of the value: far inside the distance of scores that decide a choice. Adding 1.5 2^52
+// |f| <= 1/2, and 2^k times a polynomial of degree 8 that meets 2^f at the nine Chebyshev points, at most 1.1e-12 of the
+// value from it: far inside the distance of scores that decide a choice. Adding 1.5 2^52
 // rounds to k and leaves it in the low word. Values below low = ref - 700 count as that. The N chains run side by side.
 template <int N>
 __device__ __forceinline__ double exp_sum(const float *x, float low, double ref2) {
-    constexpr double c[10] = {1.0178086009239699728e-7, 1.3215486790144309488e-6, 1.5252733804059840280e-5, 1.5403530393381609954e-4,
-                              1.3333558146428443423e-3, 9.6181291076284771619e-3, 5.5504108664821579953e-2, 2.4022650695910071233e-1,
-                              6.9314718055994530942e-1, 1.0};
+    constexpr double c[8] = {1.531007940249083e-05, 0.00015403455852408237, 0.0013333450567999663, 0.009618129159402626,
+                             0.05550410941205934, 0.2402265069581299, 0.6931471805459335, 1.0};
     double t[N], s[N], p[N];
 #pragma unroll
     for (int j = 0; j < N; j++) t[j] = __builtin_fma((double)fmaxf(x[j], low), 1.4426950408889634074, -ref2);
@@ -33,9 +32,9 @@ __device__ __forceinline__ double exp_sum(const float *x, float low, double ref2
 #pragma unroll
     for (int j = 0; j < N; j++) t[j] = t[j] - (s[j] - 0x1.8p52);
 #pragma unroll
-    for (int j = 0; j < N; j++) p[j] = 7.0549116208011233299e-9;
+    for (int j = 0; j < N; j++) p[j] = 1.3255224888009091e-06;
 #pragma unroll
-    for (int k = 0; k < 10; k++)
+    for (int k = 0; k < 8; k++)
 #pragma unroll
         for (int j = 0; j < N; j++) p[j] = __builtin_fma(p[j], t[j], c[k]);
 #pragma unroll
@@ -68,13 +67,16 @@ struct scan_head { // a wave's part of a segment of a row: the sum of exp(x - re
     float ref, pad;
 };
 
-// The largest t that at least n <= 64 of a wave's values reach, 0 if there is none above: bit by bit, by ballots.
+// The largest t that at least n <= 64 of a wave's values reach, 0 if there is none above; with LOW, the largest whose LOW
+// lowest bits are 0 (a bound for less). Two bits a round, by ballots.
+template <int LOW = 0>
 __device__ __forceinline__ uint32_t wave_nth(uint32_t v, int n) {
     uint32_t t = 0;
 #pragma unroll
-    for (int b = 31; b >= 0; b--) {
-        const uint32_t u = t | 1u << b;
-        t = __popcll(__ballot(v >= u)) >= n ? u : t;
+    for (int b = 30; b >= LOW; b -= 2) {
+        const uint32_t u1 = t | 1u << b, u2 = t | 2u << b, u3 = t | 3u << b;
+        const int c1 = __popcll(__ballot(v >= u1)), c2 = __popcll(__ballot(v >= u2)), c3 = __popcll(__ballot(v >= u3));
+        t = c3 >= n ? u3 : c2 >= n ? u2 : c1 >= n ? u1 : t;
     }
     return t;
 }
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
                 e[j] = lane + 64 * j < n ? list[lane + 64 * j] : make_uint2(0, 0);
                 best = e[j].x > best ? e[j].x : best;
             }
-            const uint32_t t = wave_nth(best, n_out);
+            const uint32_t t = wave_nth<12>(best, n_out);
             wave_sync();
             n = 0;
 #pragma unroll
@@ -235,7 +237,7 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
                     mine = q > mine ? q : mine;
                 }
             }
-            const uint32_t t = wave_nth(mine, n_out);
+            const uint32_t t = wave_nth<12>(mine, n_out);
             if (t > 1) bound = fmaxf(bound, of_key(t - (t == 0x80000000u ? 2 : 1))); // below 0 is not -0
         };
         auto passing = [&]() {
@@ -253,13 +255,13 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
         };
         if (it == 0) raise();
         if (!__any(top > bound) && !bad) continue;
-        bool searched = false;
-        if (n + passing() > SEL_CAP) {
+        bool full = n + passing() > SEL_CAP;
+        if (full) {
             cut();
             raise();
-            searched = n + passing() > SEL_CAP;
+            full = n + passing() > SEL_CAP;
         }
-        if (!searched) {
+        if (!full) {
 #pragma unroll
             for (int k = 0; k < EPT; k++) append(k, xs[k] > bound);
         } else {
@@ -305,20 +307,31 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     if (tid == 0) ncand = 0;
     // few beams: several waves a row, each with the row's log sum for itself
     const int share = K < NW ? NW / K : 1, per = segs * n_out;
-    for (int b = w / share; b < K; b += NW / share) {
-        if (w / share >= NW / share) break;
+    const int b0 = w / share < NW / share ? w / share : K, j0 = (w % share) * 64 + lane;
+    // the first row's first heads and candidates are asked for at once with its score (of a dead row they are not used)
+    scan_head h0 = {0.0, 0.0f, 0.0f};
+    uint2 v0[4];
+    if (b0 < K) {
+        const int64_t at = (int64_t)(g * K + b0) * segs;
+        if (lane < segs) h0 = heads[at + lane];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v0[k] = j0 + 64 * share * k < per ? cands[at * n_out + j0 + 64 * share * k] : make_uint2(0, 0);
+    }
+    for (int b = b0; b < K; b += NW / share) {
         const int row = g * K + b;
         const float sc = a.score[row];
         const bool done = a.done && a.done[row];
         double s = __builtin_nan("");
         if (!done && sc > -__builtin_inff()) {
             const scan_head *h = heads + (int64_t)row * segs;
-            float m = -__builtin_inff();
-            for (int c = lane; c < segs; c += 64) m = h[c].sum == 0.0 ? m : fmaxf(m, h[c].ref);
+            const scan_head one = b == b0 || lane >= segs ? h0 : h[lane];
+            float m = one.sum == 0.0 ? -__builtin_inff() : one.ref;
+            for (int c = lane + 64; c < segs; c += 64) m = h[c].sum == 0.0 ? m : fmaxf(m, h[c].ref);
             m = qmh_wave_max(m);
-            s = 0.0;
             const double ref2 = (double)m * 1.4426950408889634074;
-            for (int c = lane; c < segs; c += 64) s = __builtin_fma(h[c].sum, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
+            const float r0 = one.ref;
+            s = one.sum == 0.0 || lane >= segs ? 0.0 : one.sum * exp_sum<1>(&r0, m - 700.0f, ref2);
+            for (int c = lane + 64; c < segs; c += 64) s = __builtin_fma(h[c].sum, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
             s = (double)m + log(qmh_wave_sum_d(s)); // a row without a logit: NaN, and no continuation
         }
         if (lane == 0 && w % share == 0) {
@@ -329,8 +342,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     __syncthreads();
     // body(ordered key of the total, place = beam * vocab + token) for each candidate of the wave's rows
     auto each = [&](auto body) {
-        if (w / share >= NW / share) return;
-        for (int b = w / share; b < K; b += NW / share) {
+        for (int b = b0; b < K; b += NW / share) {
             const double L = lse[b], sc = score[b];
             if (L == __builtin_inf()) { // finished: one continuation
                 const uint64_t q = key_of_d(sc);
@@ -339,10 +351,13 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
             }
             if (L != L) continue;
             const uint2 *c = cands + (int64_t)(g * K + b) * per;
-            for (int j0 = (w % share) * 64 + lane; j0 < per; j0 += 256 * share) {
+            for (int i = 0; i < per; i += 256 * share) {
                 uint2 v[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = j0 + 64 * share * k < per ? c[j0 + 64 * share * k] : make_uint2(0, 0);
+                for (int k = 0; k < 4; k++) {
+                    const int j = i + j0 + 64 * share * k;
+                    v[k] = b == b0 && i == 0 ? v0[k] : j < per ? c[j] : make_uint2(0, 0);
+                }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint64_t q = v[k].x ? key_of_d(sc + ((double)of_key(v[k].x) - L)) : 0ull;
@@ -353,7 +368,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     };
     uint32_t mine = 0;
     each([&](uint64_t q, uint32_t) { mine = (uint32_t)(q >> 32) > mine ? (uint32_t)(q >> 32) : mine; });
-    const uint32_t bw = wave_nth(mine, n_out);
+    const uint32_t bw = wave_nth<12>(mine, n_out);
     if (lane == 0) bounds[w] = bw;
     __syncthreads();
     uint32_t from = 1;
