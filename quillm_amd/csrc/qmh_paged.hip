@@ -22,13 +22,14 @@ struct append_args {
     int lanes;           // lanes per head, a power of two
 };
 
-// One wave takes one token's heads, 64 / lanes of them at a time. A lane holds a unit of a head: two vectors of VW
-// elements, whose elements pair up in the rotated part (HALVES: VW elements of each half; PAIRS: 2 VW elements in
-// a row) and follow one another behind it. So both layouts turn in registers, a head's sum of squares is one
-// reduction over its lanes, and the sines and cosines of a lane's pairs are made once for all heads of the token:
-// position 1024 h + l is turned by the angle sum of two table rows, in 64 bits. IT: units of a lane (2 only for
-// one-element vectors of heads past 128).
-template <typename T, int VW, int IT>
+// One wave takes one token's heads (or a share of them), 64 / lanes of them at a time, the next ones' loads under way.
+// A lane holds a unit of a head: two vectors of VW elements, whose elements pair up in the rotated part (halves: VW elements
+// of each half; PAIRS: 2 VW elements in a row) and follow one another behind it. So both layouts turn in
+// registers and a head's sum of squares is one reduction over its lanes. The sines and cosines are made once for all
+// heads of the token, a pair a lane, and handed round: position 1024 h + l is turned by the angle sum of two
+// table rows, in 64 bits, rounded to 32 at the end. IT: units of a lane (2 only for one-element vectors of heads past 128).
+// Bound by the rows' bytes: 4001 tokens of (32 + 2 x 32) x 128 f16 take 41 us (197 MB, 4.75 TB/s; a large copy reaches 5.1).
+template <typename T, int VW, int IT, bool PAIRS>
 __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
     const qmh_append_args &a = s.a;
     const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
@@ -49,49 +50,69 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
         row0 = (int64_t)page * KV * ps + sl % ps;
     }
     const int l = lane & (s.lanes - 1), per = 64 / s.lanes, units = hd / (2 * VW);
+    // the token's sines and cosines, pair p (and p + 64) by lane p; each lane then takes those of its unit
+    float cp[2] = {1.0f, 1.0f}, wp[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int pr = lane + 64 * k;
+        if (pr < half) {
+            const double2 hi = ((const double2 *)s.r.hi)[(int64_t)(pos / QMH_ROTARY_LO) * half + pr];
+            const double2 lo = ((const double2 *)s.r.lo)[(int64_t)(pos % QMH_ROTARY_LO) * half + pr];
+            cp[k] = (float)__builtin_fma(hi.x, lo.x, -(hi.y * lo.y));
+            wp[k] = (float)__builtin_fma(hi.y, lo.x, hi.x * lo.y);
+        }
+    }
     int at0[IT], at1[IT];
     float c[IT][VW], w[IT][VW];
 #pragma unroll
     for (int k = 0; k < IT; k++) {
         const int u = l + k * s.lanes;
         const bool turn = u * VW < half;
-        at0[k] = !turn ? rot + 2 * (u * VW - half) : s.r.layout == QMH_ROTARY_HALVES ? u * VW : 2 * u * VW;
-        at1[k] = turn && s.r.layout == QMH_ROTARY_HALVES ? at0[k] + half : at0[k] + VW;
+        at0[k] = !turn ? rot + 2 * (u * VW - half) : PAIRS ? 2 * u * VW : u * VW;
+        at1[k] = turn && !PAIRS ? at0[k] + half : at0[k] + VW;
 #pragma unroll
         for (int i = 0; i < VW; i++) {
-            c[k][i] = 1.0f;
-            w[k][i] = 0.0f;
-            if (turn) {
-                const int pr = u * VW + i;
-                const double2 hi = ((const double2 *)s.r.hi)[(int64_t)(pos / QMH_ROTARY_LO) * half + pr];
-                const double2 lo = ((const double2 *)s.r.lo)[(int64_t)(pos % QMH_ROTARY_LO) * half + pr];
-                c[k][i] = (float)__builtin_fma(hi.x, lo.x, -(hi.y * lo.y));
-                w[k][i] = (float)__builtin_fma(hi.y, lo.x, hi.x * lo.y);
+            const int pr = u * VW + i;
+            c[k][i] = __shfl(cp[0], pr & 63);
+            w[k][i] = __shfl(wp[0], pr & 63);
+            if (half > 64) {
+                const float c1 = __shfl(cp[1], pr & 63), w1 = __shfl(wp[1], pr & 63);
+                c[k][i] = pr < 64 ? c[k][i] : c1;
+                w[k][i] = pr < 64 ? w[k][i] : w1;
             }
+            c[k][i] = turn ? c[k][i] : 1.0f;
+            w[k][i] = turn ? w[k][i] : 0.0f;
         }
     }
-    const bool pairs = s.r.layout == QMH_ROTARY_PAIRS;
-    for (int h0 = part * per; h0 < NH; h0 += s.split * per) {
-        const int h = h0 + lane / s.lanes;
-        if (h >= NH) continue;
-        const int kind = h < H ? 0 : h < H + KV ? 1 : 2;
-        const int g = kind == 0 ? h : kind == 1 ? h - H : h - H - KV;
-        const T *src;
-        T *dst;
-        if (kind == 0) {
-            src = (const T *)a.q + t * a.q_stride + g * hd;
-            dst = (T *)a.q_out + t * a.q_out_stride + g * hd;
-        } else {
-            src = kind == 1 ? (const T *)a.k + t * a.k_stride + g * hd : (const T *)a.v + t * a.v_stride + g * hd;
-            dst = (kind == 1 ? (T *)s.p.k : (T *)s.p.v) + (row0 + (int64_t)g * ps) * hd;
-        }
-        qmh_vec<T, VW> v0[IT], v1[IT];
+    // a head's row by its number: queries, keys, values
+    auto source = [&](int h) {
+        if (h < H) return (const T *)a.q + t * a.q_stride + h * hd;
+        return h < H + KV ? (const T *)a.k + t * a.k_stride + (h - H) * hd : (const T *)a.v + t * a.v_stride + (h - H - KV) * hd;
+    };
+    qmh_vec<T, VW> v0[IT], v1[IT], n0[IT], n1[IT]; // this head's unit and the next one's, on its way
+    auto fetch = [&](int h) {
+        if (h >= NH) return;
+        const T *src = source(h);
 #pragma unroll
         for (int k = 0; k < IT; k++)
             if (l + k * s.lanes < units) {
-                v0[k] = *(const qmh_vec<T, VW> *)(src + at0[k]);
-                v1[k] = *(const qmh_vec<T, VW> *)(src + at1[k]);
+                n0[k] = *(const qmh_vec<T, VW> *)(src + at0[k]);
+                n1[k] = *(const qmh_vec<T, VW> *)(src + at1[k]);
             }
+    };
+    const int step = s.split * per;
+    for (int h = part * per + lane / s.lanes, first = 1; h - lane / s.lanes < NH; h += step, first = 0) {
+        if (first) fetch(h);
+#pragma unroll
+        for (int k = 0; k < IT; k++) {
+            v0[k] = n0[k];
+            v1[k] = n1[k];
+        }
+        fetch(h + step);
+        if (h >= NH) continue;
+        const int kind = h < H ? 0 : h < H + KV ? 1 : 2;
+        const int g = kind == 0 ? h : kind == 1 ? h - H : h - H - KV;
+        T *dst = kind == 0 ? (T *)a.q_out + t * a.q_out_stride + g * hd : (kind == 1 ? (T *)s.p.k : (T *)s.p.v) + (row0 + (int64_t)g * ps) * hd;
         const float *gain = kind == 0 ? a.q_gain : kind == 1 ? a.k_gain : nullptr;
         float inv = 1.0f;
         if (a.q_gain || a.k_gain) { // every lane takes part in the exchange
@@ -113,22 +134,18 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
                 if (kind != 2) { // values go as they are
 #pragma unroll
                     for (int i = 0; i < VW; i++) {
-                        // the i-th pair of the unit: element i of both vectors, or two neighbours
-                        T *px = &v0[k].e[i], *py = &v1[k].e[i];
-                        int ex = at0[k] + i, ey = at1[k] + i;
-                        if (pairs && VW > 1) {
-                            px = 2 * i < VW ? &v0[k].e[(2 * i) % VW] : &v1[k].e[(2 * i) % VW];
-                            py = 2 * i < VW ? &v0[k].e[(2 * i + 1) % VW] : &v1[k].e[(2 * i + 1) % VW];
-                            ex = at0[k] + 2 * i;
-                            ey = ex + 1;
-                        }
-                        float x = qmh_to_f(*px), y = qmh_to_f(*py);
+                        // the i-th pair of the unit: two neighbours, or element i of both vectors
+                        constexpr bool NB = PAIRS && VW > 1;
+                        qmh_vec<T, VW> &vx = NB && 2 * i >= VW ? v1[k] : v0[k], &vy = NB && 2 * i < VW ? v0[k] : v1[k];
+                        const int ix = NB ? (2 * i) % VW : i, iy = NB ? (2 * i + 1) % VW : i;
+                        const int ex = NB ? at0[k] + 2 * i : at0[k] + i, ey = NB ? at0[k] + 2 * i + 1 : at1[k] + i;
+                        float x = qmh_to_f(vx.e[ix]), y = qmh_to_f(vy.e[iy]);
                         if (gain) {
                             x = x * inv * gain[ex];
                             y = y * inv * gain[ey];
                         }
-                        *px = (T)__builtin_fmaf(x, c[k][i], -(y * w[k][i]));
-                        *py = (T)__builtin_fmaf(x, w[k][i], y * c[k][i]);
+                        vx.e[ix] = (T)__builtin_fmaf(x, c[k][i], -(y * w[k][i]));
+                        vy.e[iy] = (T)__builtin_fmaf(x, w[k][i], y * c[k][i]);
                     }
                 }
                 *(qmh_vec<T, VW> *)(dst + at0[k]) = v0[k];
@@ -789,19 +806,26 @@ extern "C" int qmh_launch_paged_append(const qmh_append_args *a, const qmh_rotar
     s.lanes = 1;
     while (s.lanes < units && s.lanes < 64) s.lanes <<= 1;
     const int passes = (nh * s.lanes + 63) / 64;
-    // few tokens: their heads over several waves, as many as there are passes; many: one wave each
+    // a token's heads over several waves, down to one pass each, while that still adds waves to the chip (8 on each of
+    // its 1024 SIMDs, three rounds of them): 4001 tokens of 96 x 128 f16 take 44, 43, 42 and 41 us in 4001, 8002, 16004 and
+    // 24006 waves
     s.split = 1;
-    while (s.split < passes && (int64_t)s.split * a->n_tokens < 4096) s.split++;
+    while (s.split < passes && (int64_t)s.split * a->n_tokens < 24576) s.split++;
     const int64_t blocks = ((int64_t)a->n_tokens * s.split + 3) / 4;
     qmh_for_type(s.p.dtype, [&](auto z) {
         using T = decltype(z);
         const dim3 g((uint32_t)blocks), t(256);
         hipStream_t st = (hipStream_t)stream;
-        if (units > 64) hipLaunchKernelGGL((k_paged_append<T, 1, 2>), g, t, 0, st, s);
-        else if (vw == 1) hipLaunchKernelGGL((k_paged_append<T, 1, 1>), g, t, 0, st, s);
-        else if (vw == 2) hipLaunchKernelGGL((k_paged_append<T, 2, 1>), g, t, 0, st, s);
-        else if (vw == 4) hipLaunchKernelGGL((k_paged_append<T, 4, 1>), g, t, 0, st, s);
-        else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((k_paged_append<T, 8, 1>), g, t, 0, st, s);
+        auto go = [&](auto layout) {
+            constexpr bool P = decltype(layout)::value;
+            if (units > 64) hipLaunchKernelGGL((k_paged_append<T, 1, 2, P>), g, t, 0, st, s);
+            else if (vw == 1) hipLaunchKernelGGL((k_paged_append<T, 1, 1, P>), g, t, 0, st, s);
+            else if (vw == 2) hipLaunchKernelGGL((k_paged_append<T, 2, 1, P>), g, t, 0, st, s);
+            else if (vw == 4) hipLaunchKernelGGL((k_paged_append<T, 4, 1, P>), g, t, 0, st, s);
+            else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((k_paged_append<T, 8, 1, P>), g, t, 0, st, s);
+        };
+        if (s.r.layout == QMH_ROTARY_PAIRS) go(std::true_type{});
+        else go(std::false_type{});
     });
     return (int)hipGetLastError();
 }
