@@ -312,6 +312,21 @@ int qmh_batch_forward(qmh_batch *b, const int32_t *tokens, const int32_t *pos, f
 int qmh_batch_greedy(qmh_batch *b, const int32_t *tokens, const int32_t *pos, int32_t n_steps, int32_t *out,
                      double *ms);
 
+/* Beam search state: sequence j of each group of n_beams (which divides n_seq) takes the first n_pos positions
+ * of the KV cache of sequence parent[j] of its group (host array [n_seq]; outside [0, n_beams): its own), in
+ * place, all layers. Synchronous. 0 or -1. */
+int qmh_batch_reorder(qmh_batch *b, const int32_t *parent, int32_t n_beams, int32_t n_pos);
+/* Beam search on the device: the batch's sequences are groups of n_beams (at most 64; it divides n_seq). Every
+ * sequence of group g holds the same prompt (positions below pos[g]); the search starts with tokens[g] at pos[g] and
+ * makes n_steps steps, each the forward of every sequence (logits bitwise those of qmh_batch_forward), then the
+ * n_beams best continuations of the group (qmh_beam_select: sums of log probabilities in 64 bits, each step's rounded to
+ * float), their caches reordered. A hypothesis that took eos (-1: none) is finished: it keeps its score and repeats
+ * eos. out[i * n_steps + k]: token k of hypothesis i, best first within a group (-1 throughout where the vocabulary
+ * leaves fewer than n_beams); scores[i] its sum (-inf there). The caches end as the hypotheses' own, at pos[g] + n_steps.
+ * ms (optional): device time of the steps. No host round trip between steps. 0 or -1. */
+int qmh_batch_beam(qmh_batch *b, int32_t n_beams, const int32_t *tokens, const int32_t *pos, int32_t n_steps, int32_t eos,
+                   int32_t *out, float *scores, double *ms);
+
 /* ------------------------------------------------------------------ sampler */
 
 /* qm_sampler (src/sampler.h:8-16): temperature / top-k / top-p sampling with an xorshift64*

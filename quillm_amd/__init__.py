@@ -156,6 +156,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "qmh_batch_free": (None, [vp]),
         "qmh_batch_forward": (ctypes.c_int, [vp, vp, vp, vp]),
         "qmh_batch_greedy": (ctypes.c_int, [vp, vp, vp, i32, vp, ctypes.POINTER(ctypes.c_double)]),
+        "qmh_batch_reorder": (ctypes.c_int, [vp, vp, i32, i32]),
+        "qmh_batch_beam": (ctypes.c_int, [vp, i32, vp, vp, i32, i32, vp, vp, ctypes.POINTER(ctypes.c_double)]),
         "qmh_sampler_create": (vp, [i32, f32, ctypes.c_int, f32, ctypes.c_uint64]),
         "qmh_sampler_free": (None, [vp]),
         "qmh_sample": (ctypes.c_int, [vp, vp, vp, vp]),
@@ -417,6 +419,25 @@ class Batch:
         _check(load_library().qmh_batch_greedy(self._h, t.ctypes.data, p.ctypes.data, int(n_steps), out.ctypes.data,
                                                 ctypes.byref(ms)), "batch_greedy")
         return out[:n_steps], ms.value
+
+    def reorder(self, parent, n_beams: int, n_pos: int):
+        """Sequence j of each group of n_beams takes the cache of sequence parent[j] of its group (qmh_batch_reorder)."""
+        p = np.ascontiguousarray(parent, np.int32)
+        assert p.size == self.n
+        _check(load_library().qmh_batch_reorder(self._h, p.ctypes.data, int(n_beams), int(n_pos)), "batch_reorder")
+
+    def beam(self, tokens, pos, n_beams: int, n_steps: int, eos: int = -1):
+        """(ids [n_seq, n_steps], scores [n_seq], device ms) of a beam search on the device (qmh_batch_beam): the batch's
+        sequences are groups of n_beams, group g starts with tokens[g] at pos[g]."""
+        t = np.ascontiguousarray(tokens, np.int32)
+        p = np.ascontiguousarray(pos, np.int32)
+        assert n_beams > 0 and t.size * n_beams == self.n and p.size == t.size
+        out = np.full((self.n, max(n_steps, 1)), -1, np.int32)
+        scores = np.zeros(self.n, np.float32)
+        ms = ctypes.c_double()
+        _check(load_library().qmh_batch_beam(self._h, int(n_beams), t.ctypes.data, p.ctypes.data, int(n_steps), int(eos), out.ctypes.data,
+                                              scores.ctypes.data, ctypes.byref(ms)), "batch_beam")
+        return out[:, :n_steps], scores, ms.value
 
     def close(self):
         if getattr(self, "_h", None):

@@ -552,6 +552,26 @@ __global__ __launch_bounds__(256, BM > 16 ? 2 : 4) void k_beam_reorder(const qmh
     }
 }
 
+// The step's choice becomes the sequences' next tokens and positions: thread j of group blockIdx.x. A place that no
+// continuation took (token -1) goes on with token 0; its score of -inf keeps it out of later choices.
+__global__ __launch_bounds__(64) void k_beam_advance(const int32_t *parent, const int32_t *token, int eos, int K, int32_t *done, int32_t *tok,
+                                                     int32_t *pos, int32_t *hist, int hist_stride, int step) {
+    const int j = threadIdx.x, i = blockIdx.x * K + j;
+    int d = 0, t = -1;
+    if (j < K) {
+        const int p = parent[i];
+        t = token[i];
+        d = p >= 0 && p < K && (done[blockIdx.x * K + p] || t == eos);
+    }
+    __syncthreads(); // every parent's flag has been read
+    if (j < K) {
+        done[i] = d;
+        tok[i] = t < 0 ? 0 : t;
+        pos[i]++;
+        hist[(int64_t)i * hist_stride + step] = t;
+    }
+}
+
 } // namespace
 
 extern "C" size_t qmh_beam_ws_bytes(const qmh_beam_args *a) {
@@ -605,4 +625,11 @@ extern "C" int qmh_launch_beam_reorder(const qmh_beam_state *s, void *dst, const
     if (all % 16 == 0 && n_beams <= 16) return reorder_as<v4u>(s, dst, src, parent, n_groups, n_beams, st);
     if (all % 4 == 0) return reorder_as<uint32_t>(s, dst, src, parent, n_groups, n_beams, st);
     return reorder_as<uint8_t>(s, dst, src, parent, n_groups, n_beams, st);
+}
+
+extern "C" int qmh_launch_beam_advance(const int32_t *parent, const int32_t *token, int eos, int n_groups, int n_beams, int32_t *done,
+                                       int32_t *tok, int32_t *pos, int32_t *hist, int hist_stride, int step, void *stream) {
+    hipLaunchKernelGGL(k_beam_advance, dim3(n_groups), dim3(64), 0, (hipStream_t)stream, parent, token, eos, n_beams, done, tok, pos, hist,
+                       hist_stride, step);
+    return (int)hipGetLastError();
 }

@@ -248,6 +248,9 @@ size_t qmh_beam_ws_bytes(const qmh_beam_args *a);
 int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *stream);
 int qmh_launch_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const int32_t *parent, int n_groups,
                             int n_beams, void *stream);
+/* one step's choice into the next tokens, positions and finished flags of a batch; hist[i][step] gets the token */
+int qmh_launch_beam_advance(const int32_t *parent, const int32_t *token, int eos, int n_groups, int n_beams, int32_t *done,
+                            int32_t *tok, int32_t *pos, int32_t *hist, int hist_stride, int step, void *stream);
 int qmh_launch_paged_reorder(const qmh_pages *p, const int32_t *table, int table_stride, const int32_t *len, int max_len,
                              const int32_t *parent, int n_groups, int n_beams, void *stream);
 

@@ -1582,11 +1582,16 @@ struct qmh_batch {
     int32_t *d_tok, *d_pos, *d_record;
     int32_t *h_io; /* pinned [2n]: tokens, positions */
     int record_cap;
+    /* beam search: scores, finished flags and the last choice [n] each, and the selection's workspace */
+    float *d_score;
+    int32_t *d_done, *d_parent, *d_choice;
+    void *d_beam_ws;
+    size_t beam_ws;
 };
 
 void qmh_batch_free(qmh_batch *b) {
     if (!b) return;
-    void *bufs[] = {b->d_kt, b->d_v, b->d_tok, b->d_pos, b->d_record};
+    void *bufs[] = {b->d_kt, b->d_v, b->d_tok, b->d_pos, b->d_record, b->d_score, b->d_done, b->d_parent, b->d_choice, b->d_beam_ws};
     for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++)
         if (bufs[i]) hipFree(bufs[i]);
     if (b->h_io) hipHostFree(b->h_io);
@@ -1622,6 +1627,14 @@ qmh_batch *qmh_batch_create(qmh_model *m, int32_t n_seq) {
     if (e == hipSuccess) e = hipMalloc((void **)&b->d_pos, sizeof(int32_t) * (size_t)n_seq);
     if (e == hipSuccess) e = hipMalloc((void **)&b->d_record, sizeof(int32_t) * (size_t)n_seq * c->max_seq);
     if (e == hipSuccess) e = hipHostMalloc((void **)&b->h_io, sizeof(int32_t) * 2 * (size_t)n_seq, hipHostMallocDefault);
+    /* the selection's workspace goes by the rows and the places of a group: rows of one beam each need as much */
+    const qmh_beam_args ba = {.dtype = QMH_F32, .n_groups = n_seq, .n_beams = 1, .vocab = c->vocab_size, .n_out = n_seq < 64 ? n_seq : 64};
+    b->beam_ws = qmh_beam_ws_bytes(&ba);
+    if (e == hipSuccess) e = hipMalloc((void **)&b->d_score, sizeof(float) * (size_t)n_seq);
+    if (e == hipSuccess) e = hipMalloc((void **)&b->d_done, sizeof(int32_t) * (size_t)n_seq);
+    if (e == hipSuccess) e = hipMalloc((void **)&b->d_parent, sizeof(int32_t) * (size_t)n_seq);
+    if (e == hipSuccess) e = hipMalloc((void **)&b->d_choice, sizeof(int32_t) * (size_t)n_seq);
+    if (e == hipSuccess) e = hipMalloc(&b->d_beam_ws, b->beam_ws);
     if (e == hipSuccess) e = hipMemsetAsync(b->d_kt, 0, kv * sizeof(float), g_stream);
     if (e == hipSuccess) e = hipMemsetAsync(b->d_v, 0, kv * sizeof(float), g_stream);
     if (e == hipSuccess) e = hipStreamSynchronize(g_stream);
@@ -1722,6 +1735,98 @@ int qmh_batch_greedy(qmh_batch *b, const int32_t *tokens, const int32_t *pos, in
     if (n_steps > 0 && out)
         HIPCHK(hipMemcpyAsync(out, b->d_record, sizeof(int32_t) * (size_t)n_steps * B, hipMemcpyDeviceToHost,
                               g_stream));
+    HIPCHK(hipStreamSynchronize(g_stream));
+    return 0;
+}
+
+/* the caches of the batch's sequences, first n_pos positions, by device parents */
+static int batch_move(qmh_batch *b, const int32_t *d_parent, int n_beams, int n_pos, hipStream_t s) {
+    const qmh_config *c = &b->m->cfg;
+    const int64_t seq = (int64_t)b->m->kvd * c->max_seq * sizeof(float), kvd = b->m->kvd;
+    const qmh_beam_state k = {c->n_layers, seq * b->n, seq, kvd, (int64_t)c->max_seq * sizeof(float), (int64_t)n_pos * sizeof(float)};
+    const qmh_beam_state v = {c->n_layers, seq * b->n, seq, 1, seq, (int64_t)n_pos * kvd * sizeof(float)};
+    LCHK(qmh_launch_beam_reorder(&k, b->d_kt, b->d_kt, d_parent, b->n / n_beams, n_beams, s));
+    LCHK(qmh_launch_beam_reorder(&v, b->d_v, b->d_v, d_parent, b->n / n_beams, n_beams, s));
+    return 0;
+}
+
+static int check_beams(const qmh_batch *b, int32_t n_beams, const char *me) {
+    if (n_beams < 1 || n_beams > 64 || b->n % n_beams) return fail("%s: %d sequences in groups of %d (1 to 64)", me, b->n, n_beams);
+    return 0;
+}
+
+int qmh_batch_reorder(qmh_batch *b, const int32_t *parent, int32_t n_beams, int32_t n_pos) {
+    if (!b || !parent) return fail("batch_reorder: NULL argument");
+    if (check_beams(b, n_beams, "batch_reorder")) return -1;
+    if (n_pos < 0 || n_pos > b->m->cfg.max_seq) return fail("batch_reorder: n_pos %d outside [0, %d]", n_pos, b->m->cfg.max_seq);
+    if (n_pos == 0) return 0;
+    memcpy(b->h_io, parent, sizeof(int32_t) * (size_t)b->n);
+    HIPCHK(hipMemcpyAsync(b->d_parent, b->h_io, sizeof(int32_t) * (size_t)b->n, hipMemcpyHostToDevice, g_stream));
+    const int rc = batch_move(b, b->d_parent, n_beams, n_pos, g_stream);
+    HIPCHK(hipStreamSynchronize(g_stream));
+    return rc;
+}
+
+/* one step of the search: forward, choice, the tokens so far and the caches after it, next tokens */
+static int beam_step(qmh_batch *b, const qmh_beam_args *a, int max_pos, int k, int eos, hipStream_t s) {
+    const int nb = a->n_beams, cap = b->record_cap;
+    if (batch_step(b, max_pos, s)) return -1;
+    LCHK(qmh_launch_beam_select(a, b->d_beam_ws, s));
+    const qmh_beam_state h = {1, 0, (int64_t)cap * sizeof(int32_t), 1, 0, (int64_t)k * sizeof(int32_t)};
+    if (k) LCHK(qmh_launch_beam_reorder(&h, b->d_record, b->d_record, b->d_parent, a->n_groups, nb, s));
+    if (batch_move(b, b->d_parent, nb, max_pos + 1, s)) return -1;
+    LCHK(qmh_launch_beam_advance(b->d_parent, b->d_choice, eos, a->n_groups, nb, b->d_done, b->d_tok, b->d_pos, b->d_record, cap, k, s));
+    return 0;
+}
+
+int qmh_batch_beam(qmh_batch *b, int32_t n_beams, const int32_t *tokens, const int32_t *pos, int32_t n_steps, int32_t eos,
+                   int32_t *out, float *scores, double *ms) {
+    if (!b || !tokens || !pos || n_steps < 0) return fail("batch_beam: bad argument");
+    if (check_beams(b, n_beams, "batch_beam")) return -1;
+    const int B = b->n, V = b->m->cfg.vocab_size, G = B / n_beams;
+    if (eos >= V) return fail("batch_beam: eos %d outside the vocabulary", eos);
+    for (int i = 0; i < B; i++) {
+        b->h_io[i] = tokens[i / n_beams];
+        b->h_io[B + i] = pos[i / n_beams];
+    }
+    int max_pos;
+    if (batch_check(b, b->h_io, b->h_io + B, n_steps, &max_pos)) return -1;
+    HIPCHK(hipMemcpyAsync(b->d_tok, b->h_io, sizeof(int32_t) * (size_t)B, hipMemcpyHostToDevice, g_stream));
+    HIPCHK(hipMemcpyAsync(b->d_pos, b->h_io + B, sizeof(int32_t) * (size_t)B, hipMemcpyHostToDevice, g_stream));
+    HIPCHK(hipStreamSynchronize(g_stream));
+    float *h = (float *)b->h_io; /* a group's beams are one at first */
+    for (int i = 0; i < B; i++) {
+        h[i] = i % n_beams ? -INFINITY : 0.0f;
+        b->h_io[B + i] = 0;
+    }
+    HIPCHK(hipMemcpyAsync(b->d_score, h, sizeof(float) * (size_t)B, hipMemcpyHostToDevice, g_stream));
+    HIPCHK(hipMemcpyAsync(b->d_done, b->h_io + B, sizeof(int32_t) * (size_t)B, hipMemcpyHostToDevice, g_stream));
+    const qmh_beam_args a = {.dtype = QMH_F32, .n_groups = G, .n_beams = n_beams, .vocab = V, .n_out = n_beams, .eos = eos < 0 ? 0 : eos,
+                             .logits = b->m->d_pf_logits, .stride = V, .score = b->d_score, .done = eos < 0 ? NULL : b->d_done,
+                             .out_score = b->d_score, .out_parent = b->d_parent, .out_token = b->d_choice};
+    if (qmh_beam_ws_bytes(&a) > b->beam_ws) return fail("batch_beam: workspace"); /* not reached: sized for every group size */
+    hipEvent_t e0 = NULL, e1 = NULL;
+    if (ms) {
+        HIPCHK(hipEventCreate(&e0));
+        HIPCHK(hipEventCreate(&e1));
+        HIPCHK(hipEventRecord(e0, g_stream));
+    }
+    int rc = 0;
+    for (int32_t k = 0; k < n_steps && !rc; k++) rc = beam_step(b, &a, max_pos + k, k, eos < 0 ? -2 : eos, g_stream);
+    if (!rc && ms) {
+        HIPCHK(hipEventRecord(e1, g_stream));
+        HIPCHK(hipEventSynchronize(e1));
+        float f = 0.0f;
+        HIPCHK(hipEventElapsedTime(&f, e0, e1));
+        *ms = f;
+    }
+    if (e0) hipEventDestroy(e0);
+    if (e1) hipEventDestroy(e1);
+    if (rc) return -1;
+    if (n_steps > 0 && out)
+        HIPCHK(hipMemcpy2DAsync(out, sizeof(int32_t) * (size_t)n_steps, b->d_record, sizeof(int32_t) * (size_t)b->record_cap,
+                                sizeof(int32_t) * (size_t)n_steps, (size_t)B, hipMemcpyDeviceToHost, g_stream));
+    if (scores) HIPCHK(hipMemcpyAsync(scores, b->d_score, sizeof(float) * (size_t)B, hipMemcpyDeviceToHost, g_stream));
     HIPCHK(hipStreamSynchronize(g_stream));
     return 0;
 }
