@@ -445,6 +445,7 @@ struct attn_wave {
     __device__ __forceinline__ void walk(const attn_args &s, const attn_list &L, int kvh, float sc, int full, bool &bad) {
         const int w = uniform((int)(threadIdx.x >> 6));
         int base = L.from + w * KS;
+        if (base > L.cap) return; // no table entry to look at (a list that is none has no table)
         pages pg = fetch(s, L, base);
         if (base >= L.to) return;
         blocks bl = locate(s, L, pg, base, kvh, bad);
@@ -575,7 +576,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(const attn_args s) {
     const attn_plan &n = s.n;
     const int KV = s.p.n_kv_heads, Q = s.a.q_len;
     uint32_t b = blockIdx.x;
-    const attn_list none = {nullptr, 0, 0, 0, 0, 0};
+    const attn_list none = {nullptr, 0, 0, 0, 0, -1};
     if (b < n.pre_blocks) { // split, (group, kv head); row tile: tiles of the same keys 8 blocks apart, on one XCD's cache
         const uint32_t gks = (uint32_t)s.a.n_groups * KV, line = b / (8 * n.pt), in = b - line * 8 * n.pt, unit = line * 8 + (in & 7);
         const int tile = (int)(in >> 3), split = (int)(unit / gks);
