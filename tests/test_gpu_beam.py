@@ -168,3 +168,40 @@ def test_beam_reorder(gpu, inplace, beams, outer, rows, row_stride, live, gap, s
         assert np.array_equal(dd.get(), want)
         if not inplace:
             assert np.array_equal(ds.get(), src)
+
+
+def test_select_more_rows_than_a_grid_dimension(gpu):
+    """80000 rows: the rows pass one launch's limit."""
+    q, G, K, V = gpu, 40000, 2, 9
+    rs = np.random.default_rng(6)
+    x, score = rs.standard_normal((G, K, V)).astype(np.float32), -rs.random((G, K)).astype(np.float32)
+    dx, ds = o.Guarded(q, x), o.Guarded(q, score)
+    out = [o.Guarded(q, np.zeros((G, 2), t)) for t in (np.float32, np.int32, np.int32)]
+    a = q.BeamArgs(dtype=o.F32, n_groups=G, n_beams=K, vocab=V, n_out=2, eos=0, logits=dx.ptr, stride=V, score=ds.ptr, out_score=out[0].ptr,
+                   out_parent=out[1].ptr, out_token=out[2].ptr)
+    L = q.load_library()
+    need = L.qmh_beam_select_ws(ctypes.byref(a))
+    ws = o.Guarded(q, np.full(need, 0xFF, np.uint8))
+    q._check(L.qmh_beam_select(ctypes.byref(a), ws.ptr, need, None), "select")
+    q.sync()
+    ws.get()
+    p, t = out[1].get(), out[2].get()
+    for g in list(range(0, 40)) + list(range(32740, 32800)) + list(range(G - 40, G)):
+        want = best_of(x[g].astype(np.float64), score[g].astype(np.float64), None, 2, 0)
+        assert list(p[g]) == [w[1] for w in want] and list(t[g]) == [w[2] for w in want], g
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n_out", [1, 16, 64])
+def test_select_long_rows(gpu, dtype, n_out):
+    """Rows of several pieces a wave (many rows share the chip): rising, falling, sawtooth, repeated and random."""
+    rs = np.random.default_rng(n_out)
+    V, G = 30011, 100
+    kinds = [np.arange(V) * 1e-3, -np.arange(V) * 1e-3, (np.arange(V) % 700) * 0.01, np.zeros(V), np.where(np.arange(V) % 5000 == 4999, 3.0, -1.0)]
+    x = rs.standard_normal((G, 2, V)).astype(np.float32) * 2
+    for i, k in enumerate(kinds):
+        x[i, 0] = k
+        x[i + 10, 1] = k
+    x[20, :, ::3] = -np.inf
+    x[21, 0, 29000] = np.nan
+    run_select(gpu, x, -rs.random((G, 2)), None, n_out, dt=o.TYPES[dtype])

@@ -407,3 +407,154 @@ def test_paged_reorder(gpu, dtype, groups, beams, KV, hd, ps):
                 if 0 <= a < n_pages and 0 <= b < n_pages:
                     wk[b, :, t % ps], wv[b, :, t % ps] = k[a, :, t % ps], v[a, :, t % ps]
         assert np.array_equal(dk.get(), wk) and np.array_equal(dv.get(), wv), trial
+
+
+# ------------------------------------------------------------------------------------- long caches, graphs, streams
+
+def test_pages_past_4_gib(gpu):
+    """Pages at both ends of pools of 5 GiB each: append writes there, attention reads there, the reorder moves them."""
+    q, L, KV, hd, ps, H = gpu, gpu.load_library(), 2, 128, 1024, 4
+    n_pages = (5 << 30) // (KV * ps * hd * 2)
+    rs = np.random.default_rng(12)
+    pool = [q.DeviceBuffer(n_pages * KV * ps * hd * 2) for _ in range(2)]
+    p = pages_of(q, o.BF16, KV, hd, ps, n_pages, pool[0].ptr, pool[1].ptr)
+    table = np.array([[n_pages - 1, 1], [n_pages - 3, n_pages - 2]], np.int32)
+    ptable = np.array([[n_pages - 4]], np.int32)
+    tabs = np.concatenate([table, np.array([[n_pages - 4, -1]], np.int32)])
+    lens = [1030, 1025, 700]
+    tok = [(s, t) for s, n in enumerate(lens) for t in range(n)]
+    seq, slot = np.array([s for s, _ in tok], np.int32), np.array([t for _, t in tok], np.int32)
+    n, width = len(tok), 2 * KV * hd
+    x = o.encode(rs.standard_normal((n, width)), o.BF16)
+    dx, ds, dl, dt = (q.DeviceBuffer.from_array(a) for a in (x, seq, slot, tabs))
+    a = q.AppendArgs(pages=ctypes.pointer(p), n_tokens=n, k=dx.ptr, k_stride=width, v=dx.ptr + 2 * KV * hd, v_stride=width, n_seq=3, table=dt.ptr,
+                     table_stride=2, seq=ds.ptr, slot=dl.ptr)
+    q._check(L.qmh_paged_append(ctypes.byref(a), None), "append")
+    xv = o.decode(x, o.BF16).reshape(n, 2, KV, hd)
+    hist = [xv[seq == s] for s in range(3)]
+    qx = o.encode(rs.standard_normal((2, H * hd)), o.BF16)
+    dq, dout, dtab, dptab = q.DeviceBuffer.from_array(qx), q.DeviceBuffer(2 * H * hd * 2), q.DeviceBuffer.from_array(table), q.DeviceBuffer.from_array(ptable)
+    dlen, dplen = q.DeviceBuffer.from_array(np.array(lens[:2], np.int32)), q.DeviceBuffer.from_array(np.array(lens[2:], np.int32))
+    t = q.AttentionArgs(pages=ctypes.pointer(p), n_heads=H, n_seq=2, q_len=1, n_groups=1, q=dq.ptr, q_stride=H * hd, out=dout.ptr, out_stride=H * hd,
+                        table=dtab.ptr, len=dlen.ptr, table_stride=2, max_len=1100, prefix_table=dptab.ptr, prefix_len=dplen.ptr, prefix_stride=1,
+                        max_prefix=700, scale=hd ** -0.5)
+    need = L.qmh_paged_attention_ws(ctypes.byref(t))
+    ws = q.DeviceBuffer(max(need, 1))
+
+    def check(own):
+        q._check(L.qmh_paged_attention(ctypes.byref(t), ws.ptr, need, None), "attention")
+        q.sync()
+        got = o.decode(dout.to_array(np.uint16), o.BF16).reshape(2, H, hd)
+        for i in range(2):
+            kk, vv = (np.concatenate([hist[2][:, c], own[i][:, c]]) for c in range(2))
+            want, mag, _ = o.attention(o.decode(qx[i], o.BF16).reshape(H, hd), kk, vv, hd ** -0.5)
+            o.close(got[i], want, mag * 2 * o.HALF[o.BF16] + np.abs(want) * o.HALF[o.BF16] + 1e-4, f"sequence {i}")
+    check(hist[:2])
+    dpar, dlen2 = q.DeviceBuffer.from_array(np.array([1, 0], np.int32)), q.DeviceBuffer.from_array(np.array([1025, 1025], np.int32))
+    q._check(L.qmh_paged_reorder(ctypes.byref(p), dtab.ptr, 2, dlen2.ptr, 1030, dpar.ptr, 1, 2, None), "reorder")
+    check([np.concatenate([hist[1], hist[0][1025:]]), hist[0][:1025]])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_long_queries(gpu, dtype):
+    # a suffix of many tokens per sequence: tiles of queries with their own ends
+    run_attention(gpu, o.TYPES[dtype], 8, 2, 64, 16, 1, 2, 200, [90], [200, 333], seed=20)
+    run_attention(gpu, o.TYPES[dtype], 2, 2, 128, 32, 2, 1, 77, [0, 40], [80, 77], seed=21)
+    run_attention(gpu, o.TYPES[dtype], 2, 2, 256, 32, 1, 2, 20, [65], [30, 20], seed=22)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_bounds_above_the_lengths(gpu, dtype):
+    # upper bounds far above every length: chunks that hold nothing
+    run_attention(gpu, o.TYPES[dtype], 4, 2, 64, 16, 2, 2, 1, [100, 5], [3, 40, 1, 17], seed=23, max_len=3000, max_prefix=9000)
+    run_attention(gpu, o.TYPES[dtype], 4, 4, 64, 16, 2, 2, 2, [0, 0], [3, 40, 2, 17], seed=24, max_len=3000, max_prefix=9000)
+
+
+def test_append_one_gain_only(gpu):
+    """Only the keys are normed: queries turn as they are."""
+    q, L, H, KV, hd, n = gpu, gpu.load_library(), 2, 1, 64, 5
+    rs = np.random.default_rng(31)
+    x = rs.standard_normal((n, (H + 2 * KV) * hd)).astype(np.float32)
+    g = (1 + 0.2 * rs.standard_normal(hd)).astype(np.float32)
+    pool = [o.Guarded(q, np.zeros((1, KV, 16, hd), np.float32)) for _ in range(2)]
+    p = pages_of(q, o.F32, KV, hd, 16, 1, pool[0].ptr, pool[1].ptr)
+    dx, dg, out = o.Guarded(q, x), o.Guarded(q, g), o.Guarded(q, np.zeros((n, H * hd), np.float32))
+    dz, dl, dt = (o.Guarded(q, np.array(a, np.int32)) for a in (np.zeros(n), np.arange(n), [[0]]))
+    with q.Rotary(hd, max_pos=64) as r:
+        a = q.AppendArgs(pages=ctypes.pointer(p), rotary=r.handle, n_tokens=n, n_heads=H, q=dx.ptr, q_stride=x.shape[1], q_out=out.ptr, q_out_stride=H * hd,
+                         k=dx.ptr + 4 * H * hd, k_stride=x.shape[1], v=dx.ptr + 4 * (H + KV) * hd, v_stride=x.shape[1], k_gain=dg.ptr, eps=1e-5, n_seq=1,
+                         table=dt.ptr, table_stride=1, seq=dz.ptr, slot=dl.ptr)
+        q._check(L.qmh_paged_append(ctypes.byref(a), None), "append")
+        q.sync()
+    f, at, xv = o.freqs(hd, "none"), np.arange(n), x.astype(np.float64).reshape(n, -1, hd)
+    tol = (hd + 12) * o.U32 * 2 * np.abs(xv).max() * 1.5
+    o.close(out.get().reshape(n, H, hd), o.rotate(xv[:, :H], at, f, "pairs"), tol, "queries")
+    o.close(pool[0].get()[0, :, :n].transpose(1, 0, 2), o.rotate(o.norm(xv[:, H:H + KV], g.astype(np.float64), 1e-5), at, f, "pairs"), tol, "keys")
+
+
+def test_step_in_a_graph(gpu):
+    """Append, attention, selection and reorder of one step captured together, replayed with new contents between eager
+    work: every replay leaves what the eager calls leave on the same contents."""
+    q, L, hip = gpu, gpu.load_library(), _hip()
+    rs = np.random.default_rng(40)
+    KV, H, hd, ps, B, V, ml = 2, 4, 64, 16, 4, 5000, 80
+    tables, n_pages = o.make_tables(rs, [8] + [5] * B, 8)
+    width = (H + 2 * KV) * hd
+    sizes = dict(k=n_pages * KV * ps * hd, v=n_pages * KV * ps * hd, x=B * width, logits=B * V)
+    dptab, dtab = q.DeviceBuffer.from_array(tables[:1]), q.DeviceBuffer.from_array(tables[1:])
+    seq = q.DeviceBuffer.from_array(np.arange(B, dtype=np.int32))
+    with q.Rotary(hd, "halves", "linear", factor=4.0, max_pos=1000) as rot:
+        sides = []
+        for _ in range(2):
+            d = {n: q.DeviceBuffer(c * (4 if n == "logits" else 2)) for n, c in sizes.items()}
+            d.update(q=q.DeviceBuffer(B * H * hd * 2), out=q.DeviceBuffer(B * H * hd * 2), slot=q.DeviceBuffer(4 * B), pos=q.DeviceBuffer(4 * B),
+                     len=q.DeviceBuffer(4 * B), plen=q.DeviceBuffer(4), score=q.DeviceBuffer(4 * B), parent=q.DeviceBuffer(4 * B), token=q.DeviceBuffer(4 * B))
+            p = pages_of(q, o.F16, KV, hd, ps, n_pages, d["k"].ptr, d["v"].ptr)
+            pp = ctypes.pointer(p)
+            a = q.AppendArgs(pages=pp, rotary=rot.handle, n_tokens=B, n_heads=H, q=d["x"].ptr, q_stride=width, q_out=d["q"].ptr, q_out_stride=H * hd,
+                             k=d["x"].ptr + 2 * H * hd, k_stride=width, v=d["x"].ptr + 2 * (H + KV) * hd, v_stride=width, n_seq=B, table=dtab.ptr, table_stride=8,
+                             seq=seq.ptr, slot=d["slot"].ptr, pos=d["pos"].ptr)
+            t = q.AttentionArgs(pages=pp, n_heads=H, n_seq=B, q_len=1, n_groups=1, q=d["q"].ptr, q_stride=H * hd, out=d["out"].ptr, out_stride=H * hd,
+                                table=dtab.ptr, len=d["len"].ptr, table_stride=8, max_len=ml, prefix_table=dptab.ptr, prefix_len=d["plen"].ptr, prefix_stride=8,
+                                max_prefix=128, scale=0.125)
+            s = q.BeamArgs(dtype=o.F32, n_groups=1, n_beams=B, vocab=V, n_out=B, logits=d["logits"].ptr, stride=V, score=d["score"].ptr,
+                           out_score=d["score"].ptr, out_parent=d["parent"].ptr, out_token=d["token"].ptr)
+            wa, wb = L.qmh_paged_attention_ws(ctypes.byref(t)), L.qmh_beam_select_ws(ctypes.byref(s))
+            ws = q.DeviceBuffer(max(wa, 1)), q.DeviceBuffer(wb)
+
+            def step(stream, a=a, t=t, s=s, p=p, d=d, ws=ws, wa=wa, wb=wb):
+                assert L.qmh_paged_append(ctypes.byref(a), stream) == 0, q.last_error()
+                assert L.qmh_paged_attention(ctypes.byref(t), ws[0].ptr, wa, stream) == 0, q.last_error()
+                assert L.qmh_beam_select(ctypes.byref(s), ws[1].ptr, wb, stream) == 0, q.last_error()
+                assert L.qmh_paged_reorder(ctypes.byref(p), dtab.ptr, 8, d["len"].ptr, ml, d["parent"].ptr, 1, B, stream) == 0, q.last_error()
+            sides.append((d, step, p))
+        stream, graph, exe = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+        assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+        try:
+            assert hip.hipStreamBeginCapture(stream, 1) == 0
+            sides[0][1](stream)
+            assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+            assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, 0) == 0
+            for trial in range(5):
+                n = int(rs.integers(1, ml + 1))
+                vals = dict(slot=np.full(B, n - 1, np.int32), pos=np.full(B, 100 + n, np.int32), len=np.full(B, n, np.int32),
+                            plen=np.array([rs.integers(0, 129)], np.int32), score=-rs.random(B).astype(np.float32))
+                for name, c in sizes.items():
+                    h = rs.standard_normal(c)
+                    vals[name] = h.astype(np.float32) if name == "logits" else o.encode(h, o.F16)
+                for d, _, _ in sides:
+                    for name, h in vals.items():
+                        L.qmh_memcpy_h2d(d[name].ptr, h.ctypes.data, h.nbytes)
+                sides[1][1](None)
+                q.sync()
+                assert hip.hipGraphLaunch(exe, stream) == 0
+                assert hip.hipStreamSynchronize(stream) == 0
+                for name in ("k", "v", "q", "out", "score", "parent", "token"):
+                    x, y = (d[name].to_array(np.uint8) for d, _, _ in sides)
+                    assert np.array_equal(x, y), (trial, name)
+        finally:
+            if exe:
+                hip.hipGraphExecDestroy(exe)
+            if graph:
+                hip.hipGraphDestroy(graph)
+            hip.hipStreamDestroy(stream)
