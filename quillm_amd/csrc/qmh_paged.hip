@@ -669,8 +669,15 @@ attn_plan plan_attention(const qmh_attention_args *a, int cus) {
     int64_t pre = 0;
     n.os = 1;
     n.oc = a->max_len ? a->max_len : 1;
-    // short sequences: each reads the prefix itself, which costs less than another launch
-    n.joint = a->max_prefix == 0 ? a->max_len <= 512 : a->max_prefix + a->max_len <= 256;
+    // Short sequences: a workgroup each that reads the prefix itself, which costs less than a launch that joins parts, while
+    // its walk is short (counted in positions of 64 16-bit values) and the prefix is not read too often. Joint against parts:
+    // 4 x 4 heads of 64 f16, 300 + 100 positions 6.6 us to 7.8; 32 of 128 bf16, 4 sequences, 180 + 60 7.3 to 8.7, but 2 x 16
+    // sequences, 200 + 50 (98 MB more) 17.3 to 15.2; own pages alone: 192 walks of 500 7.5 to 11, 32 of 500 x 128 even, 2 of
+    // 500 f32 8.7 to 7.9.
+    const int64_t far = (int64_t)a->max_prefix + a->max_len, es = p->dtype == QMH_F32 ? 4 : 2;
+    const int64_t walk = far * (p->head_dim <= 64 ? 1 : p->head_dim <= 128 ? 2 : 4) * (es / 2);
+    const int64_t again = (uo - up) * a->max_prefix * p->head_dim * es * 2;
+    n.joint = a->max_prefix ? walk <= 512 && again <= 32 << 20 : walk <= (uo >= 32 ? 1024 : 512);
     if (!n.joint) {
         // chunks of positions, about the same for both, that fill the chip's workgroups (two per CU) once
         const int64_t all = up * a->max_prefix + uo * a->max_len;
