@@ -309,11 +309,15 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     const int share = K < NW ? NW / K : 1, per = segs * n_out;
     const int b0 = w / share < NW / share ? w / share : K, j0 = (w % share) * 64 + lane;
     // the first row's first heads and candidates are asked for at once with its score (of a dead row they are not used)
-    scan_head h0 = {0.0, 0.0f, 0.0f};
+    double sum0 = 0.0;
+    float ref0 = 0.0f;
     uint2 v0[4];
     if (b0 < K) {
         const int64_t at = (int64_t)(g * K + b0) * segs;
-        if (lane < segs) h0 = heads[at + lane];
+        if (lane < segs) {
+            sum0 = heads[at + lane].sum;
+            ref0 = heads[at + lane].ref;
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) v0[k] = j0 + 64 * share * k < per ? cands[at * n_out + j0 + 64 * share * k] : make_uint2(0, 0);
     }
@@ -324,13 +328,15 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
         double s = __builtin_nan("");
         if (!done && sc > -__builtin_inff()) {
             const scan_head *h = heads + (int64_t)row * segs;
-            const scan_head one = b == b0 || lane >= segs ? h0 : h[lane];
-            float m = one.sum == 0.0 ? -__builtin_inff() : one.ref;
+            if (b != b0 && lane < segs) {
+                sum0 = h[lane].sum;
+                ref0 = h[lane].ref;
+            }
+            float m = sum0 == 0.0 ? -__builtin_inff() : ref0;
             for (int c = lane + 64; c < segs; c += 64) m = h[c].sum == 0.0 ? m : fmaxf(m, h[c].ref);
             m = qmh_wave_max(m);
             const double ref2 = (double)m * 1.4426950408889634074;
-            const float r0 = one.ref;
-            s = one.sum == 0.0 || lane >= segs ? 0.0 : one.sum * exp_sum<1>(&r0, m - 700.0f, ref2);
+            s = sum0 == 0.0 ? 0.0 : sum0 * exp_sum<1>(&ref0, m - 700.0f, ref2);
             for (int c = lane + 64; c < segs; c += 64) s = __builtin_fma(h[c].sum, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
             s = (double)m + log(qmh_wave_sum_d(s)); // a row without a logit: NaN, and no continuation
         }
@@ -340,46 +346,63 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
         }
     }
     __syncthreads();
-    // body(ordered key of the total, place = beam * vocab + token) for each candidate of the wave's rows
+    // body(ordered keys of the totals (0: none), places beam * vocab + token), four candidates a lane, all lanes at once
     auto each = [&](auto body) {
         for (int b = b0; b < K; b += NW / share) {
             const double L = lse[b], sc = score[b];
+            uint64_t q[4] = {};
+            uint32_t p[4] = {};
             if (L == __builtin_inf()) { // finished: one continuation
-                const uint64_t q = key_of_d(sc);
-                if (lane == 0 && w % share == 0 && q) body(q, (uint32_t)(b * a.vocab + a.eos));
+                if (lane == 0 && w % share == 0) q[0] = key_of_d(sc);
+                p[0] = (uint32_t)(b * a.vocab + a.eos);
+                body(q, p);
                 continue;
             }
             if (L != L) continue;
             const uint2 *c = cands + (int64_t)(g * K + b) * per;
             for (int i = 0; i < per; i += 256 * share) {
-                uint2 v[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const int j = i + j0 + 64 * share * k;
-                    v[k] = b == b0 && i == 0 ? v0[k] : j < per ? c[j] : make_uint2(0, 0);
+                    const uint2 v = b == b0 && i == 0 ? v0[k] : j < per ? c[j] : make_uint2(0, 0);
+                    q[k] = v.x ? key_of_d(sc + ((double)of_key(v.x) - L)) : 0ull;
+                    p[k] = (uint32_t)(b * a.vocab) + v.y;
                 }
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint64_t q = v[k].x ? key_of_d(sc + ((double)of_key(v[k].x) - L)) : 0ull;
-                    if (q) body(q, (uint32_t)(b * a.vocab) + v[k].y);
-                }
+                body(q, p);
             }
         }
     };
     uint32_t mine = 0;
-    each([&](uint64_t q, uint32_t) { mine = (uint32_t)(q >> 32) > mine ? (uint32_t)(q >> 32) : mine; });
+    each([&](const uint64_t *q, const uint32_t *) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) mine = (uint32_t)(q[k] >> 32) > mine ? (uint32_t)(q[k] >> 32) : mine;
+    });
     const uint32_t bw = wave_nth<12>(mine, n_out);
     if (lane == 0) bounds[w] = bw;
     __syncthreads();
     uint32_t from = 1;
 #pragma unroll
     for (int k = 0; k < NW; k++) from = bounds[k] > from ? bounds[k] : from;
-    each([&](uint64_t q, uint32_t place) {
-        if ((uint32_t)(q >> 32) < from) return;
-        const int at = atomicAdd(&ncand, 1);
-        if (at < JOIN_CAP) {
-            ckey[at] = q;
-            cplace[at] = place;
+    each([&](const uint64_t *q, const uint32_t *p) { // places by ballots, one addition to the count a wave
+        uint64_t in[4];
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            in[k] = __ballot((uint32_t)(q[k] >> 32) >= from);
+            n += __popcll(in[k]);
+        }
+        if (!n) return;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&ncand, n);
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int to = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in[k] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[k], 0));
+            if ((in[k] >> lane & 1) && to < JOIN_CAP) {
+                ckey[to] = q[k];
+                cplace[to] = p[k];
+            }
+            at += __popcll(in[k]);
         }
     });
     __syncthreads();
@@ -404,11 +427,14 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     for (int o = 0; o < n_out; o++) {
         uint64_t best = 0;
         uint32_t at = 0xffffffffu;
-        each([&](uint64_t q, uint32_t place) {
-            if (q > below || (q == below && (int64_t)place <= after)) return;
-            if (q > best || (q == best && place < at)) {
-                best = q;
-                at = place;
+        each([&](const uint64_t *q, const uint32_t *p) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (!q[k] || q[k] > below || (q[k] == below && (int64_t)p[k] <= after)) continue;
+                if (q[k] > best || (q[k] == best && p[k] < at)) {
+                    best = q[k];
+                    at = p[k];
+                }
             }
         });
         for (int x = 1; x < 64; x <<= 1) {
