@@ -111,6 +111,8 @@ __device__ __forceinline__ void wave_sync() {
 // n_out best, the least of them, which only larger logits pass, since later ones lose a tie. Where a piece brings
 // more than the list holds (a rising row, repeated values) its own lane maxima raise the bound, and if that does not help
 // the exact bound of the piece is searched bit by bit.
+// Bound by VALU issue (34 instructions a logit, 14 of them the exponential's 64-bit ones: 21 of the 33 us of 24.6 million f32
+// logits) beside the loads (98 MB).
 template <typename T, int EPT, int VEC>
 __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_head *heads, uint2 *cands, int row0, int iters) {
     constexpr int PIECE = 64 * EPT;
@@ -295,8 +297,9 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
     if (lane == 0) heads[slot] = scan_head{bad ? __builtin_nan("") : none ? 0.0 : sum, ref, 0.0f};
 }
 
-// A group's choice from its rows' chunks: each row's log sum (a wave a row), then the n_out best totals as in the scan:
-// a bound from the lanes' best, what reaches it ranked in LDS. Where more than JOIN_CAP reach it, one after another.
+// A group's choice from its rows' segments: each row's log sum (a wave a row), then the n_out best totals as in the scan:
+// a bound from the lanes' best, what reaches it ranked in LDS. Where more than JOIN_CAP reach it, one after another. A
+// chain of short steps in one workgroup: 5 to 7 us, 4 of them an empty launch's.
 __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int segs) {
     constexpr int NW = JOIN_T / 64;
     __shared__ double lse[64], score[64];
@@ -467,13 +470,10 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     if (tid < n_out) write(tid, ckey[tid], cplace[tid]);
 }
 
-#ifndef SC_WAVES
-#define SC_WAVES 3072
-#endif
-#ifndef SC_EPT
-#define SC_EPT 16
-#endif
-// How a row is cut: into segments of whole pieces, one a wave, as many as give the chip about SC_WAVES waves.
+// How a row is cut: into segments of whole pieces, one a wave, as many as give the chip SCAN_WAVES waves: three a SIMD, so
+// that they run in one round. 192 rows of 128256 f32 measured 43 us so, 52 with two a SIMD and 47 with four (pieces then
+// divide worse); pieces of 8 logits a lane where that many waves have no more.
+constexpr int SCAN_WAVES = 3072, SCAN_EPT = 16;
 struct scan_plan {
     int ept, iters, segs; // segs: of a row, a multiple of a workgroup's waves
 };
@@ -481,9 +481,9 @@ scan_plan plan_scan(const qmh_beam_args *a) {
     constexpr int W = SEL_T / 64;
     const int64_t rows = (int64_t)a->n_groups * a->n_beams, len = (int64_t)a->vocab + 15; // 15: a row that starts inside a vector
     scan_plan p;
-    p.ept = rows * len <= (int64_t)SC_WAVES * 64 * 8 ? 8 : SC_EPT;
+    p.ept = rows * len <= (int64_t)SCAN_WAVES * 64 * 8 ? 8 : SCAN_EPT;
     const int64_t piece = 64 * p.ept, pieces = (len + piece - 1) / piece;
-    int64_t segs = SC_WAVES / rows / W * W;
+    int64_t segs = SCAN_WAVES / rows / W * W;
     segs = segs < W ? W : segs;
     p.iters = (int)((pieces + segs - 1) / segs);
     p.segs = (int)((pieces + (int64_t)p.iters * W - 1) / ((int64_t)p.iters * W)) * W;
@@ -492,7 +492,8 @@ scan_plan plan_scan(const qmh_beam_args *a) {
 
 // --------------------------------------------------------------------------- reorder
 
-// Thread: one unit of U (the widest that every row is aligned to) of one row, for all beams of a group. Every beam that
+// Thread: one unit of U (the widest that every row is aligned to) of one row, for all beams of a group. 12 MB take 6.2 us, 4 of
+// them an empty launch's; 684 MB (32 sequences, rows of 2800 bytes) 4.1 TB/s. Every beam that
 // takes another's state is read before any is written, so any parents move in place; a row's last bytes go in 4-byte
 // pieces, read together too, and single bytes. parents: uniform, by scalar loads.
 typedef const __attribute__((address_space(4))) int32_t *const_i32;
@@ -618,7 +619,7 @@ extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *st
         for (int r0 = 0; r0 < rows; r0 += 65535) {
             const dim3 g(p.segs / (SEL_T / 64), rows - r0 < 65535 ? rows - r0 : 65535);
             if (p.ept == 8) hipLaunchKernelGGL((k_beam_scan<T, 8, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
-            else hipLaunchKernelGGL((k_beam_scan<T, SC_EPT, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
+            else hipLaunchKernelGGL((k_beam_scan<T, SCAN_EPT, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
         }
     });
     hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);

@@ -167,7 +167,16 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
 //                 16-bit pairs are turned by byte permutes.
 // Rows behind a list's end are out of the loads' range and read as zero, whatever lies there. The four waves
 // of a workgroup take the steps of one chunk of positions in turn and are joined through LDS; chunks are joined by
-// k_attention_join.
+// k_attention_join. Probabilities are rounded to the rows' 16-bit type for the product with V (half a step of a value at
+// most 2^8 above the row's largest, as the sum of a few is; their sum is taken of the rounded ones), everything
+// else is f32; f32 rows stay f32 throughout, on the f32 MFMAs.
+// What bounds it: reading keys and values while a kv head has few rows (32 sequences of 350 to 700 own positions and
+// two shared prefixes of up to 4096, 32 x 128 bf16: 78 us for 396 MB, 5.1 TB/s, the rate of a large copy); VALU
+// issue where many rows share them (64 sequences x 8 heads on a prefix of 16380, 4 x 64 f16: a step of 64 rows and 32
+// positions is 36 MFMAs (577 cycles) and 163 VALU instructions, 32 of them exponentials at a quarter of the rate; the
+// prefix runs at 800 TFLOP/s between 32760 and 65520 positions, 28 us in all with starts, ends and the join of parts).
+// Two waves a SIMD (at most 256 registers) measured 47 -> 35 us against one; eight waves a workgroup and the next
+// scores between this step's exponentials gained nothing.
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -607,7 +616,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(const attn_args s) {
     attend<T, HDP, NRO>(s, lds, tile * 16 * NRO, Q * n.G, sq * Q, kvh, S, L, bad, n.ps + n.os > 1 ? n.ps + (int)split : -1);
 }
 
-// out = the parts of a row joined, a wave a row (parts at most 64: lane k weighs part k). 64 / D4 parts are read at
+// 4 to 5 us, most of it a launch. out = the parts of a row joined, a wave a row (parts at most 64: lane k weighs part k). 64 / D4 parts are read at
 // once, 4 values a lane.
 template <typename T, int D4>
 __global__ __launch_bounds__(256) void k_attention_join(const attn_args s, int parts) {
