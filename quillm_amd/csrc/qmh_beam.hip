@@ -15,6 +15,7 @@ constexpr int SEL_T = 256;    // threads of the scan
 constexpr int SEL_CAP = 256;  // candidates a wave of it lists
 constexpr int JOIN_T = 512;   // threads of the join
 constexpr int JOIN_CAP = 1024;
+constexpr int SCAN_WAVES = 3072, SCAN_EPT = 16; // of plan_scan
 
 // The sum of e^(x - ref) over N floats, in 64 bits, x at most 600 above ref (finite): x log2 e - ref log2 e = k + f,
 // |f| <= 1/2, and 2^k times a polynomial of degree 8 that meets 2^f at the nine Chebyshev points, at most 1.1e-12 of the
@@ -62,9 +63,10 @@ __device__ __forceinline__ double of_key_d(uint64_t k) {
     return __longlong_as_double((long long)((k >> 63) ? k ^ (1ull << 63) : ~k));
 }
 
-struct scan_head { // a wave's part of a segment of a row: the sum of exp(x - ref); NaN: the row has no continuation
+struct scan_head { // a segment of a row: the sum of exp(x - ref) (NaN: the row has no continuation), its largest logit's key
     double sum;
-    float ref, pad;
+    float ref;
+    uint32_t top;
 };
 
 // The largest t that at least n <= 64 of a wave's values reach, 0 if there is none above; with LOW, the largest whose LOW
@@ -92,6 +94,7 @@ __device__ __forceinline__ void rank_all(int n, int threads, B before, D done) {
         const int c = c0 + tid / per;
         int r = 0;
         if (c < n)
+#pragma unroll 8
             for (int i = part; i < n; i += per) r += before(i, c);
         for (int x = 1; x < per; x *= 2) r += __shfl_xor(r, x);
         if (c < n && part == 0) done(c, r);
@@ -294,28 +297,34 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
     cut();
     if (lane < n_out) cands[slot * n_out + lane] = lane < n ? list[lane] : make_uint2(0, 0);
     sum = qmh_wave_sum_d(sum);
-    if (lane == 0) heads[slot] = scan_head{bad ? __builtin_nan("") : none ? 0.0 : sum, ref, 0.0f};
+    if (lane == 0) heads[slot] = scan_head{bad ? __builtin_nan("") : none ? 0.0 : sum, ref, key_of(max)};
 }
 
 // A group's choice from its rows' segments: each row's log sum (a wave a row), then the n_out best totals as in the scan:
 // a bound from the lanes' best, what reaches it ranked in LDS. Where more than JOIN_CAP reach it, one after another. A
 // chain of short steps in one workgroup: 5 to 7 us, 4 of them an empty launch's.
+// MANY: a segment whose largest total is below the n_out-th largest of these has none of the best. The others are found
+// first (a bound from each row's, then one from what that leaves), and only their candidates are read.
+template <bool MANY>
 __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int segs) {
-    constexpr int NW = JOIN_T / 64;
+    constexpr int NW = JOIN_T / 64, TOPS = MANY ? SCAN_WAVES : 1;
     __shared__ double lse[64], score[64];
     __shared__ uint64_t ckey[JOIN_CAP], bk[NW];
     __shared__ uint32_t cplace[JOIN_CAP], bounds[NW], bf[NW];
-    __shared__ int ncand;
+    __shared__ uint32_t tops[TOPS], list_key[TOPS];
+    __shared__ uint16_t list[TOPS], chosen[TOPS];
+    __shared__ int ncand, nlist, nchosen;
     const int g = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63, K = a.n_beams, n_out = a.n_out;
-    if (tid == 0) ncand = 0;
-    // few beams: several waves a row, each with the row's log sum for itself
-    const int share = K < NW ? NW / K : 1, per = segs * n_out;
+    if (tid == 0) ncand = nlist = nchosen = 0;
+    // few beams: several waves a row, each with the row's log sum for itself (MANY: a wave a row)
+    const int share = !MANY && K < NW ? NW / K : 1, per = segs * n_out;
     const int b0 = w / share < NW / share ? w / share : K, j0 = (w % share) * 64 + lane;
+    auto behind = [&](uint64_t all) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0)); };
     // the first row's first heads and candidates are asked for at once with its score (of a dead row they are not used)
     double sum0 = 0.0;
     float ref0 = 0.0f;
     uint2 v0[4];
-    if (b0 < K) {
+    if (!MANY && b0 < K) {
         const int64_t at = (int64_t)(g * K + b0) * segs;
         if (lane < segs) {
             sum0 = heads[at + lane].sum;
@@ -324,13 +333,14 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
 #pragma unroll
         for (int k = 0; k < 4; k++) v0[k] = j0 + 64 * share * k < per ? cands[at * n_out + j0 + 64 * share * k] : make_uint2(0, 0);
     }
+    uint32_t mine = 0;
     for (int b = b0; b < K; b += NW / share) {
         const int row = g * K + b;
         const float sc = a.score[row];
-        const bool done = a.done && a.done[row];
+        const bool done = a.done && a.done[row], live = !done && sc > -__builtin_inff();
         double s = __builtin_nan("");
-        if (!done && sc > -__builtin_inff()) {
-            const scan_head *h = heads + (int64_t)row * segs;
+        const scan_head *h = heads + (int64_t)row * segs;
+        if (!MANY && live) {
             if (b != b0 && lane < segs) {
                 sum0 = h[lane].sum;
                 ref0 = h[lane].ref;
@@ -341,41 +351,152 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
             const double ref2 = (double)m * 1.4426950408889634074;
             s = sum0 == 0.0 ? 0.0 : sum0 * exp_sum<1>(&ref0, m - 700.0f, ref2);
             for (int c = lane + 64; c < segs; c += 64) s = __builtin_fma(h[c].sum, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
-            s = (double)m + log(qmh_wave_sum_d(s)); // a row without a logit: NaN, and no continuation
+            s = (double)m + log(qmh_wave_sum_d(s));
+        }
+        if constexpr (MANY) {
+            uint32_t *top = tops + b * segs;
+            scan_head v[4]; // the first 256 are asked for with the score
+            auto load = [&](int c) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = c + 64 * k < segs ? h[c + 64 * k] : scan_head{0.0, 0.0f, 0u};
+            };
+            load(lane);
+            if (live) {
+                float m = -__builtin_inff();
+                s = 0.0;
+                for (int c0 = lane; c0 - lane < segs; c0 += 256) {
+                    if (c0 != lane) load(c0);
+                    float to = m;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) to = v[k].sum == 0.0 ? to : fmaxf(to, v[k].ref);
+                    to = qmh_wave_max(to);
+                    const float ref = to > -__builtin_inff() ? to : 0.0f; // nothing yet: sums of 0
+                    const double ref2 = (double)ref * 1.4426950408889634074;
+                    if (to > m && m > -__builtin_inff()) s *= exp_sum<1>(&m, ref - 700.0f, ref2);
+                    m = to;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float r = v[k].sum == 0.0 ? ref : v[k].ref;
+                        s = __builtin_fma(v[k].sum, exp_sum<1>(&r, ref - 700.0f, ref2), s);
+                        if (c0 + 64 * k < segs) top[c0 + 64 * k] = v[k].top;
+                    }
+                }
+                s = (double)m + log(qmh_wave_sum_d(s));
+            }
+            uint32_t best = 0; // the tops become the high words of their totals' ordered keys
+            for (int c = lane; c < segs; c += 64) {
+                const uint32_t t = live && s == s ? top[c] : 0;
+                const uint32_t q = done && c == 0 ? (uint32_t)(key_of_d(sc) >> 32)
+                                   : t            ? (uint32_t)(key_of_d((double)sc + ((double)of_key(t) - s)) >> 32)
+                                                  : 0;
+                top[c] = q;
+                best = q > best ? q : best;
+            }
+            const uint32_t t = wave_nth<12>(best, n_out);
+            mine = t > mine ? t : mine;
         }
         if (lane == 0 && w % share == 0) {
             lse[b] = done ? __builtin_inf() : s; // marks a finished row
             score[b] = (double)sc;
         }
     }
-    __syncthreads();
-    // body(ordered keys of the totals (0: none), places beam * vocab + token), four candidates a lane, all lanes at once
-    auto each = [&](auto body) {
-        for (int b = b0; b < K; b += NW / share) {
-            const double L = lse[b], sc = score[b];
-            uint64_t q[4] = {};
-            uint32_t p[4] = {};
-            if (L == __builtin_inf()) { // finished: one continuation
-                if (lane == 0 && w % share == 0) q[0] = key_of_d(sc);
-                p[0] = (uint32_t)(b * a.vocab + a.eos);
-                body(q, p);
-                continue;
-            }
-            if (L != L) continue;
-            const uint2 *c = cands + (int64_t)(g * K + b) * per;
-            for (int i = 0; i < per; i += 256 * share) {
+    auto highest = [&](uint32_t at_least) { // of the waves' bounds
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int j = i + j0 + 64 * share * k;
-                    const uint2 v = b == b0 && i == 0 ? v0[k] : j < per ? c[j] : make_uint2(0, 0);
-                    q[k] = v.x ? key_of_d(sc + ((double)of_key(v.x) - L)) : 0ull;
-                    p[k] = (uint32_t)(b * a.vocab) + v.y;
-                }
-                body(q, p);
+        for (int k = 0; k < NW; k++) at_least = bounds[k] > at_least ? bounds[k] : at_least;
+        return at_least;
+    };
+    const int lanes = n_out <= 1 ? 1 : 1 << (32 - __builtin_clz(n_out - 1)); // of a chosen segment: a power of two
+    if constexpr (MANY) {
+        if (lane == 0) bounds[w] = mine;
+        __syncthreads();
+        uint32_t from = highest(1);
+        for (int c0 = 0; c0 < K * segs; c0 += JOIN_T) {
+            const int c = c0 + tid;
+            const uint32_t q = c < K * segs ? tops[c] : 0;
+            const uint64_t in = __ballot(q >= from);
+            int at = 0;
+            if (lane == 0 && in) at = atomicAdd(&nlist, __popcll(in));
+            at = __builtin_amdgcn_readfirstlane(at) + behind(in);
+            if (q >= from) {
+                list_key[at] = q;
+                list[at] = (uint16_t)c;
+            }
+        }
+        __syncthreads();
+        const int n = nlist;
+        uint32_t best = 0;
+        for (int i = lane; i < n; i += 64) best = list_key[i] > best ? list_key[i] : best;
+        const uint32_t t = wave_nth<12>(best, n_out);
+        from = t > from ? t : from;
+        for (int i0 = 0; i0 < n; i0 += JOIN_T) {
+            const int i = i0 + tid;
+            const bool take = i < n && list_key[i] >= from;
+            const uint64_t in = __ballot(take);
+            int at = 0;
+            if (lane == 0 && in) at = atomicAdd(&nchosen, __popcll(in));
+            at = __builtin_amdgcn_readfirstlane(at) + behind(in);
+            if (take) chosen[at] = list[i];
+        }
+    }
+    __syncthreads();
+    const int n_chosen = MANY ? nchosen : 0;
+    // lanes of them for each chosen segment, four a thread from segment number i on
+    auto of_chosen = [&](int i, uint64_t *q, uint32_t *p) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int e = i + ((k * NW + w) * 64 + lane) / lanes, o = lane & (lanes - 1);
+            q[k] = 0;
+            if (e < n_chosen && o < n_out) {
+                const int c = chosen[e];
+                const uint2 v = cands[((int64_t)g * K * segs + c) * n_out + o];
+                const int b = c / segs;
+                const double L = lse[b], sc = score[b];
+                const bool done = L == __builtin_inf(); // one continuation
+                q[k] = done ? o == 0 ? key_of_d(sc) : 0ull : v.x ? key_of_d(sc + ((double)of_key(v.x) - L)) : 0ull;
+                p[k] = (uint32_t)(b * a.vocab) + (done ? (uint32_t)a.eos : v.y);
             }
         }
     };
-    uint32_t mine = 0;
+    uint64_t q0[4] = {};
+    uint32_t p0[4] = {};
+    if constexpr (MANY) of_chosen(0, q0, p0);
+    // body(ordered keys of the totals (0: none), places beam * vocab + token), four candidates a lane, all lanes at once
+    auto each = [&](auto body) {
+        if constexpr (MANY) {
+            body(q0, p0);
+            for (int i = 4 * JOIN_T / lanes; i < n_chosen; i += 4 * JOIN_T / lanes) {
+                uint64_t q[4];
+                uint32_t p[4] = {};
+                of_chosen(i, q, p);
+                body(q, p);
+            }
+        } else {
+            for (int b = b0; b < K; b += NW / share) {
+                const double L = lse[b], sc = score[b];
+                uint64_t q[4] = {};
+                uint32_t p[4] = {};
+                if (L == __builtin_inf()) { // finished
+                    if (lane == 0 && w % share == 0) q[0] = key_of_d(sc);
+                    p[0] = (uint32_t)(b * a.vocab + a.eos);
+                    body(q, p);
+                    continue;
+                }
+                if (L != L) continue;
+                const uint2 *c = cands + (int64_t)(g * K + b) * per;
+                for (int i = 0; i < per; i += 256 * share) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int j = i + j0 + 64 * share * k;
+                        const uint2 v = b == b0 && i == 0 ? v0[k] : j < per ? c[j] : make_uint2(0, 0);
+                        q[k] = v.x ? key_of_d(sc + ((double)of_key(v.x) - L)) : 0ull;
+                        p[k] = (uint32_t)(b * a.vocab) + v.y;
+                    }
+                    body(q, p);
+                }
+            }
+        }
+    };
+    mine = 0;
     each([&](const uint64_t *q, const uint32_t *) {
 #pragma unroll
         for (int k = 0; k < 4; k++) mine = (uint32_t)(q[k] >> 32) > mine ? (uint32_t)(q[k] >> 32) : mine;
@@ -383,9 +504,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     const uint32_t bw = wave_nth<12>(mine, n_out);
     if (lane == 0) bounds[w] = bw;
     __syncthreads();
-    uint32_t from = 1;
-#pragma unroll
-    for (int k = 0; k < NW; k++) from = bounds[k] > from ? bounds[k] : from;
+    const uint32_t from = highest(1);
     each([&](const uint64_t *q, const uint32_t *p) { // places by ballots, one addition to the count a wave
         uint64_t in[4];
         int n = 0;
@@ -400,7 +519,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
         at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int to = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in[k] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[k], 0));
+            const int to = at + behind(in[k]);
             if ((in[k] >> lane & 1) && to < JOIN_CAP) {
                 ckey[to] = q[k];
                 cplace[to] = p[k];
@@ -418,7 +537,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     const int n = ncand;
     if (n <= JOIN_CAP) { // every score has been read: out_score may be score
         rank_all(
-            n, JOIN_T, [&](int i, int c) { return ckey[i] > ckey[c] || (ckey[i] == ckey[c] && cplace[i] < cplace[c]); },
+            n, JOIN_T, [&](int i, int c) { return (ckey[i] > ckey[c]) | ((ckey[i] == ckey[c]) & (cplace[i] < cplace[c])); }, // no branches: the reads overlap
             [&](int c, int r) {
                 if (r < n_out) write(r, ckey[c], cplace[c]);
             });
@@ -473,7 +592,6 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
 // How a row is cut: into segments of whole pieces, one a wave, as many as give the chip SCAN_WAVES waves: three a SIMD, so
 // that they run in one round. 192 rows of 128256 f32 measured 43 us so, 52 with two a SIMD and 47 with four (pieces then
 // divide worse); pieces of 8 logits a lane where that many waves have no more.
-constexpr int SCAN_WAVES = 3072, SCAN_EPT = 16;
 struct scan_plan {
     int ept, iters, segs; // segs: of a row, a multiple of a workgroup's waves
 };
@@ -488,6 +606,13 @@ scan_plan plan_scan(const qmh_beam_args *a) {
     p.iters = (int)((pieces + segs - 1) / segs);
     p.segs = (int)((pieces + (int64_t)p.iters * W - 1) / ((int64_t)p.iters * W)) * W;
     return p;
+}
+// Which join: with more than 8 candidates of a row a lane, most of them not worth reading. 12 rows of 57576, n_out 24 (116
+// segments a row): 18.6 us with it, 64 without; 4 rows of 151936, n_out 8 (300): 14.9 and 25; 4 rows of 32000, n_out 8
+// (64): 12.1 and 10.9; 40 rows of 3488, n_out 6 (8): 13.7 and 10.9.
+bool many_segments(const qmh_beam_args *a, int segs) {
+    const int share = a->n_beams < JOIN_T / 64 ? JOIN_T / 64 / a->n_beams : 1;
+    return segs * a->n_out > 512 * share;
 }
 
 // --------------------------------------------------------------------------- reorder
@@ -622,7 +747,8 @@ extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *st
             else hipLaunchKernelGGL((k_beam_scan<T, SCAN_EPT, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
         }
     });
-    hipLaunchKernelGGL(k_beam_join, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);
+    if (many_segments(a, p.segs)) hipLaunchKernelGGL(k_beam_join<true>, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);
+    else hipLaunchKernelGGL(k_beam_join<false>, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);
     return (int)hipGetLastError();
 }
 

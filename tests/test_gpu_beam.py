@@ -87,6 +87,32 @@ def test_select_ties(gpu, n_out, V):
     run_select(gpu, -np.sort(rs.standard_normal((1, 2, V)), -1), np.array([[0.0, -1.0]]), None, n_out)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("G,K,V,n_out", [(1, 12, 57576, 24), (1, 4, 151936, 8), (2, 16, 9000, 32), (3, 2, 40000, 64), (1, 64, 20000, 64), (1, 7, 70001, 1)])
+def test_select_many_segments(gpu, dtype, G, K, V, n_out):
+    """Few rows cut into many segments, most of which hold none of the best; finished and dead rows, masked stretches,
+    the best all in one place, equal values."""
+    rs = np.random.default_rng(V + n_out)
+    dt = o.TYPES[dtype]
+    x = rs.standard_normal((G, K, V)) * 2.5
+    s = -3 * rs.random((G, K))
+    done = (rs.random((G, K)) < 0.3).astype(np.int32)
+    run_select(gpu, x, s, None, n_out, dt=dt)
+    run_select(gpu, x, s, done, n_out, eos=V - 1, dt=dt)
+    first = np.where(np.arange(K) == K - 1, s, -np.inf)
+    run_select(gpu, x, first, None, n_out, dt=dt)
+    y = x.copy()
+    y[:, 0, : V - V // 16] = -np.inf
+    y[:, K // 2, V // 9 :] = -np.inf
+    y[:, K - 1, 700:1000] += 40
+    run_select(gpu, y, s, None, n_out, dt=dt)
+    y[0, 0, V // 2] = np.nan
+    y[0, K - 1] = -np.inf
+    run_select(gpu, y, s, done, n_out, dt=dt)
+    run_select(gpu, rs.integers(0, 2, (G, K, V)).astype(np.float64), np.zeros((G, K)), None, n_out, dt=dt)
+    run_select(gpu, np.zeros((G, K, V)), np.zeros((G, K)), done, n_out, dt=dt)
+
+
 def test_select_masked_and_dead(gpu):
     rs = np.random.default_rng(3)
     x = rs.standard_normal((4, 4, 3000))
