@@ -350,7 +350,10 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
             m = qmh_wave_max(m);
             const double ref2 = (double)m * 1.4426950408889634074;
             s = sum0 == 0.0 ? 0.0 : sum0 * exp_sum<1>(&ref0, m - 700.0f, ref2);
-            for (int c = lane + 64; c < segs; c += 64) s = __builtin_fma(h[c].sum, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
+            for (int c = lane + 64; c < segs; c += 64) { // a sum of 0 has no reference to be in range of
+                const double e = h[c].sum;
+                if (e != 0.0) s = __builtin_fma(e, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
+            }
             s = (double)m + log(qmh_wave_sum_d(s));
         }
         if constexpr (MANY) {

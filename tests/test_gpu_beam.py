@@ -113,6 +113,18 @@ def test_select_many_segments(gpu, dtype, G, K, V, n_out):
     run_select(gpu, np.zeros((G, K, V)), np.zeros((G, K)), done, n_out, dt=dt)
 
 
+@pytest.mark.parametrize("level", [-710.0, -709.5, 710.0, -3e38])
+@pytest.mark.parametrize("K,n_out", [(1, 2), (1, 64), (4, 32)])
+def test_select_masked_segments_far_from_zero(gpu, K, n_out, level):
+    """Segments without a logit, before, between and behind, in rows whose values lie far from 0."""
+    rs = np.random.default_rng(int(abs(level)) % 1000)
+    V = 150000
+    x = np.full((1, K, V), -np.inf)
+    for a in (70000, 90000, 149000):
+        x[..., a : a + 800] = level - rs.random((1, K, 800)) * 20
+    run_select(gpu, x, np.zeros((1, K)), None, n_out)
+
+
 def test_select_masked_and_dead(gpu):
     rs = np.random.default_rng(3)
     x = rs.standard_normal((4, 4, 3000))
