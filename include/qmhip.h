@@ -140,14 +140,14 @@ void qmh_rotary_free(qmh_rotary *r);
 
 /* New tokens into a paged cache, in one pass: queries and keys of each head normed (optional) and rotated
  * (optional), keys and values written to the pages, queries to q_out. Rows are of the pages' dtype.
- * Token t < n_tokens belongs to sequence seq[t] (a row of table [n_seq][table_stride]), is its position slot[t]
+ * Token t < n_tokens (at most 2^24) belongs to sequence seq[t] (a row of table [n_seq][table_stride]), is its position slot[t]
  * in the pages, and is rotated by position pos[t] (NULL: slot[t]; they differ where a shared prefix lies before
  * the sequence's own pages). With gains: x_i g_i / sqrt(mean x^2 + eps) over a head, g of head_dim floats.
  * q: row t at q + t * q_stride elements, n_heads heads after one another; q_out alike (q_out = q with the same
  * stride is allowed); both NULL: no queries. k, v: n_kv_heads heads a row; both NULL: queries only, and then
  * pages->k, v, table, seq and (with pos) slot are not looked at. k, v and q may be parts of the same rows.
  * A token whose seq, slot, page or pos is outside its range (slot < table_stride * page_size, pos < the rotary's
- * max_pos) is left out, nothing of it is written: pos or slot -1 pads a batch. No two tokens of a call may name
+ * max_pos; pos at least 0 also without a rotation) is left out, nothing of it is written: pos or slot -1 pads a batch. No two tokens of a call may name
  * the same slot of the same sequence (the slot then holds a mixture of theirs). */
 typedef struct {
     const qmh_pages *pages;

@@ -628,8 +628,8 @@ typedef const __attribute__((address_space(4))) int32_t *const_i32;
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 template <typename U, int BM>
 __global__ __launch_bounds__(256, BM > 16 ? 2 : 4) void k_beam_reorder(const qmh_beam_state s, uint8_t *dst, const uint8_t *src, const int32_t *parent,
-                                                      uint32_t n_groups, int K, uint32_t row_units, uint32_t blocks_per) {
-    const uint32_t og = blockIdx.x / blocks_per, ub = blockIdx.x - og * blocks_per;
+                                                      uint32_t n_groups, int K, uint32_t row_units, uint32_t blocks_per, uint32_t first) {
+    const uint32_t block = blockIdx.x + first, og = block / blocks_per, ub = block - og * blocks_per;
     const uint32_t o = og / n_groups, g = og - o * n_groups;
     const uint32_t u = ub * 256 + threadIdx.x, r = u / row_units, c = u - r * row_units;
     const_i32 par = (const_i32)(uintptr_t)(parent + g * K);
@@ -761,14 +761,18 @@ static int reorder_as(const qmh_beam_state *s, void *dst, const void *src, const
     const int64_t row_units = (s->live + (int64_t)sizeof(U) - 1) / (int64_t)sizeof(U), units = row_units * s->n_rows;
     const int64_t per = (units + 255) / 256, blocks = per * n_groups * s->n_outer;
     if (row_units > 0x7fffffff || units > 0x7fffff00 || blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
-    const dim3 g((uint32_t)blocks), t(256);
+    const dim3 t(256);
     uint8_t *d = (uint8_t *)dst;
     const uint8_t *f = (const uint8_t *)src;
     const uint32_t ru = (uint32_t)row_units, p = (uint32_t)per;
-    if (K <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 4>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
-    else if (K <= 8) hipLaunchKernelGGL((k_beam_reorder<U, 8>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
-    else if (K <= 16) hipLaunchKernelGGL((k_beam_reorder<U, 16>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
-    else if constexpr (sizeof(U) <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 64>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p);
+    for (int64_t b0 = 0; b0 < blocks; b0 += QMH_MOST_BLOCKS) { // blocks move different bytes: any number of launches
+        const dim3 g((uint32_t)(blocks - b0 < QMH_MOST_BLOCKS ? blocks - b0 : QMH_MOST_BLOCKS));
+        const uint32_t b = (uint32_t)b0;
+        if (K <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 4>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p, b);
+        else if (K <= 8) hipLaunchKernelGGL((k_beam_reorder<U, 8>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p, b);
+        else if (K <= 16) hipLaunchKernelGGL((k_beam_reorder<U, 16>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p, b);
+        else if constexpr (sizeof(U) <= 4) hipLaunchKernelGGL((k_beam_reorder<U, 64>), g, t, 0, st, *s, d, f, parent, n_groups, K, ru, p, b);
+    }
     return (int)hipGetLastError();
 }
 

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
     const int hd = s.p.head_dim, KV = s.p.n_kv_heads, H = a.q ? a.n_heads : 0, NH = H + (a.k ? 2 * KV : 0);
     const int half = s.r.pairs, rot = 2 * half;
     const int pos = a.pos ? a.pos[t] : a.slot ? a.slot[t] : 0;
-    if (half && (pos < 0 || pos >= s.r.max_pos)) return;
+    if (pos < 0 || (half && pos >= s.r.max_pos)) return; // padding, rotated or not
     int64_t row0 = 0; // the token's row of its page, for kv head 0
     int ps = 0;
     if (a.k) {
@@ -738,11 +738,11 @@ void launch_attention(const attn_args &s, hipStream_t st) {
 template <typename U, int BM>
 __global__ __launch_bounds__(256) void k_paged_reorder(const qmh_pages p, const int32_t *__restrict__ table, int table_stride,
                                                        const int32_t *__restrict__ len, int max_len,
-                                                       const int32_t *__restrict__ parent, int K, uint32_t n_pi, uint32_t subs, uint32_t row_bytes) {
+                                                       const int32_t *__restrict__ parent, int K, uint32_t n_pi, uint32_t subs, uint32_t row_bytes, uint32_t first) {
     __shared__ int2 from_to[64];
     __shared__ int live[64], count, least;
     // block: ((group * page indexes + page index) * 2 + (k, v)) * subs + piece
-    uint32_t b = blockIdx.x;
+    const uint32_t b = blockIdx.x + first;
     const uint32_t rest = b / subs, sub = b - rest * subs, gp = rest >> 1, g = gp / n_pi, pi = gp - g * n_pi;
     if (threadIdx.x < 64) {
         const int j = threadIdx.x, from = j < K ? parent[g * K + j] : -1;
@@ -862,7 +862,7 @@ extern "C" int qmh_launch_paged_attention(const qmh_attention_args *a, int cus, 
     s.lg_ps = __builtin_ctz(s.p.page_size);
     s.part = (float *)ws;
     s.ml = (float2 *)(s.part + (size_t)(s.n.ps + s.n.os) * s.n.rows * s.p.head_dim);
-    if (s.n.blocks > 0x7fffffff || s.n.rows > 0x7fffffff) return (int)hipErrorInvalidValue;
+    if (s.n.blocks > QMH_MOST_BLOCKS || (s.n.rows + 3) / 4 > QMH_MOST_BLOCKS) return (int)hipErrorInvalidValue;
     qmh_for_type(s.p.dtype, [&](auto z) {
         using T = decltype(z);
         if (s.p.head_dim <= 64) launch_attention<T, 64>(s, (hipStream_t)stream);
@@ -879,13 +879,17 @@ extern "C" int qmh_launch_paged_reorder(const qmh_pages *p, const int32_t *table
     const int64_t page_bytes = (int64_t)p->n_kv_heads * p->page_size * row_bytes;
     const int64_t subs = (page_bytes + 256 * unit - 1) / (256 * unit), blocks = (int64_t)n_groups * n_pi * 2 * subs;
     if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
-    const dim3 g((uint32_t)blocks), t(256);
+    const dim3 t(256);
     hipStream_t st = (hipStream_t)stream;
-    if (n_beams <= 8)
-        hipLaunchKernelGGL((k_paged_reorder<v4u, 8>), g, t, 0, st, *p, table, table_stride, len, max_len, parent, n_beams, n_pi, subs, row_bytes);
-    else if (n_beams <= 16)
-        hipLaunchKernelGGL((k_paged_reorder<v4u, 16>), g, t, 0, st, *p, table, table_stride, len, max_len, parent, n_beams, n_pi, subs, row_bytes);
-    else
-        hipLaunchKernelGGL((k_paged_reorder<uint32_t, 64>), g, t, 0, st, *p, table, table_stride, len, max_len, parent, n_beams, n_pi, subs, row_bytes);
+    for (int64_t b0 = 0; b0 < blocks; b0 += QMH_MOST_BLOCKS) { // blocks move different bytes: any number of launches
+        const dim3 g((uint32_t)(blocks - b0 < QMH_MOST_BLOCKS ? blocks - b0 : QMH_MOST_BLOCKS));
+        const uint32_t b = (uint32_t)b0;
+        if (n_beams <= 8)
+            hipLaunchKernelGGL((k_paged_reorder<v4u, 8>), g, t, 0, st, *p, table, table_stride, len, max_len, parent, n_beams, n_pi, subs, row_bytes, b);
+        else if (n_beams <= 16)
+            hipLaunchKernelGGL((k_paged_reorder<v4u, 16>), g, t, 0, st, *p, table, table_stride, len, max_len, parent, n_beams, n_pi, subs, row_bytes, b);
+        else
+            hipLaunchKernelGGL((k_paged_reorder<uint32_t, 64>), g, t, 0, st, *p, table, table_stride, len, max_len, parent, n_beams, n_pi, subs, row_bytes, b);
+    }
     return (int)hipGetLastError();
 }

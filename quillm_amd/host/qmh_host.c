@@ -354,7 +354,7 @@ int qmh_paged_append(const qmh_append_args *a, void *stream) {
     if (check_pages(a->pages, kv, me)) return -1;
     const qmh_pages *p = a->pages;
     const int es = elem_bytes(p->dtype), hd = p->head_dim;
-    if (a->n_tokens < 0) return fail("%s: n_tokens %d", me, a->n_tokens);
+    if (a->n_tokens < 0 || a->n_tokens > 1 << 24) return fail("%s: n_tokens %d outside [0, 2^24]", me, a->n_tokens);
     if (!a->q && !a->q_out && !kv) return fail("%s: neither queries nor keys and values", me);
     if (a->q || a->q_out) {
         if (a->n_heads < 1 || a->n_heads > 4096) return fail("%s: n_heads %d outside [1, 4096]", me, a->n_heads);
@@ -478,7 +478,9 @@ int qmh_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const 
     if (s->n_outer < 0 || s->n_rows < 0 || s->live < 0 || s->n_outer > 1 << 24 || s->n_rows > 1 << 30 || s->live > (int64_t)1 << 40 ||
         s->outer_stride < 0 || s->seq_stride < 0 || s->row_stride < 0 || s->outer_stride > top || s->seq_stride > top || s->row_stride > top)
         return fail("%s: a size or stride is negative or too large", me);
-    if (s->n_rows > 1 && s->row_stride < s->live) return fail("%s: rows of %lld bytes overlap", me, (long long)s->live);
+    if ((s->n_rows > 1 && s->row_stride < s->live) || ((int64_t)n_groups * n_beams > 1 && s->seq_stride < s->live) ||
+        (s->n_outer > 1 && s->outer_stride < s->live))
+        return fail("%s: pieces of %lld bytes overlap", me, (long long)s->live);
     if (on_device(me)) return -1;
     if (!n_groups || !s->n_outer || !s->n_rows || !s->live) return 0;
     LCHK(qmh_launch_beam_reorder(s, dst, src, parent, n_groups, n_beams, S(stream)));
@@ -489,7 +491,7 @@ int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t tabl
                       int32_t max_len, const int32_t *parent, int32_t n_groups, int32_t n_beams, void *stream) {
     static const char *me = "paged_reorder";
     if (check_pages(pages, 1, me) || check_parents(me, parent, n_groups, n_beams)) return -1;
-    if (max_len < 0) return fail("%s: max_len %d", me, max_len);
+    if (max_len < 0 || max_len > 1 << 30) return fail("%s: max_len %d outside [0, 2^30]", me, max_len);
     if (max_len && (!table || !len || max_len > (int64_t)table_stride * pages->page_size))
         return fail("%s: max_len %d needs len and a table of that many positions", me, max_len);
     if (on_device(me)) return -1;

@@ -208,6 +208,52 @@ def test_beam_reorder(gpu, inplace, beams, outer, rows, row_stride, live, gap, s
             assert np.array_equal(ds.get(), src)
 
 
+def test_beam_reorder_of_more_pieces_than_a_launch(gpu):
+    """2^24 pieces of a byte for each of two groups: more workgroups than one launch may have."""
+    q, outer, groups, beams = gpu, 1 << 24, 2, 2
+    rs = np.random.default_rng(9)
+    src = rs.integers(0, 256, (outer, groups, beams), dtype=np.uint8)
+    ds, dp = q.DeviceBuffer.from_array(src), q.DeviceBuffer.from_array(np.array([1, 1, 1, 0], np.int32))
+    st = q.BeamState(n_outer=outer, outer_stride=4, seq_stride=1, n_rows=1, row_stride=1, live=1)
+    q._check(q.load_library().qmh_beam_reorder(ctypes.byref(st), ds.ptr, ds.ptr, dp.ptr, groups, beams, None), "reorder")
+    q.sync()
+    got = ds.to_array(np.uint8).reshape(src.shape)
+    assert np.array_equal(got[:, 0], src[:, 0, [1, 1]]) and np.array_equal(got[:, 1], src[:, 1, [1, 0]])
+
+
+def test_select_on_two_streams_at_once(gpu):
+    """Two selections of different sizes under way together, each with its own workspace, again and again."""
+    q, L = gpu, gpu.load_library()
+    hip = ctypes.CDLL("libamdhip64.so")
+    hip.hipStreamCreate.argtypes = [ctypes.POINTER(ctypes.c_void_p)]
+    hip.hipStreamSynchronize.argtypes = hip.hipStreamDestroy.argtypes = [ctypes.c_void_p]
+    rs = np.random.default_rng(10)
+    sides = []
+    for G, K, V, n_out in ((2, 5, 60000, 20), (30, 4, 3001, 8)):
+        x, score = rs.standard_normal((G, K, V)).astype(np.float32), -rs.random((G, K)).astype(np.float32)
+        d = dict(x=q.DeviceBuffer.from_array(x), s=q.DeviceBuffer.from_array(score),
+                 out=[q.DeviceBuffer.from_array(np.zeros((G, n_out), t)) for t in (np.float32, np.int32, np.int32)])
+        d["a"] = q.BeamArgs(dtype=o.F32, n_groups=G, n_beams=K, vocab=V, n_out=n_out, eos=0, logits=d["x"].ptr, stride=V, score=d["s"].ptr,
+                            out_score=d["out"][0].ptr, out_parent=d["out"][1].ptr, out_token=d["out"][2].ptr)
+        d["need"] = L.qmh_beam_select_ws(ctypes.byref(d["a"]))
+        d["ws"] = q.DeviceBuffer.from_array(np.full(d["need"], 0xFF, np.uint8))
+        d["want"] = [best_of(x[g].astype(np.float64), score[g].astype(np.float64), None, n_out, 0) for g in range(G)]
+        d["stream"] = ctypes.c_void_p()
+        assert hip.hipStreamCreate(ctypes.byref(d["stream"])) == 0
+        sides.append(d)
+    q.sync()
+    try:
+        for _ in range(20):
+            for d in sides:
+                assert L.qmh_beam_select(ctypes.byref(d["a"]), d["ws"].ptr, d["need"], d["stream"]) == 0
+        for d in sides:
+            assert hip.hipStreamSynchronize(d["stream"]) == 0
+            assert [w[1:] for g in d["want"] for w in g] == list(zip(d["out"][1].to_array(np.int32).ravel().tolist(), d["out"][2].to_array(np.int32).ravel().tolist()))
+    finally:
+        for d in sides:
+            hip.hipStreamDestroy(d["stream"])
+
+
 def test_select_more_rows_than_a_grid_dimension(gpu):
     """80000 rows: the rows pass one launch's limit."""
     q, G, K, V = gpu, 40000, 2, 9

@@ -155,6 +155,12 @@ def test_append_leaves_out_what_is_out_of_range(gpu):
     run_append(gpu, o.F16, 4, 2, 64, 16, 80, "halves", gains=True, seqs=4, seed=9, max_pos=2048, drop=bad)
 
 
+@pytest.mark.parametrize("use_kv", [True, False])
+def test_append_pads_without_a_rotation(gpu, use_kv):
+    """A negative position marks padding whether or not it is used to rotate."""
+    run_append(gpu, o.F16, 4, 2, 64, 16, 40, rot=0, gains=True, seqs=2, seed=12, use_kv=use_kv, drop=[("pos", -1), ("pos", -2 ** 31)])
+
+
 # ------------------------------------------------------------------------------------- attention
 
 def run_attention(q, dt, H, KV, hd, ps, groups, per, q_len, prefix, own, seed=0, scale=None, pad=0, values=None, keys=None,
@@ -291,6 +297,12 @@ def test_attention_large_and_lowest_scores(gpu, dtype):
     # keys of the type's lowest value, at scale 0: equal scores, or NaN where the products pass 32 bits
     run_attention(gpu, o.TYPES[dtype], 2, 1, 64, 16, 1, 1, 1, [0], [40], keys=lambda k: np.where(np.arange(64) == 0, -big, 0 * k), scale=0.0,
                   seed=5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attention_negative_scale(gpu, dtype):
+    run_attention(gpu, o.TYPES[dtype], 4, 2, 64, 16, 2, 2, 3, [70, 0], [3, 17, 40, 600], scale=-0.125, seed=14)
+    run_attention(gpu, o.TYPES[dtype], 2, 2, 128, 32, 1, 3, 1, [1500], [1, 0, 33], scale=-0.5, seed=15)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

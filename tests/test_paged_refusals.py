@@ -99,6 +99,19 @@ def test_reorder(qmh, kw):
     refused(qmh, qmh.load_library().qmh_beam_reorder(ctypes.byref(s), P, P, P, 2, 4, None), "beam_reorder")
 
 
+@pytest.mark.parametrize("kw", [dict(seq_stride=63), dict(outer_stride=63)])
+def test_reorder_overlapping_states(qmh, kw):
+    d = dict(n_outer=2, outer_stride=1 << 16, seq_stride=1 << 12, n_rows=1, row_stride=128, live=64)
+    d.update(kw)
+    refused(qmh, qmh.load_library().qmh_beam_reorder(ctypes.byref(qmh.BeamState(**d)), P, P, P, 1, 4, None), "beam_reorder")
+
+
+def test_most_tokens_and_positions(qmh):
+    refused(qmh, append(qmh, n_tokens=(1 << 24) + 1), "paged_append")
+    p = pages(qmh)
+    refused(qmh, qmh.load_library().qmh_paged_reorder(ctypes.byref(p), P, 1 << 27, P, (1 << 30) + 1, P, 2, 2, None), "paged_reorder")
+
+
 def test_reorder_arguments(qmh):
     L = qmh.load_library()
     s = qmh.BeamState(n_outer=1, outer_stride=0, seq_stride=64, n_rows=1, row_stride=64, live=64)
