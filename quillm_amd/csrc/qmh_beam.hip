@@ -13,9 +13,8 @@ namespace {
 
 constexpr int SEL_T = 256;    // threads of the scan
 constexpr int SEL_CAP = 256;  // candidates a wave of it lists
-constexpr int JOIN_T = 512;   // threads of the join
 constexpr int JOIN_CAP = 1024;
-constexpr int SCAN_WAVES = 3072, SCAN_EPT = 16; // of plan_scan
+constexpr int SCAN_WAVES = 3 * 1024, SCAN_EPT = 16; // of plan_scan
 
 // The sum of e^(x - ref) over N floats, in 64 bits, x at most 600 above ref (finite): x log2 e - ref log2 e = k + f,
 // |f| <= 1/2, and 2^k times a polynomial of degree 8 that meets 2^f at the nine Chebyshev points, at most 1.1e-12 of the
@@ -301,24 +300,27 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
 }
 
 // A group's choice from its rows' segments: each row's log sum (a wave a row), then the n_out best totals as in the scan:
-// a bound from the lanes' best, what reaches it ranked in LDS. Where more than JOIN_CAP reach it, one after another. A
-// chain of short steps in one workgroup: 5 to 7 us, 4 of them an empty launch's.
+// a bound, what reaches it ranked in LDS. The bound is the n_out-th largest of 64 parts' maxima, a part being one lane of
+// every wave; from 64 parts it lets about 64 (1 + 1/2 + ... + 1/64) pass at the most on average, however many candidates there are, as
+// long as their best are spread over the parts. Where more than JOIN_CAP reach it (equal totals), one after another. A
+// chain of short steps in one workgroup: 5 to 7 us, 4 of them an empty launch's; past 8 beams twice the threads (12 rows of
+// 8000 13.2 us with 1024, 14.7 with 512).
 // MANY: a segment whose largest total is below the n_out-th largest of these has none of the best. The others are found
-// first (a bound from each row's, then one from what that leaves), and only their candidates are read.
-template <bool MANY>
-__global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int segs) {
-    constexpr int NW = JOIN_T / 64, TOPS = MANY ? SCAN_WAVES : 1;
+// first, by the same bound, and only their candidates are read.
+template <bool MANY, int JT>
+__global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int segs) {
+    constexpr int NW = JT / 64, TOPS = MANY ? SCAN_WAVES : 1;
     __shared__ double lse[64], score[64];
     __shared__ uint64_t ckey[JOIN_CAP], bk[NW];
-    __shared__ uint32_t cplace[JOIN_CAP], bounds[NW], bf[NW];
-    __shared__ uint32_t tops[TOPS], list_key[TOPS];
-    __shared__ uint16_t list[TOPS], chosen[TOPS];
-    __shared__ int ncand, nlist, nchosen;
+    __shared__ uint32_t cplace[JOIN_CAP], best_of[JT], bf[NW], tops[TOPS];
+    __shared__ uint16_t chosen[TOPS];
+    __shared__ int ncand, nchosen;
     const int g = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63, K = a.n_beams, n_out = a.n_out;
-    if (tid == 0) ncand = nlist = nchosen = 0;
+    if (tid == 0) ncand = nchosen = 0;
     // few beams: several waves a row, each with the row's log sum for itself (MANY: a wave a row)
     const int share = !MANY && K < NW ? NW / K : 1, per = segs * n_out;
-    const int b0 = w / share < NW / share ? w / share : K, j0 = (w % share) * 64 + lane;
+    const int b0 = w / share < NW / share ? w / share : K, j0 = (w % share) * 64;
+    auto number = [&](int k) { return j0 + 64 * share * k + ((lane + 21 * k + 9 * w) & 63); }; // of a row's candidates: every part gets some of a segment's first
     auto behind = [&](uint64_t all) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0)); };
     // the first row's first heads and candidates are asked for at once with its score (of a dead row they are not used)
     double sum0 = 0.0;
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
             ref0 = heads[at + lane].ref;
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) v0[k] = j0 + 64 * share * k < per ? cands[at * n_out + j0 + 64 * share * k] : make_uint2(0, 0);
+        for (int k = 0; k < 4; k++) v0[k] = number(k) < per ? cands[at * n_out + number(k)] : make_uint2(0, 0);
     }
     uint32_t mine = 0;
     for (int b = b0; b < K; b += NW / share) {
@@ -386,59 +388,44 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
                 }
                 s = (double)m + log(qmh_wave_sum_d(s));
             }
-            uint32_t best = 0; // the tops become the high words of their totals' ordered keys
+            // the tops become the high words of their totals' ordered keys
             for (int c = lane; c < segs; c += 64) {
                 const uint32_t t = live && s == s ? top[c] : 0;
                 const uint32_t q = done && c == 0 ? (uint32_t)(key_of_d(sc) >> 32)
                                    : t            ? (uint32_t)(key_of_d((double)sc + ((double)of_key(t) - s)) >> 32)
                                                   : 0;
                 top[c] = q;
-                best = q > best ? q : best;
             }
-            const uint32_t t = wave_nth<12>(best, n_out);
-            mine = t > mine ? t : mine;
         }
         if (lane == 0 && w % share == 0) {
             lse[b] = done ? __builtin_inf() : s; // marks a finished row
             score[b] = (double)sc;
         }
     }
-    auto highest = [&](uint32_t at_least) { // of the waves' bounds
+    // What the n_out-th largest is not below, from each thread's largest: the n_out-th largest of 64 parts' (one lane of
+    // every wave). All threads take part.
+    auto bound = [&]() {
+        best_of[tid] = mine;
+        __syncthreads();
+        uint32_t v = 0;
 #pragma unroll
-        for (int k = 0; k < NW; k++) at_least = bounds[k] > at_least ? bounds[k] : at_least;
-        return at_least;
+        for (int k = 0; k < NW; k++) v = best_of[64 * k + lane] > v ? best_of[64 * k + lane] : v;
+        v = wave_nth<12>(v, n_out);
+        return v > 1 ? v : 1;
     };
     const int lanes = n_out <= 1 ? 1 : 1 << (32 - __builtin_clz(n_out - 1)); // of a chosen segment: a power of two
     if constexpr (MANY) {
-        if (lane == 0) bounds[w] = mine;
         __syncthreads();
-        uint32_t from = highest(1);
-        for (int c0 = 0; c0 < K * segs; c0 += JOIN_T) {
+        for (int c = tid; c < K * segs; c += JT) mine = tops[c] > mine ? tops[c] : mine;
+        const uint32_t from = bound();
+        for (int c0 = 0; c0 < K * segs; c0 += JT) {
             const int c = c0 + tid;
-            const uint32_t q = c < K * segs ? tops[c] : 0;
-            const uint64_t in = __ballot(q >= from);
-            int at = 0;
-            if (lane == 0 && in) at = atomicAdd(&nlist, __popcll(in));
-            at = __builtin_amdgcn_readfirstlane(at) + behind(in);
-            if (q >= from) {
-                list_key[at] = q;
-                list[at] = (uint16_t)c;
-            }
-        }
-        __syncthreads();
-        const int n = nlist;
-        uint32_t best = 0;
-        for (int i = lane; i < n; i += 64) best = list_key[i] > best ? list_key[i] : best;
-        const uint32_t t = wave_nth<12>(best, n_out);
-        from = t > from ? t : from;
-        for (int i0 = 0; i0 < n; i0 += JOIN_T) {
-            const int i = i0 + tid;
-            const bool take = i < n && list_key[i] >= from;
+            const bool take = c < K * segs && tops[c] >= from;
             const uint64_t in = __ballot(take);
             int at = 0;
             if (lane == 0 && in) at = atomicAdd(&nchosen, __popcll(in));
             at = __builtin_amdgcn_readfirstlane(at) + behind(in);
-            if (take) chosen[at] = list[i];
+            if (take) chosen[at] = (uint16_t)c;
         }
     }
     __syncthreads();
@@ -447,7 +434,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     auto of_chosen = [&](int i, uint64_t *q, uint32_t *p) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int e = i + ((k * NW + w) * 64 + lane) / lanes, o = lane & (lanes - 1);
+            const int e = i + ((k * NW + w) * 64 + lane) / lanes, o = (lane + 5 * e) & (lanes - 1); // every part gets some of the first
             q[k] = 0;
             if (e < n_chosen && o < n_out) {
                 const int c = chosen[e];
@@ -467,7 +454,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     auto each = [&](auto body) {
         if constexpr (MANY) {
             body(q0, p0);
-            for (int i = 4 * JOIN_T / lanes; i < n_chosen; i += 4 * JOIN_T / lanes) {
+            for (int i = 4 * JT / lanes; i < n_chosen; i += 4 * JT / lanes) {
                 uint64_t q[4];
                 uint32_t p[4] = {};
                 of_chosen(i, q, p);
@@ -489,7 +476,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
                 for (int i = 0; i < per; i += 256 * share) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const int j = i + j0 + 64 * share * k;
+                        const int j = i + number(k);
                         const uint2 v = b == b0 && i == 0 ? v0[k] : j < per ? c[j] : make_uint2(0, 0);
                         q[k] = v.x ? key_of_d(sc + ((double)of_key(v.x) - L)) : 0ull;
                         p[k] = (uint32_t)(b * a.vocab) + v.y;
@@ -504,10 +491,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
 #pragma unroll
         for (int k = 0; k < 4; k++) mine = (uint32_t)(q[k] >> 32) > mine ? (uint32_t)(q[k] >> 32) : mine;
     });
-    const uint32_t bw = wave_nth<12>(mine, n_out);
-    if (lane == 0) bounds[w] = bw;
-    __syncthreads();
-    const uint32_t from = highest(1);
+    const uint32_t from = bound();
     each([&](const uint64_t *q, const uint32_t *p) { // places by ballots, one addition to the count a wave
         uint64_t in[4];
         int n = 0;
@@ -540,7 +524,7 @@ __global__ __launch_bounds__(JOIN_T) void k_beam_join(const qmh_beam_args a, con
     const int n = ncand;
     if (n <= JOIN_CAP) { // every score has been read: out_score may be score
         rank_all(
-            n, JOIN_T, [&](int i, int c) { return (ckey[i] > ckey[c]) | ((ckey[i] == ckey[c]) & (cplace[i] < cplace[c])); }, // no branches: the reads overlap
+            n, JT, [&](int i, int c) { return (ckey[i] > ckey[c]) | ((ckey[i] == ckey[c]) & (cplace[i] < cplace[c])); }, // no branches: the reads overlap
             [&](int c, int r) {
                 if (r < n_out) write(r, ckey[c], cplace[c]);
             });
@@ -610,13 +594,10 @@ scan_plan plan_scan(const qmh_beam_args *a) {
     p.segs = (int)((pieces + (int64_t)p.iters * W - 1) / ((int64_t)p.iters * W)) * W;
     return p;
 }
-// Which join: with more than 8 candidates of a row a lane, most of them not worth reading. 12 rows of 57576, n_out 24 (116
-// segments a row): 18.6 us with it, 64 without; 4 rows of 151936, n_out 8 (300): 14.9 and 25; 4 rows of 32000, n_out 8
-// (64): 12.1 and 10.9; 40 rows of 3488, n_out 6 (8): 13.7 and 10.9.
-bool many_segments(const qmh_beam_args *a, int segs) {
-    const int share = a->n_beams < JOIN_T / 64 ? JOIN_T / 64 / a->n_beams : 1;
-    return segs * a->n_out > 512 * share;
-}
+// Which join: MANY where most of a row's candidates are not worth reading. One prompt, 12 rows of 57576, n_out 24 (116 segments a
+// row): 15.2 us with it, 39 without; 4 rows of 151936, n_out 8 (300): 13.7 and 24; 64 rows of 32000, n_out 16 (32): 14.4 and 15.9;
+// 192 rows of 128256, n_out 16 (16): 41.2 and 40.3; 16 rows of 3000, n_out 64 (8): 45 and 33.
+bool many_segments(const qmh_beam_args *a, int segs) { return segs >= 32 && segs * a->n_out > 256; }
 
 // --------------------------------------------------------------------------- reorder
 
@@ -750,8 +731,15 @@ extern "C" int qmh_launch_beam_select(const qmh_beam_args *a, void *ws, void *st
             else hipLaunchKernelGGL((k_beam_scan<T, SCAN_EPT, VEC>), g, dim3(SEL_T), 0, st, *a, heads, cands, r0, p.iters);
         }
     });
-    if (many_segments(a, p.segs)) hipLaunchKernelGGL(k_beam_join<true>, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);
-    else hipLaunchKernelGGL(k_beam_join<false>, dim3(a->n_groups), dim3(JOIN_T), 0, st, *a, heads, cands, p.segs);
+    const bool many = many_segments(a, p.segs);
+    const dim3 g(a->n_groups);
+    if (a->n_beams <= 8) {
+        if (many) hipLaunchKernelGGL((k_beam_join<true, 512>), g, dim3(512), 0, st, *a, heads, cands, p.segs);
+        else hipLaunchKernelGGL((k_beam_join<false, 512>), g, dim3(512), 0, st, *a, heads, cands, p.segs);
+    } else {
+        if (many) hipLaunchKernelGGL((k_beam_join<true, 1024>), g, dim3(1024), 0, st, *a, heads, cands, p.segs);
+        else hipLaunchKernelGGL((k_beam_join<false, 1024>), g, dim3(1024), 0, st, *a, heads, cands, p.segs);
+    }
     return (int)hipGetLastError();
 }
 
