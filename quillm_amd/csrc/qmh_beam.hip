@@ -144,9 +144,15 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
     float bound = -__builtin_inff(); // logits above it are candidates
     bool bad = false, none = true;
     int n = 0; // candidates in the list
-    auto before = [](uint2 u, uint2 v) { return u.x > v.x || (u.x == v.x && u.y < v.y); };
     auto place = [&](uint64_t all) { return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0)); };
-    // the list's n_out best, in any order
+    // the largest index that leaves fewer than n_out, and then the next one
+    auto lowest = [&](auto count) {
+        int last = -1;
+        for (int b = 24; b >= 0; b--) last = count(last + (1 << b)) < n_out ? last + (1 << b) : last;
+        return last + 1;
+    };
+    // the list's n_out best, in any order: the n_out-th largest key by ballots, the lowest indexes among those equal to it
+    // (by ballots too where it is long: every entry's rank among 250 is a chain of 12 us, this one of 2)
     auto cut = [&]() {
         constexpr int E = SEL_CAP / 64;
         wave_sync();
@@ -158,26 +164,29 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
                 e[j] = lane + 64 * j < n ? list[lane + 64 * j] : make_uint2(0, 0);
                 best = e[j].x > best ? e[j].x : best;
             }
-            const uint32_t t = wave_nth<12>(best, n_out);
+            const uint32_t u = wave_nth<12>(best, n_out);
             wave_sync();
             n = 0;
 #pragma unroll
             for (int j = 0; j < E; j++) {
-                const uint64_t all = __ballot(e[j].x >= t && e[j].x);
-                if (e[j].x >= t && e[j].x) list[n + place(all)] = e[j];
+                const uint64_t all = __ballot(e[j].x >= u && e[j].x);
+                if (e[j].x >= u && e[j].x) list[n + place(all)] = e[j];
                 n += __popcll(all);
             }
             wave_sync();
         }
         if (n < n_out) return;
-        uint32_t t;
+        uint32_t t = 0; // stays above 0: n entries have keys
         if (n <= 64) {
             const uint2 e = lane < n ? list[lane] : make_uint2(0, 0);
             t = wave_nth(e.x, n_out);
-            bool keep = e.x >= t; // t is not 0: n entries have keys
-            if (__popcll(__ballot(keep)) > n_out) { // equal values
+            bool keep = e.x >= t;
+            if (__popcll(__ballot(keep)) > n_out) {
                 int r = 0;
-                for (int i = 0; i < n; i++) r += before(list[i], e);
+                for (int i = 0; i < n; i++) {
+                    const uint2 u = list[i];
+                    r += (u.x > e.x) | ((u.x == e.x) & (u.y < e.y));
+                }
                 keep = lane < n && r < n_out;
             }
             const uint64_t all = __ballot(keep);
@@ -185,20 +194,31 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
             if (keep) list[place(all)] = e;
         } else {
             uint2 e[E];
-            int r[E] = {};
 #pragma unroll
-            for (int j = 0; j < E; j++) e[j] = list[lane + 64 * j];
-            for (int i = 0; i < n; i++) {
-                const uint2 u = list[i];
+            for (int j = 0; j < E; j++) e[j] = lane + 64 * j < n ? list[lane + 64 * j] : make_uint2(0, 0);
+            auto count = [&](auto in) {
+                int c = 0;
 #pragma unroll
-                for (int j = 0; j < E; j++) r[j] += before(u, e[j]);
+                for (int j = 0; j < E; j++) c += __popcll(__ballot(in(e[j])));
+                return c;
+            };
+            for (int b = 31; b >= 0; b--) {
+                const uint32_t u = t | 1u << b;
+                t = count([&](uint2 v) { return v.x >= u; }) >= n_out ? u : t;
             }
+            int last = 0x7fffffff;
+            if (count([&](uint2 v) { return v.x >= t; }) > n_out) last = lowest([&](int i) {
+                return count([&](uint2 v) { return (v.x > t) | ((v.x == t) & ((int)v.y <= i)); });
+            });
             wave_sync();
+            n = 0;
 #pragma unroll
-            for (int j = 0; j < E; j++)
-                if (lane + 64 * j < n && r[j] < n_out) list[r[j]] = e[j];
-            wave_sync();
-            t = __builtin_amdgcn_readfirstlane(list[n_out - 1].x);
+            for (int j = 0; j < E; j++) {
+                const bool keep = (e[j].x > t) | ((e[j].x == t) & ((int)e[j].y <= last));
+                const uint64_t all = __ballot(keep);
+                if (keep) list[n + place(all)] = e[j];
+                n += __popcll(all);
+            }
         }
         wave_sync();
         n = n_out;
@@ -270,26 +290,26 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
             for (int k = 0; k < EPT; k++) append(k, xs[k] > bound);
         } else {
             // the largest key that n_out of the piece's reach, then the lowest indexes among those equal to it
+            uint32_t keys[EPT];
+#pragma unroll
+            for (int k = 0; k < EPT; k++) keys[k] = key_of(xs[k]);
+            auto count = [&](auto in) {
+                int c = 0;
+#pragma unroll
+                for (int k = 0; k < EPT; k++) c += __popcll(__ballot(in(k)));
+                return c;
+            };
             uint32_t from = 0;
             for (int b = 31; b >= 0; b--) {
                 const uint32_t t = from | 1u << b;
-                int c = 0;
-#pragma unroll
-                for (int k = 0; k < EPT; k++) c += __popcll(__ballot(key_of(xs[k]) >= t));
-                if (c >= n_out) from = t;
+                from = count([&](int k) { return keys[k] >= t; }) >= n_out ? t : from;
             }
-            const float exact = of_key(from);
-            int last = -1; // the largest index that leaves fewer than n_out, and then the next one
-            for (int b = 24; b >= 0; b--) {
-                const int t = last + (1 << b);
-                int c = 0;
+            int last = 0x7fffffff;
+            if (count([&](int k) { return keys[k] >= from; }) > n_out) last = lowest([&](int i) {
+                return count([&](int k) { return (keys[k] > from) | ((keys[k] == from) & (index(k) <= i)); });
+            });
 #pragma unroll
-                for (int k = 0; k < EPT; k++) c += __popcll(__ballot(xs[k] > exact || (xs[k] == exact && index(k) <= t)));
-                if (c < n_out) last = t;
-            }
-            last++;
-#pragma unroll
-            for (int k = 0; k < EPT; k++) append(k, xs[k] > exact || (xs[k] == exact && index(k) <= last));
+            for (int k = 0; k < EPT; k++) append(k, keys[k] && ((keys[k] > from) | ((keys[k] == from) & (index(k) <= last))));
         }
         if (n > SEL_CAP / 2) cut();
     }
@@ -596,8 +616,8 @@ scan_plan plan_scan(const qmh_beam_args *a) {
 }
 // Which join: MANY where most of a row's candidates are not worth reading. One prompt, 12 rows of 57576, n_out 24 (116 segments a
 // row): 15.2 us with it, 39 without; 4 rows of 151936, n_out 8 (300): 13.7 and 24; 64 rows of 32000, n_out 16 (32): 14.4 and 15.9;
-// 192 rows of 128256, n_out 16 (16): 41.2 and 40.3; 16 rows of 3000, n_out 64 (8): 45 and 33.
-bool many_segments(const qmh_beam_args *a, int segs) { return segs >= 32 && segs * a->n_out > 256; }
+// 128 rows of 50000, n_out 32 (20): 30.5 and 39.4; 192 of 128256, n_out 16 (16): 41.2 and 40.3; 16 rows of 3000, n_out 64 (8): 42 and 30.
+bool many_segments(const qmh_beam_args *a, int segs) { return segs >= 16 && segs * a->n_out > 256; }
 
 // --------------------------------------------------------------------------- reorder
 
