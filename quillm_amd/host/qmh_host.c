@@ -482,7 +482,7 @@ int qmh_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const 
         (s->n_outer > 1 && s->outer_stride < s->live))
         return fail("%s: pieces of %lld bytes overlap", me, (long long)s->live);
     if (on_device(me)) return -1;
-    if (!n_groups || !s->n_outer || !s->n_rows || !s->live) return 0;
+    if (!n_groups || !s->n_outer || !s->n_rows || !s->live || (n_beams == 1 && dst == src)) return 0; /* one beam has only itself to take */
     LCHK(qmh_launch_beam_reorder(s, dst, src, parent, n_groups, n_beams, S(stream)));
     return 0;
 }
@@ -495,7 +495,7 @@ int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t tabl
     if (max_len && (!table || !len || max_len > (int64_t)table_stride * pages->page_size))
         return fail("%s: max_len %d needs len and a table of that many positions", me, max_len);
     if (on_device(me)) return -1;
-    if (!n_groups || !max_len) return 0;
+    if (!n_groups || !max_len || n_beams == 1) return 0; /* one beam has only itself to take */
     LCHK(qmh_launch_paged_reorder(pages, table, table_stride, len, max_len, parent, n_groups, n_beams, S(stream)));
     return 0;
 }
