@@ -110,3 +110,17 @@ def test_batch_beam_refusals(gpu, small_models):
         for args in ((None, 3, 4), (par.ctypes.data, 4, 4), (par.ctypes.data, 3, -1), (par.ctypes.data, 3, m.cfg.max_seq + 1)):
             assert L.qmh_batch_reorder(b._h, *args) == -1 and "batch_reorder" in gpu.last_error()
         assert L.qmh_batch_reorder(None, par.ctypes.data, 3, 4) == -1 and L.qmh_batch_beam(None, 3, t.ctypes.data, p.ctypes.data, 1, -1, None, None, None) == -1
+
+
+def test_batch_beam_again_and_with_other_group_sizes(gpu, small_models):
+    """One batch used for searches of every group size and other calls in between gives what fresh ones give."""
+    path = small_models[("gqa", "q4_0")]
+    with gpu.Model.load(path) as m, gpu.Batch(m, 6) as a:
+        for n_beams, steps in ((6, 9), (3, 12), (1, 5), (2, 7), (6, 9)):
+            groups = 6 // n_beams
+            tok, pos = list(range(2, 2 + groups)), [0] * groups
+            got = a.beam(tok, pos, n_beams, steps, 1)
+            a.greedy([7] * 6, [0] * 6, 4)
+            with gpu.Batch(m, 6) as b:
+                want = b.beam(tok, pos, n_beams, steps, 1)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(bits(got[1]), bits(want[1])), n_beams
