@@ -635,17 +635,13 @@ __global__ __launch_bounds__(256) void k_attention_join(const attn_args s, int p
     v4f o = {0.f, 0.f, 0.f, 0.f};
     const float *part = s.part + (int64_t)row * hd + (d < hd ? d : 0);
     const int64_t step = s.n.rows * hd;
-    int k = lane / D4;
-    for (; k + 3 * PG < parts; k += 4 * PG) {
+    for (int r = 0; r < parts; r += 4 * PG) { // by all lanes together: each one's weight is asked for by others
+        const int k0 = r + lane / D4;
         v4f v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = *(const v4f *)(part + (k + j * PG) * step);
+        for (int j = 0; j < 4; j++) v[j] = k0 + j * PG < parts ? *(const v4f *)(part + (k0 + j * PG) * step) : (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 4; j++) o += v[j] * __shfl(f, k + j * PG);
-    }
-    for (int j = 0; j < 4; j++, k += PG) { // __shfl by all lanes
-        const float fk = __shfl(f, k & 63);
-        if (k < parts) o += *(const v4f *)(part + k * step) * fk;
+        for (int j = 0; j < 4; j++) o += v[j] * __shfl(f, (k0 + j * PG) & 63);
     }
 #pragma unroll
     for (int x = D4; x < 64; x <<= 1)
