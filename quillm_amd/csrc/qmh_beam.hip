@@ -639,22 +639,22 @@ __global__ __launch_bounds__(256, BM > 16 ? 2 : 4) void k_beam_reorder(const qmh
         if (r >= s.n_rows) return;
         const int64_t at = (int64_t)c * sizeof(U), base = o * s.outer_stride + (int64_t)g * K * s.seq_stride + r * s.row_stride + at;
         auto source = [&](int j) { return par[j] >= 0 && par[j] < K ? par[j] : j; };
-        auto move = [&](auto z, U *slot, int64_t b) {
+        auto move = [&](auto z, int64_t b) { // a byte has the thread's word to itself, too
             using V = decltype(z);
             qmh_move_many(
-                (V *)slot, K,
-                [&](int j, V &u) {
+                keep + threadIdx.x, K,
+                [&](int j, U &u) {
                     if (source(j) == j && dst == src) return false;
                     u = *(const V *)(src + b + source(j) * s.seq_stride);
                     return true;
                 },
-                [&](int j, V u) {
-                    if (source(j) != j || dst != src) *(V *)(dst + b + j * s.seq_stride) = u;
+                [&](int j, U u) {
+                    if (source(j) != j || dst != src) *(V *)(dst + b + j * s.seq_stride) = (V)u;
                 });
         };
-        if (at + (int64_t)sizeof(U) <= s.live) move(U{}, keep + threadIdx.x, base);
+        if (at + (int64_t)sizeof(U) <= s.live) move(U{}, base);
         else
-            for (int64_t k = 0; at + k < s.live; k++) move(uint8_t{}, (U *)((uint8_t *)keep + threadIdx.x), base + k);
+            for (int64_t k = 0; at + k < s.live; k++) move(uint8_t{}, base + k);
         return;
     }
     int from[BM]; // -1: nothing to do
