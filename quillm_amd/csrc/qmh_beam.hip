@@ -16,17 +16,14 @@ constexpr int SEL_CAP = 256;  // candidates a wave of it lists
 constexpr int JOIN_CAP = 1024;
 constexpr int SCAN_WAVES = 3 * 1024, SCAN_EPT = 16; // of plan_scan
 
-// The sum of e^(x - ref) over N floats, in 64 bits, x at most 600 above ref (finite): x log2 e - ref log2 e = k + f,
-// |f| <= 1/2, and 2^k times a polynomial of degree 8 that meets 2^f at the nine Chebyshev points, at most 1.1e-12 of the
-// value from it: far inside the distance of scores that decide a choice. Adding 1.5 2^52
-// rounds to k and leaves it in the low word. Values below low = ref - 700 count as that. The N chains run side by side.
+// The sum of 2^t over N numbers between -1022 and 1022: t = k + f, |f| <= 1/2, and 2^k times a polynomial of degree 8 that
+// meets 2^f at the nine Chebyshev points, at most 1.1e-12 of the value from it: far inside the distance of scores that
+// decide a choice. Adding 1.5 2^52 rounds to k and leaves it in the low word. The N chains run side by side.
 template <int N>
-__device__ __forceinline__ double exp_sum(const float *x, float low, double ref2) {
+__device__ __forceinline__ double exp2_sum(double (&t)[N]) {
     constexpr double c[8] = {1.531007940249083e-05, 0.00015403455852408237, 0.0013333450567999663, 0.009618129159402626,
                              0.05550410941205934, 0.2402265069581299, 0.6931471805459335, 1.0};
-    double t[N], s[N], p[N];
-#pragma unroll
-    for (int j = 0; j < N; j++) t[j] = __builtin_fma((double)fmaxf(x[j], low), 1.4426950408889634074, -ref2);
+    double s[N], p[N];
 #pragma unroll
     for (int j = 0; j < N; j++) s[j] = t[j] + 0x1.8p52;
 #pragma unroll
@@ -44,6 +41,26 @@ __device__ __forceinline__ double exp_sum(const float *x, float low, double ref2
 #pragma unroll
         for (int j = 0; j < n / 2; j++) p[j] += p[j + n / 2];
     return p[0];
+}
+constexpr double LOG2E = 1.4426950408889634074;
+
+// e^d, d <= 600, and e^-700 below -700
+__device__ __forceinline__ double exp_of(double d) {
+    double t[1] = {fmax(d, -700.0) * LOG2E};
+    return exp2_sum<1>(t);
+}
+
+// The sum of e^(x - ref) over N floats, in 64 bits, x at most 600 above ref (finite); values more than 700 below it count as that.
+// NEAR is for |ref| up to 2^14: one fused product, with ref2 = ref log2 e rounded (2^-38 at the most) and a limit in floats,
+// low = ref - 700. Further out these two no longer fit (x = ref would not give 1, low not be 700 away), so the difference is taken first: two
+// 64-bit instructions more a logit.
+constexpr float NEAR_REF = 16384.0f;
+template <bool NEAR, int N>
+__device__ __forceinline__ double exp_sum(const float *x, float ref, float low, double ref2) {
+    double t[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) t[j] = NEAR ? __builtin_fma((double)fmaxf(x[j], low), LOG2E, -ref2) : fmax((double)x[j] - (double)ref, -700.0) * LOG2E;
+    return exp2_sum<N>(t);
 }
 
 // the order of floats as unsigned numbers, -0 as 0; 0 for -inf and NaN, which are no continuations
@@ -139,8 +156,9 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
     };
     load(base);
     float xs[EPT];
-    float max = -__builtin_inff(), ref = 0.0f; // the segment's maximum; what its exponentials are taken below
+    float max = -__builtin_inff(), ref = 0.0f, low = -700.0f; // the segment's maximum; what its exponentials are taken below
     double sum = 0.0, ref2 = 0.0;
+    bool near = true;
     float bound = -__builtin_inff(); // logits above it are candidates
     bool bad = false, none = true;
     int n = 0; // candidates in the list
@@ -240,15 +258,22 @@ __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan
         if (__any(top > max)) {
             // a new maximum: the sums stay in range as long as it is within 600 of the reference
             max = fmaxf(max, qmh_wave_max(top));
-            if (max < __builtin_inff() && (none || max > ref + 600.0f)) {
-                sum *= none ? 0.0 : exp_sum<1>(&ref, max - 700.0f, (double)max * 1.4426950408889634074);
+            if (max < __builtin_inff() && (none || (double)max > (double)ref + 600.0)) {
+                sum *= none ? 0.0 : exp_of((double)ref - (double)max);
                 ref = max;
-                ref2 = (double)ref * 1.4426950408889634074;
+                low = ref - 700.0f;
+                ref2 = (double)ref * LOG2E;
+                near = !__any(__builtin_fabsf(ref) > NEAR_REF);
                 none = false;
             }
         }
+        if (near) {
 #pragma unroll
-        for (int k = 0; k < EPT; k += 4) sum += exp_sum<4>(xs + k, ref - 700.0f, ref2);
+            for (int k = 0; k < EPT; k += 4) sum += exp_sum<true, 4>(xs + k, ref, low, ref2);
+        } else {
+#pragma unroll
+            for (int k = 0; k < EPT; k += 4) sum += exp_sum<false, 4>(xs + k, ref, low, ref2);
+        }
         // the largest float below the n_out-th largest of the lanes' maxima, if that is more than the bound
         auto raise = [&]() {
             uint32_t mine = 0;
@@ -370,11 +395,10 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
             float m = sum0 == 0.0 ? -__builtin_inff() : ref0;
             for (int c = lane + 64; c < segs; c += 64) m = h[c].sum == 0.0 ? m : fmaxf(m, h[c].ref);
             m = qmh_wave_max(m);
-            const double ref2 = (double)m * 1.4426950408889634074;
-            s = sum0 == 0.0 ? 0.0 : sum0 * exp_sum<1>(&ref0, m - 700.0f, ref2);
+            s = sum0 == 0.0 ? 0.0 : sum0 * exp_of((double)ref0 - (double)m);
             for (int c = lane + 64; c < segs; c += 64) { // a sum of 0 has no reference to be in range of
                 const double e = h[c].sum;
-                if (e != 0.0) s = __builtin_fma(e, exp_sum<1>(&h[c].ref, m - 700.0f, ref2), s);
+                if (e != 0.0) s = __builtin_fma(e, exp_of((double)h[c].ref - (double)m), s);
             }
             s = (double)m + log(qmh_wave_sum_d(s));
         }
@@ -396,13 +420,12 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
                     for (int k = 0; k < 4; k++) to = v[k].sum == 0.0 ? to : fmaxf(to, v[k].ref);
                     to = qmh_wave_max(to);
                     const float ref = to > -__builtin_inff() ? to : 0.0f; // nothing yet: sums of 0
-                    const double ref2 = (double)ref * 1.4426950408889634074;
-                    if (to > m && m > -__builtin_inff()) s *= exp_sum<1>(&m, ref - 700.0f, ref2);
+                    if (to > m && m > -__builtin_inff()) s *= exp_of((double)m - (double)ref);
                     m = to;
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const float r = v[k].sum == 0.0 ? ref : v[k].ref;
-                        s = __builtin_fma(v[k].sum, exp_sum<1>(&r, ref - 700.0f, ref2), s);
+                        s = __builtin_fma(v[k].sum, exp_of((double)r - (double)ref), s);
                         if (c0 + 64 * k < segs) top[c0 + 64 * k] = v[k].top;
                     }
                 }
@@ -418,7 +441,7 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
             }
         }
         if (lane == 0 && w % share == 0) {
-            lse[b] = done ? __builtin_inf() : s; // marks a finished row
+            lse[b] = done ? __builtin_inf() : s; // marks a finished row: another's sum is at most 2^24 e^600, or NaN
             score[b] = (double)sc;
         }
     }
