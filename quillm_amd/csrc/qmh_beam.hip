@@ -754,6 +754,7 @@ __global__ __launch_bounds__(64) void k_beam_advance(const int32_t *parent, cons
 } // namespace
 
 extern "C" size_t qmh_beam_ws_bytes(const qmh_beam_args *a) {
+    if (a->n_groups == 0) return 0; // no rows to divide the waves among
     const size_t lists = (size_t)a->n_groups * a->n_beams * plan_scan(a).segs;
     return lists * (sizeof(scan_head) + a->n_out * sizeof(uint2));
 }
