@@ -234,7 +234,7 @@ int qmh_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const 
                      int32_t n_beams, void *stream);
 /* The same for sequences' own pages, in place: positions below len[parent] of the parent's pages go to the
  * same positions of the sequence's own (table [n_groups * n_beams][table_stride], len on the device, at most
- * max_len, a longer one counts as max_len). Tables and lengths stay (beams of a group are usually equally long; a
+ * max_len, a longer one counts as max_len, one below 0 as 0). Tables and lengths stay (beams of a group are usually equally long; a
  * program that keeps them otherwise reorders len with qmh_beam_reorder). A page outside the pool is neither read nor written.
  * No page may be in two rows of a group's tables. */
 int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t table_stride, const int32_t *len,

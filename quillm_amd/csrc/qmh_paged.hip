@@ -746,7 +746,8 @@ __global__ __launch_bounds__(256) void k_paged_reorder(const qmh_pages p, const 
         int2 ft = make_int2(-1, -1);
         if (from >= 0 && from < K && from != j) {
             n = len[g * K + from];
-            n = (n < max_len ? n : max_len) - (int)(pi * p.page_size); // positions of this page
+            n = n < 0 ? 0 : n < max_len ? n : max_len;
+            n -= (int)(pi * p.page_size); // positions of this page
             n = n < p.page_size ? n : p.page_size;
             if (n > 0) ft = make_int2(table[(int64_t)(g * K + from) * table_stride + pi], table[(int64_t)(g * K + j) * table_stride + pi]);
         }
