@@ -252,7 +252,9 @@ struct attn_wave {
     // l: the sum of a row's probabilities: a lane's own positions in l[0], or (16 bit) all of them in every element, by a
     // product with ones
     v4f l[NR];
-    float m[NR], off[NR], pass[NR]; // the reference, its negative in powers of two, the score that raises it
+    // the reference, its negative in powers of two (0: it is far from 0, scores are taken less m first), the score that raises it
+    float m[NR], off[NR], pass[NR];
+    bool far; // some row's is, or was
     int lim[NR];
     v4u k[RT][KC];
     uint32_t v[RT * 4][VW];
@@ -358,6 +360,9 @@ struct attn_wave {
         }
         // The reference value of a row's exponentials is raised only when a score passes it by 2^8: the sums stay exact
         // floats either way, and the rescaling of O is rare. (maximum: NaN wins, and needs no canonical operands.)
+        // Exponents are one fused product while the reference is at most 1024 powers of two: rounding it moves them by 2^-15 then. Beyond, that
+        // grows to whole powers and past the types' ranges, so the scores' own difference is taken first (an instruction more a
+        // score in waves that have such a row), and every larger score raises the reference.
         bool up = false;
         float mx[NR];
 #pragma unroll
@@ -371,6 +376,7 @@ struct attn_wave {
             up |= x > pass[c];
         }
         if (__any(up)) {
+            bool out = far;
 #pragma unroll
             for (int c = 0; c < NR; c++) {
                 float x = mx[c];
@@ -379,12 +385,26 @@ struct attn_wave {
                 if (x > m[c]) {
                     const float f = m[c] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[c] - x) * sc);
                     m[c] = x;
-                    off[c] = -x * sc;
-                    pass[c] = x + 8.0f / sc;
+                    const float o = -x * sc;
+                    const bool distant = __builtin_fabsf(o) > 1024.0f;
+                    off[c] = distant ? 0.0f : o;
+                    pass[c] = distant ? x : x + 8.0f / sc;
+                    out |= distant;
                     l[c] = l[c] * f;
 #pragma unroll
                     for (int t = 0; t < VE; t++) O[c][t] = O[c][t] * f;
                 }
+            }
+            far = __any(out);
+        }
+        if (far) {
+#pragma unroll
+            for (int c = 0; c < NR; c++) {
+                const float from = off[c] == 0.0f ? m[c] : 0.0f;
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) S[c][r][e] -= from;
             }
         }
 #pragma unroll
@@ -487,6 +507,7 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     const int H = s.a.n_heads, h0 = kvh * G;
     const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f; // exponentials are powers of two
     W x;
+    x.far = false;
 #pragma unroll
     for (int c = 0; c < NR; c++) {
         int r = row0 + 16 * c + i;
@@ -501,7 +522,7 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             x.Q[c][k] = v;
         }
         x.m[c] = x.pass[c] = -__builtin_inff();
-        x.off[c] = 0.0f;
+        x.off[c] = 1.0f; // not 0: no score yet
         x.l[c] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < W::VE; t++) x.O[c][t] = (v4f){0.f, 0.f, 0.f, 0.f};
