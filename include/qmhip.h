@@ -179,7 +179,9 @@ int qmh_paged_append(const qmh_append_args *a, void *stream);
  * heads after one another (n_heads a multiple of n_kv_heads: consecutive heads share a kv head); out must not
  * overlap q. Lengths are read on the device; max_len and max_prefix are their upper bounds, from which the work
  * is divided (0: no own pages / no prefix, the table and lengths then unused).
- * Scores are held in 32 bits: products that pass their range are infinite. A query that sees nothing (or only scores of
+ * Scores are held in 32 bits: products that pass their range are infinite. With 16-bit rows each position's probability is
+ * rounded to their type before its product with the values, and the sum of probabilities is of the rounded ones (f16: multiples of 2^-31
+ * of the largest, so one below 2^-32 of it counts as 0); with f32 rows it is not. A query that sees nothing (or only scores of
  * -inf) gives zeros. Where a sequence's len is outside [0, max_len] or a page it needs is outside
  * the pool, its rows are NaN; a group's prefix does so for all its sequences. What lies in pages behind a length
  * has no effect, whatever it holds. A position below len is the sequence's: an infinite or NaN value

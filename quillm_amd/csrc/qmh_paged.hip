@@ -167,9 +167,10 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
 //                 16-bit pairs are turned by byte permutes.
 // Rows behind a list's end are out of the loads' range and read as zero, whatever lies there. The four waves
 // of a workgroup take the steps of one chunk of positions in turn and are joined through LDS; chunks are joined by
-// k_attention_join. Probabilities are rounded to the rows' 16-bit type for the product with V (half a step of a value at
-// most 2^8 above the row's largest, as the sum of a few is; their sum is taken of the rounded ones), everything
-// else is f32; f32 rows stay f32 throughout, on the f32 MFMAs.
+// k_attention_join. Probabilities are rounded to the rows' 16-bit type for the product with V, which the matrix units then take
+// at their full rate (their sum is taken of the rounded ones), everything else is f32; f32 rows stay f32 throughout, on the f32
+// MFMAs. They are multiples of 2^7 there (ONE below): with the 2^8 that a score may pass its reference by, f16 holds them up to 2^15 of its 2^16,
+// and down to 2^-32 of the row's largest, half of its smallest step.
 // What bounds it: reading keys and values while a kv head has few rows (32 sequences of 350 to 700 own positions and
 // two shared prefixes of up to 4096, 32 x 128 bf16: 78 us for 396 MB, 5.1 TB/s, the rate of a large copy); VALU
 // issue where many rows share them (64 sequences x 8 heads on a prefix of 16380, 4 x 64 f16: a step of 64 rows and 32
@@ -252,7 +253,9 @@ struct attn_wave {
     // l: the sum of a row's probabilities: a lane's own positions in l[0], or (16 bit) all of them in every element, by a
     // product with ones
     v4f l[NR];
-    // the reference, its negative in powers of two (0: it is far from 0, scores are taken less m first), the score that raises it
+    static constexpr float ONE = 7.0f; // the exponent of a score at its row's reference
+    // the reference, its negative in powers of two and ONE (ONE alone: it is far from 0, scores are taken less m first), the score
+    // that raises it
     float m[NR], off[NR], pass[NR];
     bool far; // some row's is, or was
     int lim[NR];
@@ -385,9 +388,9 @@ struct attn_wave {
                 if (x > m[c]) {
                     const float f = m[c] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[c] - x) * sc);
                     m[c] = x;
-                    const float o = -x * sc;
+                    const float o = __builtin_fmaf(-x, sc, ONE);
                     const bool distant = __builtin_fabsf(o) > 1024.0f;
-                    off[c] = distant ? 0.0f : o;
+                    off[c] = distant ? ONE : o;
                     pass[c] = distant ? x : x + 8.0f / sc;
                     out |= distant;
                     l[c] = l[c] * f;
@@ -400,7 +403,7 @@ struct attn_wave {
         if (far) {
 #pragma unroll
             for (int c = 0; c < NR; c++) {
-                const float from = off[c] == 0.0f ? m[c] : 0.0f;
+                const float from = off[c] == ONE ? m[c] : 0.0f;
 #pragma unroll
                 for (int r = 0; r < RT; r++)
 #pragma unroll
@@ -522,7 +525,7 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             x.Q[c][k] = v;
         }
         x.m[c] = x.pass[c] = -__builtin_inff();
-        x.off[c] = 1.0f; // not 0: no score yet
+        x.off[c] = 0.0f; // not ONE: no score yet
         x.l[c] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < W::VE; t++) x.O[c][t] = (v4f){0.f, 0.f, 0.f, 0.f};
