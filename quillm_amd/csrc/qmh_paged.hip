@@ -64,10 +64,11 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
     }
     int at0[IT], at1[IT];
     float c[IT][VW], w[IT][VW];
+    bool turns[IT]; // a unit that does not is left out of the products: an infinite element would reach its neighbour through a sine of 0
 #pragma unroll
     for (int k = 0; k < IT; k++) {
         const int u = l + k * s.lanes;
-        const bool turn = u * VW < half;
+        const bool turn = turns[k] = u * VW < half;
         at0[k] = !turn ? rot + 2 * (u * VW - half) : PAIRS ? 2 * u * VW : u * VW;
         at1[k] = turn && !PAIRS ? at0[k] + half : at0[k] + VW;
 #pragma unroll
@@ -80,8 +81,6 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
                 c[k][i] = pr < 64 ? c[k][i] : c1;
                 w[k][i] = pr < 64 ? w[k][i] : w1;
             }
-            c[k][i] = turn ? c[k][i] : 1.0f;
-            w[k][i] = turn ? w[k][i] : 0.0f;
         }
     }
     // a head's row by its number: queries, keys, values
@@ -144,8 +143,9 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
                             x = x * inv * gain[ex];
                             y = y * inv * gain[ey];
                         }
-                        vx.e[ix] = (T)__builtin_fmaf(x, c[k][i], -(y * w[k][i]));
-                        vy.e[iy] = (T)__builtin_fmaf(x, w[k][i], y * c[k][i]);
+                        const float xt = __builtin_fmaf(x, c[k][i], -(y * w[k][i])), yt = __builtin_fmaf(x, w[k][i], y * c[k][i]);
+                        vx.e[ix] = (T)(turns[k] ? xt : x);
+                        vy.e[iy] = (T)(turns[k] ? yt : y);
                     }
                 }
                 *(qmh_vec<T, VW> *)(dst + at0[k]) = v0[k];
