@@ -105,8 +105,9 @@ int qmh_argmax(const float *x, int32_t n, int32_t *out, void *stream);
 /* Keys and values in pages on the device: k and v are [n_pages][n_kv_heads][page_size][head_dim] of dtype
  * (QMH_F32, QMH_F16 or QMH_BF16), 16-byte aligned; page_size a power of two in [16, 1024], head_dim a
  * multiple of 8 in [8, 256]. A table row of page numbers says where a sequence's positions lie: position
- * t is row t % page_size of page table[t / page_size]. Entries behind a sequence's last page are not
- * read. A page number outside [0, n_pages) is never followed (each op says what it does instead). */
+ * t is row t % page_size of page table[t / page_size]. Tables are whole arrays, [rows][stride]; entries
+ * behind a sequence's last page may hold anything (qmh_paged_attention may read those up to max_len or max_prefix, no op
+ * follows them). A page number outside [0, n_pages) is never followed (each op says what it does instead). */
 typedef struct {
     int32_t dtype;
     int32_t n_kv_heads, head_dim, page_size;
@@ -179,12 +180,13 @@ int qmh_paged_append(const qmh_append_args *a, void *stream);
  * heads after one another (n_heads a multiple of n_kv_heads: consecutive heads share a kv head); out must not
  * overlap q. Lengths are read on the device; max_len and max_prefix are their upper bounds, from which the work
  * is divided (0: no own pages / no prefix, the table and lengths then unused).
- * Scores are held in 32 bits: products that pass their range are infinite. With 16-bit rows each position's probability is
- * rounded to their type before its product with the values, and the sum of probabilities is of the rounded ones (f16: multiples of 2^-31
- * of the largest, so one below 2^-32 of it counts as 0); with f32 rows it is not. A query that sees nothing (or only scores of
- * -inf) gives zeros. Where a sequence's len is outside [0, max_len] or a page it needs is outside
- * the pool, its rows are NaN; a group's prefix does so for all its sequences. What lies in pages behind a length
- * has no effect, whatever it holds. A position below len is the sequence's: an infinite or NaN value
+ * Scores are held in 32 bits: products that pass their range are infinite. With 16-bit rows each position's
+ * probability is rounded to their type before its product with the values, and the sum of probabilities is of the
+ * rounded ones (f16: multiples of 2^-31 of the largest, so one below 2^-32 of it counts as 0); with f32 rows it is
+ * not. A query that sees nothing (or only scores of -inf) gives zeros. Where a sequence's len is outside [0,
+ * max_len] all its rows are NaN, where a page is outside the pool the rows of every query that sees a position of
+ * it (and maybe of its earlier queries); a group's prefix does so for all its sequences. What lies in pages behind
+ * a length has no effect, whatever it holds. A position below len is the sequence's: an infinite or NaN value
  * there may reach its queries that do not see it, too.
  * ws: qmh_paged_attention_ws(a) bytes (0 for bad arguments), 16-byte aligned, any contents. */
 typedef struct {
@@ -204,12 +206,15 @@ size_t qmh_paged_attention_ws(const qmh_attention_args *a);
 int qmh_paged_attention(const qmh_attention_args *a, void *ws, size_t ws_bytes, void *stream);
 
 /* A beam search's choice: the n_out best continuations of each group of n_beams rows of logits. Row b of a group
- * continues with token t at score[b] + logits[b][t] - log sum exp logits[b], in 64 bits; the best come first, among
- * equals the lower beam, then the lower token. logits: row r = group * n_beams + b at logits + r * stride elements of
- * dtype (QMH_F32, QMH_F16, QMH_BF16). done (NULL or [rows]): a nonzero row is finished, its one continuation
- * is token eos at score[b]. Continuations at -inf or NaN are none (a row of score -inf has none: a group's first
- * step gives its other beams -inf; a row with a NaN or +inf logit has none); places that stay over get score -inf,
- * parent -1 and token -1. out_*: [n_groups][n_out]; out_parent is b.
+ * continues with token t at score[b] + logits[b][t] - log sum exp logits[b], in 64 bits; the best come first,
+ * among equals the lower beam, then the lower token. (Different logits of a row can come to one total, where its
+ * score or log sum is some 2^26 times as far from 0 as they are: a larger one may then be taken before a lower
+ * token.) logits: row r = group * n_beams + b at logits + r * stride elements of dtype (QMH_F32, QMH_F16,
+ * QMH_BF16), read as aligned 16 bytes: up to 15 on either side of a row are read, too, and have no effect. done
+ * (NULL or [rows]): a nonzero row is finished, its one continuation is token eos at score[b]. Continuations at
+ * -inf or NaN are none (a row of score -inf has none: a group's first step gives its other beams -inf; a row with
+ * a NaN or +inf logit has none); places that stay over get score -inf, parent -1 and token -1. out_*:
+ * [n_groups][n_out]; out_parent is b.
  * n_beams and n_out at most 64, vocab at most 2^24. out_score may be score where n_out = n_beams.
  * ws: qmh_beam_select_ws(a) bytes (0 for bad arguments), 16-byte aligned, any contents. */
 typedef struct {
