@@ -188,6 +188,7 @@ int qmh_paged_append(const qmh_append_args *a, void *stream);
  * it (and maybe of its earlier queries); a group's prefix does so for all its sequences. What lies in pages behind
  * a length has no effect, whatever it holds. A position below len is the sequence's: an infinite or NaN value
  * there may reach its queries that do not see it, too.
+ * scale: any sign, at most 2^127 in magnitude.
  * ws: qmh_paged_attention_ws(a) bytes (0 for bad arguments), 16-byte aligned, any contents. */
 typedef struct {
     const qmh_pages *pages;

@@ -411,7 +411,8 @@ static int check_attention(const qmh_attention_args *a, const char *me) {
         return fail("%s: max_len %d needs len and a table of that many positions", me, a->max_len);
     if (a->max_prefix && (!a->prefix_table || !a->prefix_len || a->max_prefix > (int64_t)a->prefix_stride * p->page_size))
         return fail("%s: max_prefix %d needs prefix_len and a table of that many positions", me, a->max_prefix);
-    if (!isfinite(a->scale)) return fail("%s: scale is not finite", me);
+    /* exponents are taken as powers of two: the scale times log2 e has to be a float, too */
+    if (!(fabsf(a->scale) <= 0x1p127f)) return fail("%s: scale %g is not finite or above 2^127", me, a->scale);
     return 0;
 }
 
