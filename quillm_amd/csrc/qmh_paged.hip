@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void k_paged_append(const append_args s) {
 // two shared prefixes of up to 4096, 32 x 128 bf16: 78 us for 396 MB, 5.1 TB/s, the rate of a large copy); VALU
 // issue where many rows share them (64 sequences x 8 heads on a prefix of 16380, 4 x 64 f16: a step of 64 rows and 32
 // positions is 36 MFMAs (577 cycles) and 163 VALU instructions, 32 of them exponentials at a quarter of the rate; the
-// prefix runs at 800 TFLOP/s between 32760 and 65520 positions, 28 us in all with starts, ends and the join of parts).
+// prefix runs at 800 TFLOP/s between 32760 and 65520 positions, 27 us in all with starts, ends and the join of parts).
 // Two waves a SIMD (at most 256 registers) measured 47 -> 35 us against one; eight waves a workgroup and the next
 // scores between this step's exponentials gained nothing.
 
