@@ -208,14 +208,12 @@ int qmh_paged_attention(const qmh_attention_args *a, void *ws, size_t ws_bytes, 
 
 /* A beam search's choice: the n_out best continuations of each group of n_beams rows of logits. Row b of a group
  * continues with token t at score[b] + logits[b][t] - log sum exp logits[b], in 64 bits; the best come first,
- * among equals the lower beam, then the lower token. (Different logits of a row can come to one total, where its
- * score or log sum is some 2^26 times as far from 0 as they are: a larger one may then be taken before a lower
- * token.) logits: row r = group * n_beams + b at logits + r * stride elements of dtype (QMH_F32, QMH_F16,
- * QMH_BF16), read as aligned 16 bytes: up to 15 on either side of a row are read, too, and have no effect. done
- * (NULL or [rows]): a nonzero row is finished, its one continuation is token eos at score[b]. Continuations at
- * -inf or NaN are none (a row of score -inf has none: a group's first step gives its other beams -inf; a row with
- * a NaN or +inf logit has none); places that stay over get score -inf, parent -1 and token -1. out_*:
- * [n_groups][n_out]; out_parent is b.
+ * among equals the lower beam, then the lower token. logits: row r = group * n_beams + b at logits + r * stride
+ * elements of dtype (QMH_F32, QMH_F16, QMH_BF16), read as aligned 16 bytes: up to 15 on either side of a row are
+ * read, too, and have no effect. done (NULL or [rows]): a nonzero row is finished, its one continuation is token
+ * eos at score[b]. Continuations at -inf or NaN are none (a row of score -inf has none: a group's first step gives
+ * its other beams -inf; a row with a NaN or +inf logit has none); places that stay over get score -inf, parent -1
+ * and token -1. out_*: [n_groups][n_out]; out_parent is b.
  * n_beams and n_out at most 64, vocab at most 2^24. out_score may be score where n_out = n_beams.
  * ws: qmh_beam_select_ws(a) bytes (0 for bad arguments), 16-byte aligned, any contents. */
 typedef struct {

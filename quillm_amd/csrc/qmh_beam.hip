@@ -356,7 +356,7 @@ template <bool MANY, int JT>
 __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const scan_head *heads, const uint2 *cands, int segs) {
     constexpr int NW = JT / 64, TOPS = MANY ? SCAN_WAVES : 1;
     __shared__ double lse[64], score[64];
-    __shared__ uint64_t ckey[JOIN_CAP], bk[NW];
+    __shared__ uint64_t ckey[JOIN_CAP], bk[NW], rkey[64]; // rkey: the chosen totals, best first
     __shared__ uint32_t cplace[JOIN_CAP], best_of[JT], bf[NW], tops[TOPS];
     __shared__ uint16_t chosen[TOPS];
     __shared__ int ncand, nchosen;
@@ -558,25 +558,29 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
         }
     });
     __syncthreads();
-    auto write = [&](int o, uint64_t k, uint32_t p) {
+    auto write = [&](int o, uint64_t k, uint32_t p) { // every score has been read: out_score may be score
         const int64_t at = (int64_t)g * n_out + o;
         a.out_score[at] = k ? (float)of_key_d(k) : -__builtin_inff();
         a.out_parent[at] = k ? (int)(p / (uint32_t)a.vocab) : -1;
         a.out_token[at] = k ? (int)(p % (uint32_t)a.vocab) : -1;
     };
     const int n = ncand;
-    if (n <= JOIN_CAP) { // every score has been read: out_score may be score
+    uint64_t below = ~0ull; // what was chosen last: its total, then its place
+    int64_t after = -1;
+    if (n <= JOIN_CAP) {
         rank_all(
             n, JT, [&](int i, int c) { return (ckey[i] > ckey[c]) | ((ckey[i] == ckey[c]) & (cplace[i] < cplace[c])); }, // no branches: the reads overlap
             [&](int c, int r) {
-                if (r < n_out) write(r, ckey[c], cplace[c]);
+                if (r < n_out) {
+                    rkey[r] = ckey[c];
+                    write(r, ckey[c], cplace[c]);
+                }
             });
-        if (tid >= n && tid < n_out) write(tid, 0, 0);
-        return;
-    }
-    uint64_t below = ~0ull; // what was chosen last: its total, then its place
-    int64_t after = -1;
-    for (int o = 0; o < n_out; o++) {
+        if (tid >= n && tid < n_out) {
+            rkey[tid] = 0;
+            write(tid, 0, 0);
+        }
+    } else for (int o = 0; o < n_out; o++) {
         uint64_t best = 0;
         uint32_t at = 0xffffffffu;
         each([&](const uint64_t *q, const uint32_t *p) {
@@ -611,12 +615,48 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
         below = best;
         after = at;
         if (tid == 0) {
-            ckey[o] = best;
-            cplace[o] = at;
+            rkey[o] = best;
+            write(o, best, at);
         }
     }
     __syncthreads();
-    if (tid < n_out) write(tid, ckey[tid], cplace[tid]);
+    // The scan chose by logits. Where different logits of a row come to one total, the last one chosen, a lower token may not be
+    // among the candidates: its logit is at most 2^-26 of the row's score, log sum and total then (a step of a float against
+    // one of a double). If some row has such, the places of that total go to the first of all logits that come to it.
+    const uint64_t last = rkey[n_out - 1];
+    bool coarse = false;
+    if (last && lane < K) {
+        const double L = lse[lane], sc = score[lane], t = of_key_d(last);
+        coarse = L > -__builtin_inf() && L < __builtin_inf() && !(fabs((t - sc) + L) > 0x1p-26 * (fabs(L) + fabs(sc) + fabs(t)));
+    }
+    if (__any(coarse)) { // every wave finds the same
+        int at = __popcll(__ballot(lane < n_out && rkey[lane] > last));
+        for (int b = 0; b < K && at < n_out; b++) {
+            const double L = lse[b], sc = score[b];
+            const bool done = L == __builtin_inf();
+            if (!done && !(L > -__builtin_inf())) continue;
+            const int64_t row = (int64_t)(g * K + b) * a.stride;
+            for (int t0 = 0; t0 < (done ? 1 : a.vocab) && at < n_out; t0 += JT) {
+                const int t = t0 + tid;
+                float x = -__builtin_inff();
+                if (!done && t < a.vocab)
+                    x = a.dtype == QMH_F32   ? ((const float *)a.logits)[row + t]
+                        : a.dtype == QMH_F16 ? qmh_to_f(((const qmh_f16 *)a.logits)[row + t])
+                                             : qmh_to_f(((const qmh_bf16 *)a.logits)[row + t]);
+                const bool in = done ? tid == 0 && key_of_d(sc) == last : x > -__builtin_inff() && key_of_d(sc + ((double)x - L)) == last;
+                const uint64_t all = __ballot(in);
+                __syncthreads(); // bf has been read
+                if (lane == 0) bf[w] = (uint32_t)__popcll(all);
+                __syncthreads();
+                int to = at + behind(all);
+                for (int k = 0; k < NW; k++) {
+                    to += k < w ? (int)bf[k] : 0;
+                    at += (int)bf[k];
+                }
+                if (in && to < n_out) write(to, last, (uint32_t)(b * a.vocab) + (uint32_t)(done ? a.eos : t));
+            }
+        }
+    }
 }
 
 // How a row is cut: into segments of whole pieces, one a wave, as many as give the chip SCAN_WAVES waves: three a SIMD, so
