@@ -359,7 +359,7 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
     __shared__ uint64_t ckey[JOIN_CAP], bk[NW], rkey[64]; // rkey: the chosen totals, best first
     __shared__ uint32_t cplace[JOIN_CAP], best_of[JT], bf[NW], tops[TOPS];
     __shared__ uint16_t chosen[TOPS];
-    __shared__ int ncand, nchosen;
+    __shared__ int ncand, nchosen, listed[64];
     const int g = blockIdx.x, tid = threadIdx.x, w = tid >> 6, lane = tid & 63, K = a.n_beams, n_out = a.n_out;
     if (tid == 0) ncand = nchosen = 0;
     // few beams: several waves a row, each with the row's log sum for itself (MANY: a wave a row)
@@ -622,39 +622,70 @@ __global__ __launch_bounds__(JT) void k_beam_join(const qmh_beam_args a, const s
     __syncthreads();
     // The scan chose by logits. Where different logits of a row come to one total, the last one chosen, a lower token may not be
     // among the candidates: its logit is at most 2^-26 of the row's score, log sum and total then (a step of a float against
-    // one of a double). If some row has such, the places of that total go to the first of all logits that come to it.
+    // one of a double), and its segment has listed n_out that are no less. If some row can have such, the places of that total go to
+    // the first of all logits that come to it: 4 rows of 128256 with their best at 0 take 48 us, 12 otherwise. (Rows of log
+    // probabilities have one next to 0 each, but not n_out: the count keeps them at 12.)
     const uint64_t last = rkey[n_out - 1];
     bool coarse = false;
     if (last && lane < K) {
         const double L = lse[lane], sc = score[lane], t = of_key_d(last);
         coarse = L > -__builtin_inf() && L < __builtin_inf() && !(fabs((t - sc) + L) > 0x1p-26 * (fabs(L) + fabs(sc) + fabs(t)));
     }
-    if (__any(coarse)) { // every wave finds the same
-        int at = __popcll(__ballot(lane < n_out && rkey[lane] > last));
-        for (int b = 0; b < K && at < n_out; b++) {
-            const double L = lse[b], sc = score[b];
-            const bool done = L == __builtin_inf();
-            if (!done && !(L > -__builtin_inf())) continue;
-            const int64_t row = (int64_t)(g * K + b) * a.stride;
-            for (int t0 = 0; t0 < (done ? 1 : a.vocab) && at < n_out; t0 += JT) {
-                const int t = t0 + tid;
+    if (!__any(coarse)) return; // every wave finds the same
+    if (n <= JOIN_CAP) {
+        if (tid < 64) listed[tid] = 0;
+        __syncthreads();
+        for (int c = tid; c < n; c += JT)
+            if (ckey[c] >= last) atomicAdd(&listed[cplace[c] / (uint32_t)a.vocab], 1);
+        __syncthreads();
+        if (!__any(coarse && listed[lane] >= n_out)) return;
+    }
+    int at = __popcll(__ballot(lane < n_out && rkey[lane] > last));
+    // the next places, up to n_out, to the lanes that have one, in their order
+    auto put = [&](bool in, uint32_t p) {
+        const uint64_t all = __ballot(in);
+        __syncthreads(); // bf has been read
+        if (lane == 0) bf[w] = (uint32_t)__popcll(all);
+        __syncthreads();
+        int to = at + behind(all);
+        for (int k = 0; k < NW; k++) {
+            to += k < w ? (int)bf[k] : 0;
+            at += (int)bf[k];
+        }
+        if (in && to < n_out) write(to, last, p);
+    };
+    for (int b = 0; b < K && at < n_out; b++) {
+        const double L = lse[b], sc = score[b];
+        const uint32_t p0 = (uint32_t)(b * a.vocab);
+        if (L == __builtin_inf()) { // finished
+            put(tid == 0 && key_of_d(sc) == last, p0 + (uint32_t)a.eos);
+            continue;
+        }
+        if (!(L > -__builtin_inf())) continue;
+        const int64_t row = (int64_t)(g * K + b) * a.stride;
+        for (int t0 = 0; t0 < a.vocab && at < n_out; t0 += 8 * JT) {
+            bool in[8], some = false;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int t = t0 + k * JT + tid;
                 float x = -__builtin_inff();
-                if (!done && t < a.vocab)
+                if (t < a.vocab)
                     x = a.dtype == QMH_F32   ? ((const float *)a.logits)[row + t]
                         : a.dtype == QMH_F16 ? qmh_to_f(((const qmh_f16 *)a.logits)[row + t])
                                              : qmh_to_f(((const qmh_bf16 *)a.logits)[row + t]);
-                const bool in = done ? tid == 0 && key_of_d(sc) == last : x > -__builtin_inff() && key_of_d(sc + ((double)x - L)) == last;
-                const uint64_t all = __ballot(in);
-                __syncthreads(); // bf has been read
-                if (lane == 0) bf[w] = (uint32_t)__popcll(all);
-                __syncthreads();
-                int to = at + behind(all);
-                for (int k = 0; k < NW; k++) {
-                    to += k < w ? (int)bf[k] : 0;
-                    at += (int)bf[k];
-                }
-                if (in && to < n_out) write(to, last, (uint32_t)(b * a.vocab) + (uint32_t)(done ? a.eos : t));
+                in[k] = x > -__builtin_inff() && key_of_d(sc + ((double)x - L)) == last;
+                some |= in[k];
             }
+            __syncthreads(); // bf has been read
+            const bool here = __any(some);
+            if (lane == 0) bf[w] = here;
+            __syncthreads();
+            uint32_t any = 0;
+            for (int k = 0; k < NW; k++) any |= bf[k];
+            if (!any) continue;
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (at < n_out) put(in[k], p0 + (uint32_t)(t0 + k * JT + tid));
         }
     }
 }
