@@ -130,7 +130,7 @@ __device__ __forceinline__ void wave_sync() {
 // n_out best, the least of them, which only larger logits pass, since later ones lose a tie. Where a piece brings
 // more than the list holds (a rising row, repeated values) its own lane maxima raise the bound, and if that does not help
 // the exact bound of the piece is searched bit by bit.
-// Bound by VALU issue (34 instructions a logit, 14 of them the exponential's 64-bit ones: 21 of the 33 us of 24.6 million f32
+// Bound by VALU issue (34 instructions a logit, 14 of them the exponential's 64-bit ones: 21 of the 34 us of 24.6 million f32
 // logits) beside the loads (98 MB).
 template <typename T, int EPT, int VEC>
 __global__ __launch_bounds__(SEL_T) void k_beam_scan(const qmh_beam_args a, scan_head *heads, uint2 *cands, int row0, int iters) {
