@@ -246,6 +246,165 @@ int qmh_beam_reorder(const qmh_beam_state *s, void *dst, const void *src, const 
 int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t table_stride, const int32_t *len,
                       int32_t max_len, const int32_t *parent, int32_t n_groups, int32_t n_beams, void *stream);
 
+/* ------------------------------------------------------------------ drafted trees over pages
+ * Op level, as the section above (types, errors, streams, workspaces, the current device). No reference counterpart. A
+ * server that checks a tree of guessed tokens for each of its sequences in one pass calls, for a step,
+ *   qmh_paged_plan       pages, rows, slots and positions of the trees' nodes, and what each node sees,
+ *   qmh_paged_append and qmh_tree_attention in each layer,
+ *   qmh_logits_edit      penalties, biases and grammars, and each row's best token (or a sampler's own choice),
+ *   qmh_tree_accept      the path that the model agrees with, its keys and values moved to follow the context,
+ * and the next qmh_paged_plan takes back the pages behind what was kept. Everything is read on the device, so a step
+ * can be captured into a graph.
+ *
+ * A tree: node j of a sequence has parent[j], an earlier node (below j), or -1. Node 0 is the root: the sequence's current
+ * token, chosen already, its keys and values not yet in the pages. A parent that is none counts as -1.
+ * Rows: sequence i's nodes are rows first[i] to first[i + 1] of the per-row arrays (first [n_seq + 1] on the device, not
+ * decreasing; qmh_paged_plan writes it), or, with first NULL, rows i * q to i * q + q, q the most nodes of a sequence. A sequence
+ * whose rows are outside the arrays, or more than q, is left out, and what rows that it shares with others hold is not
+ * defined. Rows before the first sequence's and behind the last one's are left as they are.
+ * Masks: row j of a sequence's mask says with bit k % 32 of word k / 32 whether node j sees node k of its sequence. */
+
+/* Pages and places for the positions that sequences are to hold. Sequence i holds len[i] positions, in the first ceil(len / page_size)
+ * pages of its table row (tables as above; numbers are moved, never followed). It keeps the first keep[i] of them (NULL: all)
+ * and gets add[i] new ones (NULL: none) behind: pages that it then lacks are taken from the ring of free ones, pages that
+ * it no longer needs go to the ring's end (another call may take them) and their table entries become -1. len[i] becomes keep + add.
+ * The ring: free_pages[free_size], free_state {first, count}: the free ones are entries first, first + 1, ... modulo free_size;
+ * pages are taken from its front, in the sequences' order, and given back in that order, too. free_size is at least the
+ * number of pages there are.
+ * Tokens: the new positions of all sequences are rows first[i] to first[i + 1] of seq, slot and pos [n_tokens], as qmh_paged_append
+ * takes them: slot keep[i] + j, pos base[i] (NULL: 0) + keep[i] + j; rows behind the last one get -1 in all three. With n_tokens = 0
+ * there are none to place: first, seq, slot, pos and base are not looked at (add is NULL then or 0 throughout).
+ * Trees (parent not NULL): parent [n_seq][parent_stride] (parent_stride 0: one tree for all), at most tree_size (1 to 1024)
+ * new positions a sequence; pos is base + keep + the node's depth, and mask (or NULL) [n_seq][tree_size][ceil(tree_size / 32)]
+ * gets the row of each new node: its ancestors and itself.
+ * refused[i] (NULL allowed) says what became of sequence i: 0 served; 3 a number outside its range (len, keep, add, or
+ * more than the table row or the tree takes); 1 pages are short (it needs some and the sum of what it and the sequences before it
+ * ask for is more than there are; or the ring has no room for what it gives); 2 rows are short (n_tokens, likewise).
+ * Of a refused sequence nothing changes, and it has no rows.
+ * n_seq at most 65535, n_seq * table_stride below 2^31, n_tokens at most 2^24. keep may be len.
+ * ws: qmh_paged_plan_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
+typedef struct {
+    int32_t n_seq, page_size;
+    int32_t *table;
+    int32_t table_stride;
+    int32_t *len;
+    const int32_t *keep, *add;
+    int32_t *free_pages;
+    int32_t free_size;
+    int32_t *free_state;
+    const int32_t *base;
+    int32_t n_tokens;
+    int32_t *first, *seq, *slot, *pos;
+    int32_t *refused;
+    const int32_t *parent;
+    int32_t parent_stride, tree_size;
+    uint32_t *mask;
+} qmh_plan_args;
+size_t qmh_paged_plan_ws(const qmh_plan_args *a);
+int qmh_paged_plan(const qmh_plan_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* qmh_paged_attention with nodes of trees in place of consecutive queries. base: as there, but q_len is the most nodes of a
+ * sequence, and q and out have n_rows rows (with first NULL at least n_seq * q_len). The n nodes of a sequence are the last n
+ * of its len positions; node j sees the group's prefix, the len - n positions before the nodes, and those nodes that row j
+ * of the sequence's mask says: words at mask + i * mask_stride + j * mask_words (mask_words >= ceil(q_len / 32), mask_stride 0: one
+ * mask for all; bits of nodes that are not there have no effect). mask NULL: nodes 0 to j, a chain.
+ * What a node does not see has no effect on it, whatever it holds. Values are summed with weights of up to 2^15 each before the sum of
+ * these divides them: finite f32 and bf16 values above 2^112 over the number of positions may come out infinite. A node that sees nothing (or only scores of -inf) gives
+ * zeros; where len is outside [n, max_len], or a page is outside the pool, rows are NaN as qmh_paged_attention says.
+ * ws: qmh_tree_attention_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
+typedef struct {
+    qmh_attention_args base;
+    int32_t n_rows;
+    const int32_t *first;
+    const uint32_t *mask;
+    int64_t mask_stride;
+    int32_t mask_words;
+} qmh_tree_args;
+size_t qmh_tree_attention_ws(const qmh_tree_args *a);
+int qmh_tree_attention(const qmh_tree_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* Logits edited before a choice: row r of logits [n_rows][stride] of dtype (QMH_F32, QMH_F16, QMH_BF16) of sequence i, token t:
+ *   x = logits; if t is in the history: x / repetition[i] where x > 0, x * repetition[i] elsewhere;
+ *   less frequency[i] * c + presence[i] * (c > 0), c how often t is in the outputs; plus its bias; -inf where the grammar forbids it.
+ * Computed in 32 bits, rounded once to dtype. out (NULL: not wanted) [n_rows][out_stride], may be logits with the same stride, must
+ * not overlap it otherwise. best (NULL: not wanted) [n_rows]: the first token of the largest edited logit, before it is
+ * rounded; -1 where all are -inf or NaN.
+ * Sequences have at most rows_per_seq rows (first as above, or NULL).
+ * history [n_seq][history_stride]: the first history_len[i] tokens (at most history_stride count), of which the first prompt_len[i]
+ * (NULL: none) are the prompt's, the others outputs. Tokens outside [0, vocab) are none. history NULL: none anywhere. repetition,
+ * presence, frequency: [n_seq] or NULL (1, 0, 0). A repetition that is not above 0 counts as 1.
+ * bias_token, bias [n_seq][bias_stride], the first bias_len[i] of them (at most bias_stride count); of a token that is there twice the
+ * last one counts. Tokens outside [0, vocab) are none. bias NULL: none.
+ * allow [n_allow][allow_stride] words: bit t % 32 of word t / 32 of row allow_row[r] says whether token t may follow (allow_row
+ * outside [0, n_allow): all may; allow_row NULL: row r of allow, n_allow >= n_rows). allow NULL: no grammar.
+ * node_token [n_seq][node_stride] (NULL: rows are no trees): row j of sequence i has the nodes that its mask's row says behind its
+ * history, as outputs: itself and its ancestors (mask, mask_stride, mask_words as for qmh_tree_attention; mask NULL: nodes 0 to j).
+ * vocab at most 2^24; n_seq at most 65535; rows_per_seq at most 1024 with node_token.
+ * ws: qmh_logits_edit_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
+typedef struct {
+    int32_t dtype, n_rows, vocab;
+    const void *logits;
+    int64_t stride;
+    void *out;
+    int64_t out_stride;
+    int32_t *best;
+    int32_t n_seq, rows_per_seq;
+    const int32_t *first;
+    const int32_t *history;
+    int64_t history_stride;
+    const int32_t *history_len, *prompt_len;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_token;
+    const float *bias;
+    const int32_t *bias_len;
+    int32_t bias_stride;
+    const uint32_t *allow;
+    int64_t allow_stride;
+    int32_t n_allow;
+    const int32_t *allow_row;
+    const int32_t *node_token;
+    int32_t node_stride;
+    const uint32_t *mask;
+    int64_t mask_stride;
+    int32_t mask_words;
+} qmh_logits_args;
+size_t qmh_logits_edit_ws(const qmh_logits_args *a);
+int qmh_logits_edit(const qmh_logits_args *a, void *ws, size_t ws_bytes, void *stream);
+
+/* The path of each tree that the model agrees with. choice[row] is the token that was chosen after the row's node (qmh_logits_edit's best, or
+ * a sampler's). Node 0 is accepted; after node p the child with token = choice of p, the one with the lowest number if there are
+ * several, until there is none (tokens below 0 are never accepted). parent [n_seq][parent_stride], token [n_seq][token_stride]
+ * (strides 0: the same for all), tree_size (1 to 1024) the most nodes of a sequence, rows as above.
+ * Of a sequence with n nodes, the last n of its len positions, count gets the nodes accepted, path (NULL or [n_seq][tree_size])
+ * their numbers, -1 behind, next the choice after the last (the next tree's node 0), keep len - n + count: the positions
+ * that stay, for qmh_paged_plan. history [n_seq][history_stride] (NULL: none) gets the accepted nodes' tokens behind its history_len, which
+ * grows by as many; both end at history_stride. Without nodes: 0, -1, -1 and len. A sequence that is left out (its rows, or
+ * len outside [n, table_stride * page_size], len < n without pages): 0, -1, -1 and -1, nothing moved.
+ * pages (NULL: nothing is moved): keys and values of accepted nodes move to the positions len - n on, in n_layers pools that
+ * are layer_stride elements apart (pages->k and v are the first layer's; a multiple of 16 bytes), through table [n_seq][table_stride].
+ * Where either place's page is outside the pool, that node is not moved. No page may be in two of the table's places.
+ * count, next and keep must not overlap each other or any input. n_seq at most 65535, n_layers at most 1024. */
+typedef struct {
+    int32_t n_seq, tree_size;
+    const int32_t *parent;
+    int32_t parent_stride;
+    const int32_t *token;
+    int32_t token_stride;
+    int32_t n_rows;
+    const int32_t *first;
+    const int32_t *choice, *len;
+    int32_t *count, *path, *next, *keep;
+    int32_t *history;
+    int64_t history_stride;
+    int32_t *history_len;
+    const qmh_pages *pages;
+    int32_t n_layers;
+    int64_t layer_stride;
+    const int32_t *table;
+    int32_t table_stride;
+} qmh_accept_args;
+int qmh_tree_accept(const qmh_accept_args *a, void *stream);
+
 /* ------------------------------------------------------------------ model level (host arguments) */
 
 /* qm_config (src/model.h:8-11) */

@@ -89,6 +89,36 @@ class BeamState(ctypes.Structure):
     _fields_ = _fields(l="n_outer outer_stride seq_stride n_rows row_stride live")
 
 
+class PlanArgs(ctypes.Structure):
+    """qmh_plan_args."""
+
+    _fields_ = _fields(i="n_seq page_size", p="table", i1="table_stride", p1="len keep add free_pages", i2="free_size", p2="free_state base",
+                       i3="n_tokens", p3="first seq slot pos refused parent", i4="parent_stride tree_size", p4="mask")
+
+
+class TreeArgs(ctypes.Structure):
+    """qmh_tree_args."""
+
+    _fields_ = [("base", AttentionArgs)] + _fields(i="n_rows", p="first mask", l="mask_stride", i1="mask_words")
+
+
+class LogitsArgs(ctypes.Structure):
+    """qmh_logits_args."""
+
+    _fields_ = _fields(i="dtype n_rows vocab", p="logits", l="stride", p1="out", l1="out_stride", p2="best", i1="n_seq rows_per_seq",
+                       p3="first history", l2="history_stride",
+                       p4="history_len prompt_len repetition presence frequency bias_token bias bias_len", i2="bias_stride", p5="allow",
+                       l3="allow_stride", i3="n_allow", p6="allow_row node_token", i4="node_stride", p7="mask", l4="mask_stride", i5="mask_words")
+
+
+class AcceptArgs(ctypes.Structure):
+    """qmh_accept_args."""
+
+    _fields_ = (_fields(i="n_seq tree_size", p="parent", i1="parent_stride", p1="token", i2="token_stride n_rows",
+                        p2="first choice len count path next keep history", l="history_stride", p3="history_len") +
+                [("pages", ctypes.POINTER(Pages))] + _fields(i="n_layers", l="layer_stride", p="table", i1="table_stride"))
+
+
 _lib = None
 
 
@@ -143,6 +173,13 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "qmh_beam_select": (ctypes.c_int, [ctypes.POINTER(BeamArgs), vp, sz, vp]),
         "qmh_beam_reorder": (ctypes.c_int, [ctypes.POINTER(BeamState), vp, vp, vp, i32, i32, vp]),
         "qmh_paged_reorder": (ctypes.c_int, [ctypes.POINTER(Pages), vp, i32, vp, i32, vp, i32, i32, vp]),
+        "qmh_paged_plan_ws": (sz, [ctypes.POINTER(PlanArgs)]),
+        "qmh_paged_plan": (ctypes.c_int, [ctypes.POINTER(PlanArgs), vp, sz, vp]),
+        "qmh_tree_attention_ws": (sz, [ctypes.POINTER(TreeArgs)]),
+        "qmh_tree_attention": (ctypes.c_int, [ctypes.POINTER(TreeArgs), vp, sz, vp]),
+        "qmh_logits_edit_ws": (sz, [ctypes.POINTER(LogitsArgs)]),
+        "qmh_logits_edit": (ctypes.c_int, [ctypes.POINTER(LogitsArgs), vp, sz, vp]),
+        "qmh_tree_accept": (ctypes.c_int, [ctypes.POINTER(AcceptArgs), vp]),
         "qmh_model_create": (vp, [ctypes.POINTER(QmhConfig), ctypes.POINTER(TensorView), ctypes.POINTER(TensorView),
                                   ctypes.POINTER(TensorView), ctypes.POINTER(TensorView)]),
         "qmh_model_load": (vp, [ctypes.c_char_p, i32]),

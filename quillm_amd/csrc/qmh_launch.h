@@ -254,6 +254,15 @@ int qmh_launch_beam_advance(const int32_t *parent, const int32_t *token, int eos
 int qmh_launch_paged_reorder(const qmh_pages *p, const int32_t *table, int table_stride, const int32_t *len, int max_len,
                              const int32_t *parent, int n_groups, int n_beams, void *stream);
 
+/* ---- drafted trees over pages (qmh_tree.hip, qmh_logits.hip): arguments checked by the host code */
+size_t qmh_plan_ws_bytes(const qmh_plan_args *a);
+int qmh_launch_paged_plan(const qmh_plan_args *a, void *ws, void *stream);
+size_t qmh_tree_ws_bytes(const qmh_tree_args *a, int cus);
+int qmh_launch_tree_attention(const qmh_tree_args *a, int cus, void *ws, void *stream);
+size_t qmh_logits_ws_bytes(const qmh_logits_args *a, int cus);
+int qmh_launch_logits_edit(const qmh_logits_args *a, int cus, void *ws, void *stream);
+int qmh_launch_tree_accept(const qmh_accept_args *a, void *stream);
+
 /* op-level kernels */
 int qmh_launch_h2f(const uint16_t *h, float *f, int64_t n, void *stream);
 int qmh_launch_f2h(const float *f, uint16_t *h, int64_t n, void *stream);

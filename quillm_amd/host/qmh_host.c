@@ -501,6 +501,155 @@ int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t tabl
     return 0;
 }
 
+/* ------------------------------------------------------------------ drafted trees over pages */
+
+static int check_ws(const char *me, size_t need, const void *ws, size_t ws_bytes) {
+    if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
+        return fail("%s: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", me, need, ws ? ws_bytes : 0);
+    return 0;
+}
+
+static int check_plan(const qmh_plan_args *a, const char *me) {
+    if (!a) return fail("%s: NULL arguments", me);
+    if (a->n_seq < 0 || a->n_seq > 65535) return fail("%s: n_seq %d outside [0, 65535]", me, a->n_seq);
+    if (a->page_size < 16 || a->page_size > 1024 || (a->page_size & (a->page_size - 1)))
+        return fail("%s: page_size %d is not a power of two in [16, 1024]", me, a->page_size);
+    if (!a->table || !a->len || !a->free_pages || !a->free_state) return fail("%s: NULL table, len, free_pages or free_state", me);
+    if (a->table_stride < 1 || (int64_t)a->n_seq * a->table_stride > 0x7fffffff || (int64_t)a->table_stride * a->page_size > 0x7fffffff)
+        return fail("%s: tables of %d x %d pages of %d positions", me, a->n_seq, a->table_stride, a->page_size);
+    if (a->free_size < 1 || a->free_size > 0x40000000) return fail("%s: free_size %d outside [1, 2^30]", me, a->free_size);
+    if (a->n_tokens < 0 || a->n_tokens > 1 << 24) return fail("%s: n_tokens %d outside [0, 2^24]", me, a->n_tokens);
+    if (a->n_tokens && (!a->first || !a->seq || !a->slot || !a->pos)) return fail("%s: NULL first, seq, slot or pos", me);
+    if (a->parent) {
+        if (!a->n_tokens) return fail("%s: trees need n_tokens", me);
+        if (a->tree_size < 1 || a->tree_size > 1024) return fail("%s: tree_size %d outside [1, 1024]", me, a->tree_size);
+        if (a->parent_stride && a->parent_stride < a->tree_size) return fail("%s: parent_stride %d of trees of %d", me, a->parent_stride, a->tree_size);
+    } else if (a->mask) {
+        return fail("%s: a mask needs parents", me);
+    }
+    return 0;
+}
+
+size_t qmh_paged_plan_ws(const qmh_plan_args *a) {
+    if (check_plan(a, "paged_plan_ws")) return 0;
+    return qmh_plan_ws_bytes(a);
+}
+
+int qmh_paged_plan(const qmh_plan_args *a, void *ws, size_t ws_bytes, void *stream) {
+    static const char *me = "paged_plan";
+    if (check_plan(a, me) || check_ws(me, qmh_plan_ws_bytes(a), ws, ws_bytes) || on_device(me)) return -1;
+    LCHK(qmh_launch_paged_plan(a, ws, S(stream)));
+    return 0;
+}
+
+/* a mask of n nodes at most */
+static int check_mask(const char *me, const uint32_t *mask, int64_t stride, int32_t words, int64_t n) {
+    if (!mask) return 0;
+    if (!aligned(mask, 4)) return fail("%s: mask is not aligned to its words", me);
+    if (words < (n + 31) / 32 || n * words > 0x7fffffff) return fail("%s: mask_words %d of %lld nodes", me, words, (long long)n);
+    if (stride && (stride < n * words || stride > (int64_t)1 << 40)) return fail("%s: mask_stride %lld", me, (long long)stride);
+    return 0;
+}
+
+static int check_tree(const qmh_tree_args *a, const char *me) {
+    if (!a) return fail("%s: NULL arguments", me);
+    if (check_attention(&a->base, me)) return -1;
+    if (a->n_rows < 0 || a->n_rows > 1 << 20) return fail("%s: n_rows %d outside [0, 2^20]", me, a->n_rows);
+    if (!a->first && (int64_t)a->base.n_seq * a->base.q_len > a->n_rows)
+        return fail("%s: %d rows for %d sequences of %d nodes", me, a->n_rows, a->base.n_seq, a->base.q_len);
+    return check_mask(me, a->mask, a->mask_stride, a->mask_words, a->base.q_len);
+}
+
+size_t qmh_tree_attention_ws(const qmh_tree_args *a) {
+    if (check_tree(a, "tree_attention_ws") || ensure()) return 0;
+    return qmh_tree_ws_bytes(a, g_cus);
+}
+
+int qmh_tree_attention(const qmh_tree_args *a, void *ws, size_t ws_bytes, void *stream) {
+    static const char *me = "tree_attention";
+    if (check_tree(a, me) || on_device(me)) return -1;
+    if (a->base.n_seq == 0 || a->n_rows == 0) return 0;
+    if (check_ws(me, qmh_tree_ws_bytes(a, g_cus), ws, ws_bytes)) return -1;
+    LCHK(qmh_launch_tree_attention(a, g_cus, ws, S(stream)));
+    return 0;
+}
+
+static int check_logits(const qmh_logits_args *a, const char *me) {
+    if (!a) return fail("%s: NULL arguments", me);
+    const int es = elem_bytes(a->dtype);
+    if (!es) return fail("%s: bad dtype %d", me, a->dtype);
+    if (a->n_rows < 0 || a->n_rows > 1 << 20) return fail("%s: n_rows %d outside [0, 2^20]", me, a->n_rows);
+    if (a->vocab < 1 || a->vocab > 1 << 24) return fail("%s: vocab %d outside [1, 2^24]", me, a->vocab);
+    if (a->n_seq < 0 || a->n_seq > 65535) return fail("%s: n_seq %d outside [0, 65535]", me, a->n_seq);
+    if (a->rows_per_seq < 1 || a->rows_per_seq > 1 << 20) return fail("%s: rows_per_seq %d outside [1, 2^20]", me, a->rows_per_seq);
+    if (!a->first && (int64_t)a->n_seq * a->rows_per_seq > a->n_rows)
+        return fail("%s: %d rows for %d sequences of %d", me, a->n_rows, a->n_seq, a->rows_per_seq);
+    if (check_rows(me, "logits", a->logits, a->stride, a->vocab, es)) return -1;
+    if (!a->out && !a->best) return fail("%s: neither out nor best", me);
+    if (a->out && check_rows(me, "out", a->out, a->out_stride, a->vocab, es)) return -1;
+    if (a->out == a->logits && a->out_stride != a->stride) return fail("%s: out = logits needs the same stride", me);
+    if (a->history && (!a->history_len || a->history_stride < 1 || a->history_stride > 1 << 24))
+        return fail("%s: history needs history_len and a stride of 1 to 2^24", me);
+    if (a->bias && (!a->bias_token || !a->bias_len || a->bias_stride < 1 || a->bias_stride > 1 << 24))
+        return fail("%s: bias needs bias_token, bias_len and a stride of 1 to 2^24", me);
+    if (a->allow) {
+        if (!aligned(a->allow, 4) || a->allow_stride < (a->vocab + 31) / 32 || a->allow_stride > (int64_t)1 << 40)
+            return fail("%s: allow_stride %lld of %d tokens", me, (long long)a->allow_stride, a->vocab);
+        if (a->n_allow < (a->allow_row ? 0 : a->n_rows)) return fail("%s: n_allow %d", me, a->n_allow);
+    }
+    if (a->node_token) {
+        if (a->rows_per_seq > 1024) return fail("%s: trees of %d nodes (at most 1024)", me, a->rows_per_seq);
+        if (a->node_stride < a->rows_per_seq) return fail("%s: node_stride %d of %d nodes", me, a->node_stride, a->rows_per_seq);
+        return check_mask(me, a->mask, a->mask_stride, a->mask_words, a->rows_per_seq);
+    }
+    return 0;
+}
+
+size_t qmh_logits_edit_ws(const qmh_logits_args *a) {
+    if (check_logits(a, "logits_edit_ws") || ensure()) return 0;
+    return qmh_logits_ws_bytes(a, g_cus);
+}
+
+int qmh_logits_edit(const qmh_logits_args *a, void *ws, size_t ws_bytes, void *stream) {
+    static const char *me = "logits_edit";
+    if (check_logits(a, me) || on_device(me)) return -1;
+    if (a->n_seq == 0 || a->n_rows == 0) return 0;
+    if (check_ws(me, qmh_logits_ws_bytes(a, g_cus), ws, ws_bytes)) return -1;
+    LCHK(qmh_launch_logits_edit(a, g_cus, ws, S(stream)));
+    return 0;
+}
+
+int qmh_tree_accept(const qmh_accept_args *a, void *stream) {
+    static const char *me = "tree_accept";
+    if (!a) return fail("%s: NULL arguments", me);
+    if (a->n_seq < 0 || a->n_seq > 65535) return fail("%s: n_seq %d outside [0, 65535]", me, a->n_seq);
+    if (a->tree_size < 1 || a->tree_size > 1024) return fail("%s: tree_size %d outside [1, 1024]", me, a->tree_size);
+    if (!a->parent || !a->token || !a->choice || !a->len) return fail("%s: NULL parent, token, choice or len", me);
+    if ((a->parent_stride && a->parent_stride < a->tree_size) || (a->token_stride && a->token_stride < a->tree_size))
+        return fail("%s: strides %d, %d of trees of %d", me, a->parent_stride, a->token_stride, a->tree_size);
+    if (a->n_rows < 0 || a->n_rows > 1 << 20) return fail("%s: n_rows %d outside [0, 2^20]", me, a->n_rows);
+    if (!a->first && (int64_t)a->n_seq * a->tree_size > a->n_rows)
+        return fail("%s: %d rows for %d sequences of %d nodes", me, a->n_rows, a->n_seq, a->tree_size);
+    if (!a->count || !a->next || !a->keep) return fail("%s: NULL count, next or keep", me);
+    if (a->keep == a->len || a->count == a->len || a->next == a->len || a->next == a->choice || a->count == a->next || a->count == a->keep || a->next == a->keep)
+        return fail("%s: outputs overlap each other or an input", me);
+    if (a->history && (!a->history_len || a->history_stride < 1 || a->history_stride > 1 << 24))
+        return fail("%s: history needs history_len and a stride of 1 to 2^24", me);
+    if (a->pages) {
+        if (check_pages(a->pages, 1, me)) return -1;
+        if (a->n_layers < 1 || a->n_layers > 1024) return fail("%s: n_layers %d outside [1, 1024]", me, a->n_layers);
+        const int64_t pool = a->pages->n_pages * a->pages->n_kv_heads * a->pages->page_size * a->pages->head_dim; /* below 2^58 */
+        if (a->n_layers > 1 && (a->layer_stride < pool || a->layer_stride > (int64_t)1 << 46 || a->layer_stride * elem_bytes(a->pages->dtype) % 16))
+            return fail("%s: layer_stride %lld of pools of %lld elements", me, (long long)a->layer_stride, (long long)pool);
+        if (!a->table || a->table_stride < 1 || (int64_t)a->table_stride * a->pages->page_size > 0x7fffffff)
+            return fail("%s: a table of %d pages a sequence", me, a->table_stride);
+    }
+    if (on_device(me)) return -1;
+    if (a->n_seq == 0) return 0;
+    LCHK(qmh_launch_tree_accept(a, S(stream)));
+    return 0;
+}
+
 /* ------------------------------------------------------------------ device weights */
 
 struct qmh_weight {

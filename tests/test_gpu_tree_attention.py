@@ -1,0 +1,224 @@
+"""Attention of drafted trees over pages (qmh_tree_attention) against a statement in 64 bits: heads, node counts, contexts that end
+anywhere in a step, masks of any kind, values that are not finite where they are not seen, bad lengths and rows."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import _ops as o
+import _trees as tr
+
+pytestmark = pytest.mark.gpu
+
+
+def run(q, dt, H, KV, hd, ps, groups, nodes, own, prefix=None, q_len=None, ragged=True, masks="tree", static=False, seed=0, scale=None, pad=0,
+        extra_words=0, spoil=None, touch=None, gap=0, check=True):
+    """nodes, own: of each sequence, own with its nodes. Returns the outputs [rows, H, hd] and where each sequence's start."""
+    rs = np.random.default_rng(seed)
+    B, per = len(nodes), len(nodes) // groups
+    prefix = prefix or [0] * groups
+    q_len = q_len or max(max(nodes), 1)
+    scale = float(np.float32(hd ** -0.5 if scale is None else scale))
+    counts = [-(-max(n, 0) // ps) for n in prefix] + [-(-max(n, 0) // ps) for n in own]
+    tables, n_pages = o.make_tables(rs, counts, max(counts) + 1)
+    pool = [rs.standard_normal((n_pages, KV, ps, hd)) for _ in range(2)]
+    first = tr.starts(nodes) + gap
+    rows = (int(first[-1]) + 3) if ragged else B * q_len
+    if not ragged:
+        assert all(n == q_len for n in nodes)
+    x = o.encode(rs.standard_normal((rows, H * hd + pad)) * 1.5, dt)
+    words = -(-q_len // 32) + extra_words
+    see = np.zeros((B, q_len, q_len), bool)
+    for i in range(1 if static else B):
+        if masks == "tree":
+            see[i] = tr.ancestors(tr.tree(rs, q_len))
+        elif masks == "chain":
+            see[i] = np.tril(np.ones((q_len, q_len), bool))
+        elif masks == "random":
+            see[i] = rs.random((q_len, q_len)) < 0.4
+        elif masks == "none":
+            see[i] = False
+    if static:
+        see[:] = see[0]
+    packed = tr.pack(see[:1] if static else see, words, rs)
+    if touch:
+        touch(pool, tables[groups:], own, nodes, see)
+    k, v = (o.encode(y, dt) for y in pool)
+    prefix, own, bad = list(prefix), list(own), np.zeros(B, bool)
+    if spoil:
+        spoil(tables[groups:], own, first, bad)
+    dk, dv, dx, dout = o.Guarded(q, k), o.Guarded(q, v), o.Guarded(q, x), o.Guarded(q, np.full((rows, H * hd + pad), 0x55, o.raw(dt)))
+    dev = q.DeviceBuffer.from_array
+    keep = [dev(a) for a in (tables[groups:], np.array(own, np.int32), tables[:groups], np.array(prefix, np.int32), first, packed)]
+    pages = q.Pages(dtype=dt, n_kv_heads=KV, head_dim=hd, page_size=ps, n_pages=n_pages, k=dk.ptr, v=dv.ptr)
+    cap = tables.shape[1] * ps
+    base = q.AttentionArgs(pages=ctypes.pointer(pages), n_heads=H, n_seq=B, q_len=q_len, n_groups=groups, q=dx.ptr, q_stride=H * hd + pad,
+                           out=dout.ptr, out_stride=H * hd + pad, table=keep[0].ptr, len=keep[1].ptr, table_stride=tables.shape[1],
+                           max_len=min(max(max(own), 0), cap), prefix_table=keep[2].ptr, prefix_len=keep[3].ptr, prefix_stride=tables.shape[1],
+                           max_prefix=max(prefix), scale=scale)
+    a = q.TreeArgs(base=base, n_rows=rows, first=keep[4].ptr if ragged else None, mask=None if masks == "chain" else keep[5].ptr,
+                   mask_stride=0 if static else q_len * words, mask_words=words)
+    L = q.load_library()
+    need = L.qmh_tree_attention_ws(ctypes.byref(a))
+    ws = o.Guarded(q, np.zeros(max(need, 16), np.uint8), pad=4096)
+    q._check(L.qmh_tree_attention(ctypes.byref(a), ws.ptr, need, None), "tree_attention")
+    q.sync()
+    ws.get()
+    full = dout.get()
+    for d in (dk, dv, dx):
+        assert d.get().tobytes() == d.like.tobytes()
+    if pad:
+        assert (full[:, H * hd:] == 0x55).all()
+    got = o.decode(full[:, :H * hd], dt).reshape(rows, H, hd)
+    if not check:
+        return got, first
+    xv = o.decode(x, dt)[:, :H * hd].reshape(rows, H, hd)
+    kv_, vv = o.decode(k, dt), o.decode(v, dt)
+    at = first if ragged else np.arange(B + 1) * q_len
+    untouched = full[:, :H * hd] == 0x55
+    assert untouched[:at[0]].all() and untouched[at[-1]:].all(), "rows that are nobody's"
+    for i, n in enumerate(nodes):
+        g = i // per
+        if bad[i]:
+            assert np.isnan(got[at[i]:at[i] + n]).all(), f"sequence {i}: NaN"
+            continue
+        pk, pv = (o.rows_of(y, tables[g], prefix[g], ps) for y in (kv_, vv))
+        ok, ov = (o.rows_of(y, tables[groups + i], own[i], ps) for y in (kv_, vv))
+        for j in range(n):
+            t = np.concatenate([np.ones(own[i] - n, bool), see[i, j, :n]])
+            kk, ww = np.concatenate([pk, ok[t]]), np.concatenate([pv, ov[t]])
+            want, mag, reach = o.attention(xv[at[i] + j], kk, ww, scale)
+            # as for consecutive queries: scores of hd products, exponentials to 2 steps, sums of n terms, 16-bit
+            # probabilities rounded to the type, then the result
+            ds = (hd + 4) * o.U32 * reach + 4 * o.U32
+            with np.errstate(invalid="ignore"):
+                tol = mag * (2 * ds + (len(kk) + 64) * o.U32 + (o.HALF[dt] if dt != o.F32 else 0)) * 1.01
+                tol = tol + o.HALF[dt] * np.abs(want) + o.TINY[dt]
+                if dt == o.F16:
+                    tol = tol + len(kk) * o.TINY[dt] * np.abs(np.nan_to_num(ww, posinf=0, neginf=0)).max(initial=0)
+            row = got[at[i] + j]
+            if dt != o.F16 and len(ww) and np.nan_to_num(np.abs(ww), nan=0, posinf=0).max() > 2.0 ** 112:
+                # weights are up to 2^15 before they are divided by their sum: 2^15 times such a value passes 32 bits (2^128)
+                assert (np.isfinite(row) | (np.sign(row) == np.sign(want))).all()
+                row = np.where(np.isfinite(row), row, want)
+            o.close(row, want, tol, f"sequence {i} node {j} of {n} ({own[i]} own, {prefix[g]} shared)")
+    return got, at
+
+
+SHAPES = [(6, 2, 48), (12, 12, 64), (32, 4, 64), (3, 3, 128), (5, 1, 80), (14, 2, 96), (2, 1, 8), (4, 2, 256), (1, 1, 136), (40, 1, 32)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd", SHAPES)
+def test_heads(gpu, dtype, H, KV, hd):
+    run(gpu, o.TYPES[dtype], H, KV, hd, 16, 2, [5, 1, 9, 7, 0, 12], [70, 33, 9, 40, 5, 13], prefix=[40, 7], seed=hd)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 2, 17, 31, 32, 33, 63, 64, 65, 100, 129])
+def test_node_counts(gpu, dtype, n):
+    run(gpu, o.TYPES[dtype], 4, 2, 64, 32, 3, [n, n, n], [n, n + 1, n + 200], ragged=False, seed=n)
+    run(gpu, o.TYPES[dtype], 2, 2, 128, 16, 1, [n, max(n // 2, 1), n - 1], [n + 45, n + 30, n + 7], seed=n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("masks", ["tree", "random"])
+def test_contexts_that_end_anywhere(gpu, dtype, masks):
+    nodes = [1 + (7 * c) % 40 for c in range(48)]
+    run(gpu, o.TYPES[dtype], 2, 1, 32, 16, 48, nodes, [c + n for c, n in zip(range(48), nodes)], q_len=45, masks=masks, extra_words=1, seed=5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("groups,nodes,own,prefix", [
+    (1, [3], [3], [0]), (1, [3], [1000], [1500]), (2, [33, 20, 40, 1], [50, 2000, 900, 1], [700, 0]), (1, [70], [3100], [0]),
+    (1, [8] * 20, list(range(8, 28)), [513])])
+def test_lengths(gpu, dtype, groups, nodes, own, prefix):
+    run(gpu, o.TYPES[dtype], 8, 2, 64, 64, groups, nodes, own, prefix=prefix, pad=64, seed=len(nodes))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_long_tree(gpu, dtype):
+    run(gpu, o.TYPES[dtype], 2, 1, 64, 16, 1, [1000], [1100], seed=3)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("static", [False, True])
+def test_masks_of_any_kind(gpu, dtype, static):
+    for masks in ("random", "tree", "chain"):
+        run(gpu, o.TYPES[dtype], 4, 2, 64, 16, 2, [37, 40, 1, 12], [37, 90, 64, 12], prefix=[0, 33], q_len=40, masks=masks, static=static, seed=9)
+    # nothing of the tree is seen: the context alone, or zeros
+    got, at = run(gpu, o.TYPES[dtype], 4, 2, 64, 16, 2, [37, 3], [37, 50], masks="none", static=static, seed=10)
+    assert (got[:37] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_what_is_not_seen_has_no_effect(gpu, dtype, hd):
+    """Keys and values of some nodes are infinite or NaN: other branches of the tree do not notice."""
+    for value in (np.inf, -np.inf, np.nan):
+        for where in (0, 1):
+            def touch(pool, table, own, nodes, see):
+                for i, n in enumerate(nodes):
+                    for k in range(3, n, 5):
+                        t = own[i] - n + k
+                        pool[where][table[i][t // 16], :, t % 16, (3 * k) % hd] = value
+            run(gpu, o.TYPES[dtype], 2, 1, hd, 16, 1, [36, 9], [70, 9], touch=touch, seed=hd)
+    # the type's largest numbers are finite
+    big = {"f32": 3e38, "f16": 65504.0, "bf16": 3e38}[dtype]
+
+    def large(pool, table, own, nodes, see):
+        t = own[0] - nodes[0] + 2
+        pool[1][table[0][t // 16], :, t % 16] = -big
+    run(gpu, o.TYPES[dtype], 2, 1, hd, 16, 1, [20], [60], touch=large, seed=1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bad_lengths_and_pages_give_nan(gpu, dtype):
+    def spoil(table, own, first, bad):
+        own[0], own[1] = 4, -7  # fewer than the nodes
+        table[2, 0] = -5
+        bad[:3] = True
+    run(gpu, o.TYPES[dtype], 4, 2, 64, 16, 5, [5, 5, 5, 5, 5], [20, 20, 20, 20, 20], spoil=spoil, seed=4)
+
+
+@pytest.mark.parametrize("first", [[0, 4, 3, 8], [0, 4, 40, 8], [-1, 4, 6, 8], [0, 7, 9, 2 ** 31 - 1], [2, 4, 6, 12]])
+def test_bad_rows_are_left_out(gpu, first):
+    """Rows that run backwards, behind the arrays or past the most nodes: nothing outside the arrays is touched (the guards of
+    run), and sequences with good rows of their own have them."""
+    def spoil(table, own, at, bad):
+        at[:] = first
+    got, _ = run(gpu, o.F32, 2, 2, 64, 16, 3, [4, 2, 2], [20, 20, 20], q_len=5, spoil=spoil, check=False, seed=6)
+    assert got.shape[0] == 11
+
+
+def test_rows_that_start_behind_others(gpu):
+    run(gpu, o.F16, 4, 2, 64, 16, 1, [3, 0, 5], [300, 20, 5], prefix=[700], gap=4, seed=11)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd,q_len,own", [(4, 2, 64, 3, 300), (2, 2, 128, 1, 2000), (8, 1, 32, 20, 57)])
+def test_a_chain_is_what_consecutive_queries_are(gpu, dtype, H, KV, hd, q_len, own):
+    """With one call's mask a chain, the result is that of qmh_paged_attention, to the bit."""
+    q, L, dt, rs = gpu, gpu.load_library(), o.TYPES[dtype], np.random.default_rng(3)
+    tables, n_pages = o.make_tables(rs, [-(-own // 16)] * 2, -(-own // 16))
+    k, v = (q.DeviceBuffer.from_array(o.encode(rs.standard_normal((n_pages, KV, 16, hd)), dt)) for _ in range(2))
+    x = q.DeviceBuffer.from_array(o.encode(rs.standard_normal((2 * q_len, H * hd)), dt))
+    out = [q.DeviceBuffer(2 * q_len * H * hd * o.BYTES[dt]) for _ in range(2)]
+    tab, n = q.DeviceBuffer.from_array(tables), q.DeviceBuffer.from_array(np.array([own, own - 1], np.int32))
+    words = -(-q_len // 32)
+    mask = q.DeviceBuffer.from_array(tr.pack(np.tril(np.ones((q_len, q_len), bool)), words))
+    pages = q.Pages(dtype=dt, n_kv_heads=KV, head_dim=hd, page_size=16, n_pages=n_pages, k=k.ptr, v=v.ptr)
+    base = q.AttentionArgs(pages=ctypes.pointer(pages), n_heads=H, n_seq=2, q_len=q_len, n_groups=2, q=x.ptr, q_stride=H * hd, out=out[0].ptr,
+                           out_stride=H * hd, table=tab.ptr, len=n.ptr, table_stride=tables.shape[1], max_len=own, scale=0.2)
+    need = L.qmh_paged_attention_ws(ctypes.byref(base))
+    ws = q.DeviceBuffer(max(need, 16))
+    q._check(L.qmh_paged_attention(ctypes.byref(base), ws.ptr, need, None), "paged")
+    q.sync()
+    want = out[0].to_array(o.raw(dt))
+    for m in (None, mask.ptr):
+        base.out = out[1].ptr
+        a = q.TreeArgs(base=base, n_rows=2 * q_len, mask=m, mask_words=words)
+        assert L.qmh_tree_attention_ws(ctypes.byref(a)) == need
+        q._check(L.qmh_tree_attention(ctypes.byref(a), ws.ptr, need, None), "tree")
+        q.sync()
+        assert np.array_equal(out[1].to_array(o.raw(dt)), want)
