@@ -14,7 +14,7 @@ namespace {
 // them (where they go elsewhere), puts -inf where the grammar forbids a token, and finds the best of the tokens that are
 // not hot; it is left out where there is nothing of it to do, and vectors that stay as they are, or are forbidden as a whole,
 // are not read. A sparse pass edits the hot ones: they are few, so their divisions and gathers do not weigh.
-constexpr int SEG = 4096;
+constexpr int SEG = 4096, NT = 512;
 constexpr int ROWS = 32; // of a workgroup, at most
 constexpr uint32_t PROMPT = 1u << 31, NODE = 1u << 30; // beside a count of outputs: in the prompt; a node's token
 
@@ -35,6 +35,11 @@ __device__ __forceinline__ float element(v4u x, int e) {
     else return qmh_to_f(__builtin_bit_cast(T, (uint16_t)(e & 1 ? x[e / 2] >> 16 : x[e / 2])));
 }
 
+// x where the mask is all ones, -inf where it is 0
+__device__ __forceinline__ float choose(int mask, float x) {
+    return __uint_as_float((__float_as_uint(x) & (uint32_t)mask) | (0xff800000u & ~(uint32_t)mask));
+}
+
 // the rows of sequence sq: t0 to t0 + the result, 0 where they are none
 __device__ __forceinline__ int logits_rows(const qmh_logits_args &a, int sq, int &t0) {
     if (!a.first) {
@@ -47,155 +52,259 @@ __device__ __forceinline__ int logits_rows(const qmh_logits_args &a, int sq, int
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_logits_edit(const qmh_logits_args a, int segs, int chunks, int chunk, uint32_t first_block, uint64_t *keys) {
-    constexpr int N = 16 / (int)sizeof(T); // tokens of a vector
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void k_logits_edit(const qmh_logits_args a, int segs, int chunks, int chunk, uint32_t first_block, uint64_t *keys) {
+    constexpr int N = 16 / (int)sizeof(T);     // tokens of a vector
+    constexpr int VB = 4, PIECE = VB * 64 * N; // vectors of a lane, tokens of a wave at a time
     constexpr uint32_t ALL = (1u << N) - 1;
     __shared__ __align__(16) uint32_t count[SEG], bias_at[SEG];
     __shared__ uint16_t hot[SEG];
-    __shared__ uint64_t hot_bits[SEG / 64], row_key[ROWS];
-    __shared__ int node[1024];
+    __shared__ __align__(16) uint8_t hot_bits[SEG / 4]; // four tokens a byte
+    __shared__ uint64_t row_key[ROWS];
+    __shared__ int row_allow[ROWS], node[1024];
     __shared__ int n_hot;
     const uint32_t b = blockIdx.x + first_block, unit = b / chunks, sq = unit / segs;
-    const int seg = unit - sq * segs, tid = threadIdx.x, lane = tid & 63;
+    const int seg = unit - sq * segs, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int t0;
     const int n = logits_rows(a, sq, t0), r0 = (int)(b - unit * chunks) * chunk, r1 = min(r0 + chunk, n);
     if (r0 >= n) return;
     const int v0 = seg * SEG, vn = min(SEG, a.vocab - v0); // the segment's tokens
     const float rep = a.repetition ? a.repetition[sq] : 1.0f, by = rep > 0.0f ? rep : 1.0f;
     const float presence = a.presence ? a.presence[sq] : 0.0f, frequency = a.frequency ? a.frequency[sq] : 0.0f;
+    const int said = a.history ? a.history_len[sq] : 0, prompt = a.prompt_len ? a.prompt_len[sq] : 0, biased = a.bias ? a.bias_len[sq] : 0;
     const bool penal = by != 1.0f || presence != 0.0f || frequency != 0.0f;
     const int n_node = penal && a.node_token ? n : 0;
+    const bool inplace = a.out == a.logits, all_read = a.best || (a.out && !inplace);
+
+    // Pieces of rows, dealt out to the waves. A wave's first one is loaded while the history is counted.
+    const bool whole = vn == SEG;
+    const int pieces = whole ? SEG / PIECE : (vn + PIECE - 1) / PIECE, tasks = (r1 - r0) * pieces;
+    v4u x[VB];
+    const uint32_t *ok;
+    uint32_t words[VB];
+    auto fetch = [&](int task) {
+        const int row = task / pieces, p0 = (task - row * pieces) * PIECE + lane * N;
+        ok = nullptr;
+        if (a.allow) {
+            const int ar = a.allow_row ? a.allow_row[t0 + r0 + row] : t0 + r0 + row;
+            if (ar >= 0 && ar < a.n_allow) ok = a.allow + ar * a.allow_stride + (v0 >> 5);
+        }
+        if (ok)
+#pragma unroll
+            for (int k = 0; k < VB; k++)
+                if (p0 + k * 64 * N < vn) words[k] = ok[(p0 + k * 64 * N) >> 5];
+        if (!all_read) return;
+        const T *from = (const T *)a.logits + (t0 + r0 + row) * a.stride + v0 + p0;
+        if (whole) {
+#pragma unroll
+            for (int k = 0; k < VB; k++) x[k] = ((const v4u_any *)(from + k * 64 * N))->v;
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < VB; k++)
+            if (p0 + k * 64 * N + N <= vn) x[k] = ((const v4u_any *)(from + k * 64 * N))->v;
+        const int k = (vn - p0) / (64 * N), left = (vn - p0) % (64 * N); // the vocabulary's last tokens, where they fill no vector
+        if (vn > p0 && k < VB && left < N) {
+            qmh_vec<T, N> e = {};
+#pragma unroll
+            for (int i = 0; i < N - 1; i++)
+                if (i < left) e.e[i] = from[k * 64 * N + i];
+#pragma unroll
+            for (int q = 0; q < VB; q++)
+                if (q == k) x[q] = __builtin_bit_cast(v4u, e);
+        }
+    };
+    if (w < tasks) fetch(w);
+    // so are the lists' first tokens
+    constexpr int HB = 4;
+    const int h = penal && said > 0 ? (int)min((int64_t)said, a.history_stride) : 0, nb = min(biased, a.bias_stride);
+    const int32_t *hist = a.history + sq * a.history_stride, *biases = a.bias_token + (int64_t)sq * a.bias_stride;
+    int early[HB];
+#pragma unroll
+    for (int k = 0; k < HB; k++) early[k] = tid + k * NT < h ? hist[tid + k * NT] : -1;
+    const int early_bias = tid < nb ? biases[tid] : -1, early_node = tid < n_node ? a.node_token[(int64_t)sq * a.node_stride + tid] : -1;
 
     // ---- what is touched
-    for (int i = tid; i < SEG; i += 256) count[i] = bias_at[i] = 0;
-    if (tid < ROWS) row_key[tid] = 0;
+    for (int i = tid; i < SEG / 4; i += NT) ((v4u *)count)[i] = ((v4u *)bias_at)[i] = (v4u){0, 0, 0, 0};
+    if (tid < ROWS) {
+        row_key[tid] = 0;
+        const int r = r0 + tid;
+        int row = -1;
+        if (a.allow && r < r1) row = a.allow_row ? a.allow_row[t0 + r] : t0 + r;
+        row_allow[tid] = row < a.n_allow ? row : -1;
+    }
     if (tid == 0) n_hot = 0;
     __syncthreads();
-    if (penal && a.history) {
-        const int64_t len = max(0, a.history_len[sq]);
-        const int h = (int)min(len, a.history_stride), prompt = a.prompt_len ? a.prompt_len[sq] : 0;
-        const int32_t *hist = a.history + sq * a.history_stride;
-        for (int i = tid; i < h; i += 256) {
-            const uint32_t e = (uint32_t)(hist[i] - v0);
-            if (hist[i] < 0 || e >= (uint32_t)vn) continue;
-            if (i < prompt) atomicOr(&count[e], PROMPT);
-            else atomicAdd(&count[e], 1u);
-        }
+    auto told = [&](int t, int i) { // token t, the history's i-th
+        const uint32_t e = (uint32_t)(t - v0);
+        if (t < 0 || e >= (uint32_t)vn) return;
+        if (i < prompt) atomicOr(&count[e], PROMPT);
+        else atomicAdd(&count[e], 1u);
+    };
+#pragma unroll
+    for (int k = 0; k < HB; k++) told(early[k], tid + k * NT);
+    for (int i0 = tid + HB * NT; i0 < h; i0 += HB * NT) {
+        int t[HB];
+#pragma unroll
+        for (int k = 0; k < HB; k++) t[k] = i0 + k * NT < h ? hist[i0 + k * NT] : -1;
+#pragma unroll
+        for (int k = 0; k < HB; k++) told(t[k], i0 + k * NT);
     }
-    for (int k = tid; k < n_node; k += 256) {
-        const int t = a.node_token[(int64_t)sq * a.node_stride + k];
+    for (int k = tid; k < n_node; k += NT) {
+        const int t = k == tid ? early_node : a.node_token[(int64_t)sq * a.node_stride + k];
         const uint32_t e = (uint32_t)(t - v0);
         node[k] = t;
         if (t >= 0 && e < (uint32_t)vn) atomicOr(&count[e], NODE);
     }
-    if (a.bias) {
-        const int nb = min(max(0, a.bias_len[sq]), a.bias_stride);
-        for (int i = tid; i < nb; i += 256) {
-            const int t = a.bias_token[(int64_t)sq * a.bias_stride + i];
-            const uint32_t e = (uint32_t)(t - v0);
-            if (t >= 0 && e < (uint32_t)vn) atomicMax(&bias_at[e], (uint32_t)i + 1);
-        }
+    for (int i = tid; i < nb; i += NT) {
+        const int t = i == tid ? early_bias : biases[i];
+        const uint32_t e = (uint32_t)(t - v0);
+        if (t >= 0 && e < (uint32_t)vn) atomicMax(&bias_at[e], (uint32_t)i + 1);
     }
     __syncthreads();
-    for (int e = tid; e < SEG; e += 256) {
-        const bool is = count[e] || bias_at[e];
-        const uint64_t all = __ballot(is);
-        int at = 0;
-        if (lane == 0) {
-            hot_bits[e / 64] = all;
-            if (all) at = atomicAdd(&n_hot, __popcll(all));
+    { // a thread looks at four tokens at a time, a wave lists the hot ones of its share with one atomic
+        constexpr int Q = SEG / (4 * NT);
+        uint64_t is[Q][4];
+        int mine = 0;
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            v4u c = ((v4u *)count)[q * NT + tid];
+            if (biased > 0) c |= ((v4u *)bias_at)[q * NT + tid];
+            uint32_t byte = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                is[q][j] = __ballot(c[j] != 0);
+                mine += __popcll(is[q][j]);
+                byte |= c[j] ? 1u << j : 0u;
+            }
+            hot_bits[q * NT + tid] = (uint8_t)byte;
         }
-        at = __shfl(at, 0);
-        if (is) hot[at + __popcll(all & ((1ull << lane) - 1))] = (uint16_t)e;
+        int at = 0;
+        if (lane == 0 && mine) at = atomicAdd(&n_hot, mine);
+        at = __builtin_amdgcn_readfirstlane(at);
+        if (mine)
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if ((is[q][j] >> lane) & 1)
+                        hot[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(is[q][j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)is[q][j], 0))] =
+                            (uint16_t)(4 * (q * NT + tid) + j);
+                    at += __popcll(is[q][j]);
+                }
     }
     __syncthreads();
 
     // ---- the rows
-    const bool inplace = a.out == a.logits;
-    auto grammar = [&](int r) -> const uint32_t * {
-        if (!a.allow) return nullptr;
-        const int row = a.allow_row ? a.allow_row[t0 + r] : t0 + r;
-        return row < 0 || row >= a.n_allow ? nullptr : a.allow + row * a.allow_stride;
-    };
-    for (int r = r0; r < r1; r++) {
-        const uint32_t *ok = grammar(r);
-        if (!a.best && (!a.out || inplace) && !ok) continue;
-        const T *x = (const T *)a.logits + (t0 + r) * a.stride + v0;
-        T *y = a.out ? (T *)a.out + (t0 + r) * a.out_stride + v0 : nullptr;
-        float best = -__builtin_inff();
-        int best_at = 0;
-        uint32_t best_may = 0;
-        v4u best_v = {0, 0, 0, 0};
-        for (int t = tid * N; t < vn; t += 256 * N) {
-            const int left = vn - t;
-            const uint32_t here = left >= N ? ALL : (1u << left) - 1;
-            uint32_t may = here;
-            if (ok) may &= ok[(v0 + t) >> 5] >> (t & 31);
-            if (!a.best && inplace && may == here) continue;
-            v4u v = {0, 0, 0, 0};
-            if (left >= N) {
-                if (a.best || may) v = ((const v4u_any *)(x + t))->v;
-            } else {
-                qmh_vec<T, N> e = {};
+    for (int task = w; task < tasks; task += NT / 64) {
+        const int row = task / pieces, r = r0 + row, p0 = (task - row * pieces) * PIECE + lane * N;
+        if (task != w) fetch(task);
+        if (!all_read && !ok) continue;
+        uint32_t may[VB];
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (i < left) e.e[i] = x[t + i];
-                v = __builtin_bit_cast(v4u, e);
-            }
-            if (a.best) {
-                const uint32_t eff = may & ~(uint32_t)(hot_bits[t / 64] >> (t & 63));
-                float m = -__builtin_inff();
-#pragma unroll
-                for (int e = 0; e < N; e++) m = fmaxf(m, (eff >> e) & 1 ? element<T>(v, e) : -__builtin_inff());
-                if (m > best) {
-                    best = m;
-                    best_at = t;
-                    best_may = eff;
-                    best_v = v;
-                }
-            }
-            if (!y || (inplace && may == here)) continue;
-            qmh_vec<T, N> e = __builtin_bit_cast(qmh_vec<T, N>, v);
-#pragma unroll
-            for (int i = 0; i < N; i++)
-                if (!((may >> i) & 1)) e.e[i] = (T)-__builtin_inff();
-            if (left >= N) ((v4u_any *)(y + t))->v = __builtin_bit_cast(v4u, e);
-            else
-#pragma unroll
-                for (int i = 0; i < N; i++)
-                    if (i < left) y[t + i] = e.e[i];
+        for (int k = 0; k < VB; k++) {
+            const int t = p0 + k * 64 * N;
+            may[k] = ALL;
+            if (!whole) may[k] = vn - t >= N ? ALL : vn > t ? (1u << (vn - t)) - 1 : 0u;
+            if (ok && t < vn) may[k] &= words[k] >> (t & 31);
         }
         if (a.best) {
-            const float top = qmh_wave_max(best);
-            if (best == top && best > -__builtin_inff()) { // mostly one lane
-                int at = 0;
+            float best = -__builtin_inff();
+            int at = 0;
+            uint32_t eff[VB];
 #pragma unroll
-                for (int e = N - 1; e >= 0; e--)
-                    if ((best_may >> e) & 1 && element<T>(best_v, e) == best) at = e;
-                atomicMax((unsigned long long *)&row_key[r - r0], (unsigned long long)best_key(best, v0 + best_at + at));
+            for (int k = 0; k < VB; k++) {
+                const int t = p0 + k * 64 * N;
+                uint32_t hots = hot_bits[t / 4];
+                if constexpr (N == 8) hots |= (uint32_t)hot_bits[t / 4 + 1] << 4;
+                eff[k] = may[k] & ~hots;
+                float m = -__builtin_inff();
+#pragma unroll
+                for (int e = 0; e < N; e++) // a bit as a mask chooses the element or -inf
+                    m = fmaxf(m, choose((int)(eff[k] << (31 - e)) >> 31, element<T>(x[k], e)));
+                if (m > best) {
+                    best = m;
+                    at = k;
+                }
+            }
+            const float top = qmh_wave_max(best); // every lane takes part
+            if (best == top && best > -__builtin_inff()) { // mostly one lane
+                uint32_t same = 0;
+#pragma unroll
+                for (int k = 0; k < VB; k++)
+                    if (at == k)
+#pragma unroll
+                        for (int e = 0; e < N; e++) same |= element<T>(x[k], e) == best ? eff[k] & 1u << e : 0u;
+                const int t = v0 + p0 + at * 64 * N + __builtin_ctz(same);
+                atomicMax((unsigned long long *)&row_key[row], (unsigned long long)best_key(best, t));
+            }
+        }
+        if (!a.out) continue;
+        const T *from = (const T *)a.logits + (t0 + r) * a.stride + v0 + p0;
+        T *to = (T *)a.out + (t0 + r) * a.out_stride + v0 + p0;
+#pragma unroll
+        for (int k = 0; k < VB; k++) {
+            const int left = vn - p0 - k * 64 * N;
+            if (inplace && may[k] == ALL) continue;
+            if (whole || left >= N) {
+                v4u v = {0, 0, 0, 0};
+                if (all_read) v = x[k];
+                else if (may[k]) v = ((const v4u_any *)(from + k * 64 * N))->v; // of what is forbidden as a whole nothing is read
+                qmh_vec<T, N> e = __builtin_bit_cast(qmh_vec<T, N>, v);
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (!((may[k] >> i) & 1)) e.e[i] = (T)-__builtin_inff();
+                ((v4u_any *)(to + k * 64 * N))->v = __builtin_bit_cast(v4u, e);
+            } else {
+                for (int i = 0; i < left; i++)
+                    if (!(inplace && (may[k] >> i) & 1)) to[k * 64 * N + i] = (may[k] >> i) & 1 ? from[k * 64 * N + i] : (T)-__builtin_inff();
             }
         }
     }
-    __syncthreads(); // the hot tokens' places are written again
+    __syncthreads(); // the hot tokens' places are written again, and what the rows hold is known
 
-    // ---- the hot tokens
+    // ---- the hot tokens: one a thread, four rows at a time
     const int hots = n_hot;
-    for (int i = tid; i < hots * (r1 - r0); i += 256) {
-        const int r = r0 + i / hots, e = hot[i % hots], t = v0 + e;
-        const uint32_t *ok = grammar(r);
-        if (ok && !((ok[t >> 5] >> (t & 31)) & 1)) continue;
-        uint32_t c = count[e], m = c & (NODE - 1);
-        if (c & NODE) {
-            const uint32_t *see = a.mask ? a.mask + sq * a.mask_stride + (int64_t)r * a.mask_words : nullptr;
-            for (int k = 0; k < n_node; k++)
-                if (node[k] == t && (see ? (see[k >> 5] >> (k & 31)) & 1 : k <= r)) m++;
+    for (int i = tid; i < hots; i += NT) {
+        const int e = hot[i], t = v0 + e;
+        const uint32_t c = count[e], ba = bias_at[e];
+        const float bias = ba ? a.bias[(int64_t)sq * a.bias_stride + ba - 1] : 0.0f;
+        for (int ra = r0; ra < r1; ra += 4) {
+            T v[4];
+            uint32_t may[4], path[4] = {0, 0, 0, 0}; // how often the rows' own paths have the token
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int r = min(ra + k, r1 - 1), ar = row_allow[r - r0];
+                v[k] = ((const T *)a.logits)[(t0 + r) * a.stride + t];
+                may[k] = ar < 0 ? ~0u : a.allow[ar * a.allow_stride + (t >> 5)];
+            }
+            if (c & NODE)
+                for (int q0 = 0; q0 < n_node; q0 += 32) {
+                    uint32_t at = 0; // which of 32 nodes have it
+                    for (int q = 0; q < 32 && q0 + q < n_node; q++) at |= (uint32_t)(node[q0 + q] == t) << q;
+                    if (!at) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int r = min(ra + k, r1 - 1), chain = r + 1 - q0;
+                        const uint32_t see = a.mask ? a.mask[sq * a.mask_stride + (int64_t)r * a.mask_words + (q0 >> 5)]
+                                                    : chain >= 32 ? ~0u : chain <= 0 ? 0u : (1u << chain) - 1;
+                        path[k] += __popc(at & see);
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int r = ra + k;
+                if (r >= r1 || !((may[k] >> (t & 31)) & 1)) continue;
+                const uint32_t m = (c & (NODE - 1)) + path[k];
+                float y = qmh_to_f(v[k]);
+                if (m || c & PROMPT) y = y > 0.0f ? y / by : y * by;
+                if (m) y -= frequency * (float)m + presence;
+                if (ba) y += bias;
+                if (a.out) ((T *)a.out)[(t0 + r) * a.out_stride + t] = (T)y;
+                if (!a.best) continue;
+                const uint64_t key = y > -__builtin_inff() ? best_key(y, t) : 0;
+                if (key > row_key[r - r0]) atomicMax((unsigned long long *)&row_key[r - r0], (unsigned long long)key); // few are
+            }
         }
-        float x = qmh_to_f(((const T *)a.logits)[(t0 + r) * a.stride + t]);
-        if (m || c & PROMPT) x = x > 0.0f ? x / by : x * by;
-        if (m) x -= frequency * (float)m + presence;
-        if (bias_at[e]) x += a.bias[(int64_t)sq * a.bias_stride + bias_at[e] - 1];
-        if (a.out) ((T *)a.out)[(t0 + r) * a.out_stride + t] = (T)x;
-        if (a.best && x > -__builtin_inff()) atomicMax((unsigned long long *)&row_key[r - r0], (unsigned long long)best_key(x, t));
     }
     if (!a.best) return;
     __syncthreads();
@@ -206,12 +315,12 @@ __global__ __launch_bounds__(256) void k_logits_edit(const qmh_logits_args a, in
     }
 }
 
-// a row's best over its segments: a wave a row, a workgroup a sequence
+// a row's best over its segments: a wave a row
 __global__ __launch_bounds__(256) void k_logits_best(const qmh_logits_args a, int segs, const uint64_t *keys) {
     const int lane = threadIdx.x & 63;
     int t0;
     const int n = logits_rows(a, blockIdx.x, t0);
-    for (int r = threadIdx.x >> 6; r < n; r += 4) {
+    for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < n; r += gridDim.y * 4) {
         uint64_t key = 0;
         for (int s = lane; s < segs; s += 64) key = max(key, keys[(int64_t)(t0 + r) * segs + s]);
 #pragma unroll
@@ -233,9 +342,9 @@ extern "C" int qmh_launch_logits_edit(const qmh_logits_args *a, int cus, void *w
     hipStream_t st = (hipStream_t)stream;
     const int segs = segments(a);
     const int64_t units = (int64_t)a->n_seq * segs;
-    // rows of a workgroup: as many as leave about four workgroups a CU, which count the history again each
+    // rows of a workgroup: as few as fill the chip's workgroups once (three a CU); each counts the history again
     int most = a->rows_per_seq < a->n_rows ? a->rows_per_seq : a->n_rows;
-    int chunks = (int)((4 * cus + units - 1) / units);
+    int chunks = units < 3 * cus ? (int)(3 * cus / units) : 1;
     chunks = chunks < most ? chunks : most;
     if (chunks < (most + ROWS - 1) / ROWS) chunks = (most + ROWS - 1) / ROWS;
     const int chunk = (most + chunks - 1) / chunks;
@@ -246,9 +355,9 @@ extern "C" int qmh_launch_logits_edit(const qmh_logits_args *a, int cus, void *w
         using T = decltype(z);
         for (int64_t b0 = 0; b0 < blocks; b0 += QMH_MOST_BLOCKS) { // workgroups write different places: any number of launches
             const dim3 g((uint32_t)(blocks - b0 < QMH_MOST_BLOCKS ? blocks - b0 : QMH_MOST_BLOCKS));
-            hipLaunchKernelGGL((k_logits_edit<T>), g, dim3(256), 0, st, *a, segs, chunks, chunk, (uint32_t)b0, (uint64_t *)ws);
+            hipLaunchKernelGGL((k_logits_edit<T>), g, dim3(NT), 0, st, *a, segs, chunks, chunk, (uint32_t)b0, (uint64_t *)ws);
         }
     });
-    if (a->best && segs > 1) hipLaunchKernelGGL(k_logits_best, dim3(a->n_seq), dim3(256), 0, st, *a, segs, (const uint64_t *)ws);
+    if (a->best && segs > 1) hipLaunchKernelGGL(k_logits_best, dim3(a->n_seq, most < 4 * 60 ? (most + 3) / 4 : 60), dim3(256), 0, st, *a, segs, (const uint64_t *)ws);
     return (int)hipGetLastError();
 }
