@@ -343,64 +343,6 @@ struct attn_wave {
         }
     }
 
-    // Trees: a node that a row does not see must not reach it, whatever its values hold, but a product with 0 makes NaN of
-    // one that is not finite. Where a step that some row does not see all of has such values, they are added one by one
-    // to the rows that do see them and taken out of the product.
-    static constexpr uint32_t EXP = F ? 0x7f800000u : std::is_same<T, qmh_f16>::value ? 0x7c00u : 0x7f80u; // all ones: not finite
-    __device__ __forceinline__ void odd_values(const v4u (&P)[NR], float *area) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
-        uint32_t lo = 0, hi = 0; // the largest exponents
-#pragma unroll
-        for (int j = 0; j < 4 * RT; j++)
-#pragma unroll
-            for (int u = 0; u < VW; u++) {
-                lo = max(lo, v[j][u] & EXP);
-                if constexpr (!F) hi = max(hi, v[j][u] & EXP << 16);
-            }
-        if (!__any(lo == EXP || (!F && hi == EXP << 16))) return;
-        T *rows = (T *)area; // [KS][HDP], of this wave alone: 16 NR rows of LDS_COL floats hold it
-#pragma unroll
-        for (int j = 0; j < 4 * RT; j++)
-#pragma unroll
-            for (int u = 0; u < VW; u++) ((uint32_t *)(rows + (16 * (j / 4) + 4 * g + j % 4) * HDP + i * VE))[u] = v[j][u];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll 1
-        for (int at = 0; at < KS; at++) {
-            const int j = 4 * (at / 16) + at % 4, from = 16 * (at % 16 / 4) + i; // the word (half of it) and the lane that hold its probability
-            float p[NR];
-#pragma unroll
-            for (int c = 0; c < NR; c++) {
-                const int x = F ? j : j / 2;
-                const uint32_t w = (uint32_t)__shfl((int)(x < 2 ? x == 0 ? P[c][0] : P[c][1] : x == 2 ? P[c][2] : P[c][3]), from);
-                if constexpr (F) p[c] = __uint_as_float(w);
-                else p[c] = qmh_to_f(__builtin_bit_cast(T, (uint16_t)(j & 1 ? w >> 16 : w)));
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int t = 0; t < VE; t++) {
-                    const float x = qmh_to_f(rows[at * HDP + (4 * g + e) * VE + t]);
-                    const float y = __builtin_isfinite(x) ? 0.0f : x;
-#pragma unroll
-                    for (int c = 0; c < NR; c++) O[c][t][e] += (vis[c] >> at) & 1 ? p[c] * y : 0.0f;
-                    __builtin_amdgcn_sched_barrier(0); // one at a time: this path must not cost the others registers
-                }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront"); // the rows are read before another step's are written
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int j = 0; j < 4 * RT; j++)
-#pragma unroll
-            for (int u = 0; u < VW; u++) {
-                uint32_t w = v[j][u];
-                w &= (w & EXP) == EXP ? F ? 0u : 0xffff0000u : ~0u;
-                if constexpr (!F) w &= (w & EXP << 16) == EXP << 16 ? 0xffffu : ~0u;
-                v[j][u] = w;
-            }
-    }
-
     __device__ __forceinline__ void add_values(const v4u (&P)[NR]) {
         if constexpr (F) {
 #pragma unroll
@@ -431,7 +373,7 @@ struct attn_wave {
 
     // This wave's steps of the list's chunk; full: positions that every row sees. The next step's keys are loaded as soon
     // as the scores are made, its values as soon as the step's are used: each has the other's work to arrive in.
-    __device__ __forceinline__ void walk(const attn_args &s, const attn_list &L, int kvh, float sc, int full, float *area, bool &bad) {
+    __device__ __forceinline__ void walk(const attn_args &s, const attn_list &L, int kvh, float sc, int full, bool &bad) {
         const int w = uniform((int)(threadIdx.x >> 6));
         int base = L.from + w * KS;
         if (base > L.cap) return; // no table entry to look at (a list that is none has no table)
@@ -449,7 +391,6 @@ struct attn_wave {
             bl = locate(s, L, pg, base + 4 * KS, kvh, bad);
             load_k(s, bl);
             weigh(S, P, base, sc, base + KS > full);
-            if (TREE && L.own && base + KS > full) odd_values(P, area);
             add_values(P);
             load_v(s, bl);
             pg = fetch(s, L, base + 8 * KS);
@@ -459,6 +400,79 @@ struct attn_wave {
         }
     }
 };
+
+// Trees: a node that a row does not see must not reach it, whatever its values hold, but a product with 0 makes NaN of a value
+// that is not finite. So a row whose sums are not finite is made once more here, by the whole workgroup, from what it sees alone: 256
+// positions at a time, their scores a thread each, then an output element a thread. It happens only there, and its few registers
+// leave the others theirs (looking at the values in the walk took 10 of 98 us of 8 sequences of 4100, 32 x 128).
+template <typename T>
+__device__ __forceinline__ void attend_row(const attn_args &s, float *lds, int r, int R, int t0, int sq, int kvh, const attn_list &shared,
+                                           const attn_list &own, bool bad, int part) {
+    const int tid = threadIdx.x, hd = s.p.head_dim, G = s.n.G, node = r / G, ctx = own.n - R / G;
+    const int64_t token = t0 + node, head = kvh * G + r % G;
+    const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f;
+    float *q = lds, *weight = lds + 256;       // [256] each; a weight of -1: not seen
+    int64_t *at = (int64_t *)(lds + 512);      // [256]: where the position's row lies in the pools
+    float *top = (float *)(at + 256);          // [4]
+    if (tid < hd) {
+        const float x = qmh_to_f(((const T *)s.a.q)[token * s.a.q_stride + head * hd + tid]);
+        q[tid] = s.a.scale < 0.0f ? -x : x;
+    }
+    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
+#pragma unroll 1
+    for (int k = 0; k < 2; k++) {
+        const attn_list L = k ? own : shared;
+#pragma unroll 1
+        for (int base = L.from; base < L.to; base += 256) {
+            __syncthreads(); // q is there, the last positions are done with
+            const int pos = base + tid, n = pos - ctx;
+            bool sees = pos < L.to;
+            if (sees && L.own && n >= 0)
+                sees = s.tree.mask ? (s.tree.mask[sq * s.tree.stride + (int64_t)node * s.tree.words + (n >> 5)] >> (n & 31)) & 1 : n <= node;
+            const int page = sees ? L.tab[pos >> s.lg_ps] : -1;
+            sees = sees && page >= 0 && page < s.p.n_pages;
+            float x = -__builtin_inff();
+            if (sees) {
+                const int64_t row = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (pos & (s.p.page_size - 1))) * hd;
+                at[tid] = row;
+                x = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < hd; d += 16 / (int)sizeof(T)) {
+                    const qmh_vec<T, 16 / sizeof(T)> kv = *(const qmh_vec<T, 16 / sizeof(T)> *)((const T *)s.p.k + row + d);
+#pragma unroll
+                    for (int i = 0; i < 16 / (int)sizeof(T); i++) x = __builtin_fmaf(q[d + i], qmh_to_f(kv.e[i]), x);
+                }
+            }
+            const float t = qmh_wave_max(x);
+            if ((tid & 63) == 0) top[tid >> 6] = t;
+            __syncthreads();
+            const float up = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3])), ref = up == -__builtin_inff() ? 0.0f : up;
+            const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - up) * sc);
+            m = up;
+            weight[tid] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x - ref, sc, 7.0f)) : -1.0f; // times 2^7, as in the walk
+            __syncthreads();
+            l *= f;
+            o *= f;
+#pragma unroll 1
+            for (int j = 0; j < 256 && base + j < L.to; j++) {
+                const float p = weight[j];
+                if (p < 0.0f) continue;
+                l += p;
+                if (tid < hd) o = __builtin_fmaf(p, qmh_to_f(((const T *)s.p.v)[at[j] + tid]), o);
+            }
+        }
+    }
+    __syncthreads();
+    if (tid >= hd) return;
+    if (bad) l = __builtin_nanf("");
+    if (part < 0) {
+        ((T *)s.a.out)[token * s.a.out_stride + head * hd + tid] = (T)(l == 0.0f ? 0.0f : o / l);
+    } else {
+        const int64_t to = (int64_t)part * s.n.rows + token * s.a.n_heads + head;
+        if (tid == 0) s.ml[to] = make_float2(m, l);
+        s.part[to * hd + tid] = o;
+    }
+}
 
 // Rows [row0, row0 + 16 NR) of the R that share a kv head's keys: row r is token t0 + r / G, head r % G of it. They see
 // the chunk of the shared prefix and then the chunk of own pages; sq: whose these are. part < 0: the result goes out, else it is part `part`.
@@ -470,6 +484,8 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     const int H = s.a.n_heads, h0 = kvh * G;
     const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f; // exponentials are powers of two
     W x;
+    __shared__ uint32_t odd[2]; // trees: which of the rows have sums that are not finite
+    if (TREE && threadIdx.x < 2) odd[threadIdx.x] = 0;
     x.far = false;
 #pragma unroll
     for (int c = 0; c < NR; c++) {
@@ -516,7 +532,7 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
                 x.lim[c] = first + (r < R ? r : R - 1) / G;
             }
         }
-        x.walk(s, L, kvh, sc, full, lds + w * 16 * NR * W::LDS_COL, bad);
+        x.walk(s, L, kvh, sc, full, bad);
     }
     // join the waves
     float *ob = lds;                                           // [wave][16 NR][LDS_COL]
@@ -545,8 +561,8 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     __syncthreads();
     constexpr int D4 = HDP / 4;
     const int d = 4 * (threadIdx.x % D4); // 256 is a multiple of D4
-    if (d >= hd) return;
-    for (int col = threadIdx.x / D4; col < 16 * NR && row0 + col < R; col += 256 / D4) {
+    if (!TREE && d >= hd) return;
+    for (int col = threadIdx.x / D4; d < hd && col < 16 * NR && row0 + col < R; col += 256 / D4) {
         float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; k++) m = fmaxf(m, mb[k * 16 * NR + col].x);
@@ -559,6 +575,8 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             o += *(const v4f *)(ob + (k * 16 * NR + col) * W::LDS_COL + d) * f;
         }
         const int2 th = where[col];
+        if constexpr (TREE)
+            if (!__builtin_isfinite(o[0] + o[1] + (o[2] + o[3]))) atomicOr(&odd[col >> 5], 1u << (col & 31));
         if (part < 0) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             qmh_vec<T, 4> y;
@@ -570,6 +588,13 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             if (d == 0) s.ml[at] = make_float2(m, l);
             *(v4f *)(s.part + at * hd + d) = o;
         }
+    }
+    if constexpr (TREE) {
+        __syncthreads();
+        if (own.to > own.n - R / G && (odd[0] | odd[1])) // a chunk without nodes is seen by all
+#pragma unroll 1
+            for (int col = 0; col < 16 * NR; col++)
+                if ((odd[col >> 5] >> (col & 31)) & 1) attend_row<T>(s, lds, row0 + col, R, t0, sq, kvh, shared, own, bad, part);
     }
 }
 
