@@ -276,7 +276,7 @@ extern "C" int qmh_launch_paged_append(const qmh_append_args *a, const qmh_rotar
 }
 
 extern "C" size_t qmh_attention_ws_bytes(const qmh_attention_args *a, int cus) {
-    return attention_ws(a, (int64_t)a->n_seq * a->q_len, cus);
+    return attention_ws<false>(a, (int64_t)a->n_seq * a->q_len, cus);
 }
 
 extern "C" int qmh_launch_paged_attention(const qmh_attention_args *a, int cus, void *ws, void *stream) {

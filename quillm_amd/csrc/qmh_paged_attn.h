@@ -699,6 +699,7 @@ __global__ __launch_bounds__(256) void k_attention_join(const attn_args s, int p
 }
 
 // n_rows: rows of q (at most n_seq * q_len are used)
+template <bool TREE>
 attn_plan plan_attention(const qmh_attention_args *a, int64_t n_rows, int cus) {
     attn_plan n = {};
     const qmh_pages *p = a->pages;
@@ -741,7 +742,17 @@ attn_plan plan_attention(const qmh_attention_args *a, int64_t n_rows, int cus) {
             n.ps = split(a->max_prefix, 40, &n.pc);
             pre = ((int64_t)a->n_groups * KV * n.ps + 7) / 8 * 8 * n.pt;
         }
-        if (a->max_len) n.os = split(a->max_len, 24, &n.oc);
+        if (TREE && !a->max_prefix && a->max_len) {
+            // Trees without a prefix: one workgroup a CU where few rows share the keys (reading them bounds it: 8 x 32 walks of 4100 x 128 take
+            // 87 us whole, 95 in two chunks each; 4 x 32 52 in two, 57 in four), two a CU where many do and their products bound it (24 tiles
+            // of 30011 x 64 35 us in 16 chunks, 31 in 21; but 256 of 6000 48 whole, 51 in two).
+            const int64_t slots = uo * 4 >= cus * 3 ? uo : n.ot >= 4 ? 2 * cus : cus;
+            const int64_t k = slots / uo < 48 ? slots / uo : 48;
+            n.oc = (int)((a->max_len + k - 1) / k + unit - 1) / unit * unit;
+            n.os = (a->max_len + n.oc - 1) / n.oc;
+        } else if (a->max_len) {
+            n.os = split(a->max_len, 24, &n.oc);
+        }
     }
     n.pre_blocks = (uint32_t)(pre < 0x7fffffff ? pre : 0x7fffffff);
     n.blocks = pre + uo * n.os;
@@ -767,9 +778,10 @@ void launch_attention(const attn_args &s, hipStream_t st) {
     }
 }
 
+template <bool TREE>
 size_t attention_ws(const qmh_attention_args *a, int64_t n_rows, int cus) {
     if (a->n_seq == 0 || n_rows == 0) return 0;
-    const attn_plan n = plan_attention(a, n_rows, cus);
+    const attn_plan n = plan_attention<TREE>(a, n_rows, cus);
     const size_t parts = n.ps + n.os;
     return parts > 1 ? parts * n.rows * (a->pages->head_dim * sizeof(float) + sizeof(float2)) : 0;
 }
@@ -780,7 +792,7 @@ int run_attention(const qmh_attention_args *a, const attn_tree &tree, int cus, v
     s.a = *a;
     s.tree = tree;
     s.p = *a->pages;
-    s.n = plan_attention(a, tree.n_rows, cus);
+    s.n = plan_attention<TREE>(a, tree.n_rows, cus);
     s.lg_ps = __builtin_ctz(s.p.page_size);
     s.part = (float *)ws;
     s.ml = (float2 *)(s.part + (size_t)(s.n.ps + s.n.os) * s.n.rows * s.p.head_dim);

@@ -340,7 +340,7 @@ extern "C" int qmh_launch_paged_plan(const qmh_plan_args *a, void *ws, void *str
     return (int)hipGetLastError();
 }
 
-extern "C" size_t qmh_tree_ws_bytes(const qmh_tree_args *a, int cus) { return attention_ws(&a->base, a->n_rows, cus); }
+extern "C" size_t qmh_tree_ws_bytes(const qmh_tree_args *a, int cus) { return attention_ws<true>(&a->base, a->n_rows, cus); }
 
 extern "C" int qmh_launch_tree_attention(const qmh_tree_args *a, int cus, void *ws, void *stream) {
     const attn_tree t = {a->n_rows, a->first, a->mask, a->mask_stride, a->mask_words};
