@@ -712,6 +712,8 @@ attn_plan plan_attention(const qmh_attention_args *a, int64_t n_rows, int cus) {
     auto tiles = [&](int64_t r) { return r <= 16 || most == 1 ? 1 : r <= 32 || most == 2 ? 2 : 4; };
     n.nrp = tiles(rp);
     n.nro = ro <= 16 ? 1 : n.nrp;
+    // f32 products take so long that rows which are none cost more than keys read again
+    if (TREE && p->dtype == QMH_F32 && (ro + 15) / 16 * 2 <= (ro + 16 * n.nro - 1) / (16 * n.nro) * n.nro) n.nro = 1;
     n.pt = (int)((rp + 16 * n.nrp - 1) / (16 * n.nrp));
     n.ot = (int)((ro + 16 * n.nro - 1) / (16 * n.nro));
     const int64_t up = (int64_t)a->n_groups * KV * n.pt, uo = (int64_t)a->n_seq * KV * n.ot;
