@@ -115,7 +115,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void k_
     };
     if (w < tasks) fetch(w);
     // so are the lists' first tokens
-    constexpr int HB = 4;
+    constexpr int HB = sizeof(T) == 4 ? 8 : 4;
     const int h = penal && said > 0 ? (int)min((int64_t)said, a.history_stride) : 0, nb = min(biased, a.bias_stride);
     const int32_t *hist = a.history + sq * a.history_stride, *biases = a.bias_token + (int64_t)sq * a.bias_stride;
     int early[HB];
