@@ -115,6 +115,7 @@ struct attn_wave {
     static constexpr int LDS_COL = HDP + 4;
     static constexpr int LDS_FLOATS = 4 * 16 * NR * LDS_COL + 4 * 16 * NR * 2 + 16 * NR * 2;
 
+    int tid;
     v4u Q[NR][KC];
     v4f O[NR][VE];
     // l: the sum of a row's probabilities: a lane's own positions in l[0], or (16 bit) all of them in every element, by a
@@ -165,7 +166,7 @@ struct attn_wave {
         return x;
     }
     __device__ __forceinline__ void load_k(const attn_args &s, const blocks &bl) {
-        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, rb = s.p.head_dim * (int)sizeof(T);
+        const int lane = tid & 63, i = lane & 15, g = lane >> 4, rb = s.p.head_dim * (int)sizeof(T);
 #pragma unroll
         for (int r = 0; r < RT; r++) {
             const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.k + bl.off[r], (short)0, bl.bytes[r], 0x00020000);
@@ -177,7 +178,7 @@ struct attn_wave {
         }
     }
     __device__ __forceinline__ void load_v(const attn_args &s, const blocks &bl) {
-        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, rb = s.p.head_dim * (int)sizeof(T);
+        const int lane = tid & 63, i = lane & 15, g = lane >> 4, rb = s.p.head_dim * (int)sizeof(T);
 #pragma unroll
         for (int r = 0; r < RT; r++) {
             const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((uint8_t *)s.p.v + bl.off[r], (short)0, bl.bytes[r], 0x00020000);
@@ -247,7 +248,7 @@ struct attn_wave {
 
     // the probabilities of a step's scores, packed for the product with V; masked: some row does not see all of it
     __device__ __forceinline__ void weigh(v4f (&S)[NR][RT], v4u (&P)[NR], int base, float sc, bool masked) {
-        const int g = (threadIdx.x & 63) >> 4;
+        const int g = (tid & 63) >> 4;
         if (masked) {
 #pragma unroll
             for (int c = 0; c < NR; c++)
@@ -374,7 +375,7 @@ struct attn_wave {
     // This wave's steps of the list's chunk; full: positions that every row sees. The next step's keys are loaded as soon
     // as the scores are made, its values as soon as the step's are used: each has the other's work to arrive in.
     __device__ __forceinline__ void walk(const attn_args &s, const attn_list &L, int kvh, float sc, int full, bool &bad) {
-        const int w = uniform((int)(threadIdx.x >> 6));
+        const int w = uniform(tid >> 6);
         int base = L.from + w * KS;
         if (base > L.cap) return; // no table entry to look at (a list that is none has no table)
         pages pg = fetch(s, L, base);
@@ -402,64 +403,60 @@ struct attn_wave {
 };
 
 // Trees: a node that a row does not see must not reach it, whatever its values hold, but a product with 0 makes NaN of a value
-// that is not finite. So a row whose sums are not finite is made once more here, by the whole workgroup, from what it sees alone: 256
-// positions at a time, their scores a thread each, then an output element a thread. It happens only there, and its few registers
-// leave the others theirs (looking at the values in the walk took 10 of 98 us of 8 sequences of 4100, 32 x 128).
+// that is not finite. Where sums are not finite, and some node's values are not either, a tile is made again: the positions before the nodes as
+// ever, then each row's nodes here, by the whole workgroup, from what the row sees alone: 256 nodes at a time, their scores a thread
+// each, then an output element a thread. That happens only there: looking at the values in the walk cost it registers, and 10 of 98 us of
+// 8 sequences of 4100, 32 x 128.
+constexpr int NODE_FLOATS = 256 + 256 + 512 + 4; // what it needs of LDS
 template <typename T>
-__device__ __forceinline__ void attend_row(const attn_args &s, float *lds, int r, int R, int t0, int sq, int kvh, const attn_list &shared,
-                                           const attn_list &own, bool bad, int part) {
+__device__ __forceinline__ void attend_nodes(const attn_args &s, float *lds, float m, float l, float o, int r, int R, int t0, int sq, int kvh,
+                                             const attn_list &own, bool bad, int part) {
     const int tid = threadIdx.x, hd = s.p.head_dim, G = s.n.G, node = r / G, ctx = own.n - R / G;
     const int64_t token = t0 + node, head = kvh * G + r % G;
     const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f;
-    float *q = lds, *weight = lds + 256;       // [256] each; a weight of -1: not seen
-    int64_t *at = (int64_t *)(lds + 512);      // [256]: where the position's row lies in the pools
-    float *top = (float *)(at + 256);          // [4]
+    float *q = lds, *weight = lds + 256;  // [256] each; a weight of -1: not seen
+    int64_t *at = (int64_t *)(lds + 512); // [256]: where the node's row lies in the pools
+    float *top = (float *)(at + 256);     // [4]
     if (tid < hd) {
         const float x = qmh_to_f(((const T *)s.a.q)[token * s.a.q_stride + head * hd + tid]);
         q[tid] = s.a.scale < 0.0f ? -x : x;
     }
-    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
 #pragma unroll 1
-    for (int k = 0; k < 2; k++) {
-        const attn_list L = k ? own : shared;
+    for (int base = own.from > ctx ? own.from : ctx; base < own.to; base += 256) {
+        __syncthreads(); // q is there, the last nodes are done with
+        const int pos = base + tid, n = pos - ctx;
+        bool sees = pos < own.to;
+        if (sees) sees = s.tree.mask ? (s.tree.mask[sq * s.tree.stride + (int64_t)node * s.tree.words + (n >> 5)] >> (n & 31)) & 1 : n <= node;
+        const int page = sees ? own.tab[pos >> s.lg_ps] : -1;
+        sees = sees && page >= 0 && page < s.p.n_pages;
+        float x = -__builtin_inff();
+        if (sees) {
+            const int64_t row = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (pos & (s.p.page_size - 1))) * hd;
+            at[tid] = row;
+            x = 0.0f;
 #pragma unroll 1
-        for (int base = L.from; base < L.to; base += 256) {
-            __syncthreads(); // q is there, the last positions are done with
-            const int pos = base + tid, n = pos - ctx;
-            bool sees = pos < L.to;
-            if (sees && L.own && n >= 0)
-                sees = s.tree.mask ? (s.tree.mask[sq * s.tree.stride + (int64_t)node * s.tree.words + (n >> 5)] >> (n & 31)) & 1 : n <= node;
-            const int page = sees ? L.tab[pos >> s.lg_ps] : -1;
-            sees = sees && page >= 0 && page < s.p.n_pages;
-            float x = -__builtin_inff();
-            if (sees) {
-                const int64_t row = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (pos & (s.p.page_size - 1))) * hd;
-                at[tid] = row;
-                x = 0.0f;
-#pragma unroll 1
-                for (int d = 0; d < hd; d += 16 / (int)sizeof(T)) {
-                    const qmh_vec<T, 16 / sizeof(T)> kv = *(const qmh_vec<T, 16 / sizeof(T)> *)((const T *)s.p.k + row + d);
+            for (int d = 0; d < hd; d += 16 / (int)sizeof(T)) {
+                const qmh_vec<T, 16 / sizeof(T)> kv = *(const qmh_vec<T, 16 / sizeof(T)> *)((const T *)s.p.k + row + d);
 #pragma unroll
-                    for (int i = 0; i < 16 / (int)sizeof(T); i++) x = __builtin_fmaf(q[d + i], qmh_to_f(kv.e[i]), x);
-                }
+                for (int i = 0; i < 16 / (int)sizeof(T); i++) x = __builtin_fmaf(q[d + i], qmh_to_f(kv.e[i]), x);
             }
-            const float t = qmh_wave_max(x);
-            if ((tid & 63) == 0) top[tid >> 6] = t;
-            __syncthreads();
-            const float up = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3])), ref = up == -__builtin_inff() ? 0.0f : up;
-            const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - up) * sc);
-            m = up;
-            weight[tid] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x - ref, sc, 7.0f)) : -1.0f; // times 2^7, as in the walk
-            __syncthreads();
-            l *= f;
-            o *= f;
+        }
+        const float t = qmh_wave_max(x);
+        if ((tid & 63) == 0) top[tid >> 6] = t;
+        __syncthreads();
+        const float up = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3])), ref = up == -__builtin_inff() ? 0.0f : up;
+        const float f = m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - up) * sc); // without a score: sums of 0 (or NaN)
+        m = up;
+        weight[tid] = sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x - ref, sc, 7.0f)) : -1.0f; // times 2^7, as in the walk
+        __syncthreads();
+        l *= f;
+        o *= f;
 #pragma unroll 1
-            for (int j = 0; j < 256 && base + j < L.to; j++) {
-                const float p = weight[j];
-                if (p < 0.0f) continue;
-                l += p;
-                if (tid < hd) o = __builtin_fmaf(p, qmh_to_f(((const T *)s.p.v)[at[j] + tid]), o);
-            }
+        for (int j = 0; j < 256 && base + j < own.to; j++) {
+            const float p = weight[j];
+            if (p < 0.0f) continue;
+            l += p;
+            if (tid < hd) o = __builtin_fmaf(p, qmh_to_f(((const T *)s.p.v)[at[j] + tid]), o);
         }
     }
     __syncthreads();
@@ -473,19 +470,39 @@ __device__ __forceinline__ void attend_row(const attn_args &s, float *lds, int r
         s.part[to * hd + tid] = o;
     }
 }
+// whether the list's nodes, of those in its chunk, have a value that is not finite (for the whole workgroup)
+template <typename T>
+__device__ __forceinline__ bool odd_nodes(const attn_args &s, int ctx, int kvh, const attn_list &own) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int from = own.from > ctx ? own.from : ctx, per = s.p.head_dim / N;
+    bool odd = false;
+    for (int i = threadIdx.x; i < (own.to - from) * per; i += 256) {
+        const int pos = from + i / per, page = own.tab[pos >> s.lg_ps];
+        if (page < 0 || page >= s.p.n_pages) continue;
+        const int64_t row = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (pos & (s.p.page_size - 1))) * s.p.head_dim;
+        const qmh_vec<T, N> x = *(const qmh_vec<T, N> *)((const T *)s.p.v + row + i % per * N);
+#pragma unroll
+        for (int e = 0; e < N; e++) odd |= !__builtin_isfinite(qmh_to_f(x.e[e]));
+    }
+    return __syncthreads_or(odd);
+}
 
 // Rows [row0, row0 + 16 NR) of the R that share a kv head's keys: row r is token t0 + r / G, head r % G of it. They see
 // the chunk of the shared prefix and then the chunk of own pages; sq: whose these are. part < 0: the result goes out, else it is part `part`.
+// True (trees): the tile has to be made again, with `again`.
 template <typename T, int HDP, int NR, bool TREE>
-__device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0, int R, int t0, int sq, int kvh, const attn_list &shared,
-                                       const attn_list &own, bool bad, int part) {
+__device__ __forceinline__ bool attend_once(const attn_args &s, float *lds, int row0, int R, int t0, int sq, int kvh, const attn_list &shared,
+                                            const attn_list &own, bool bad, int part, bool again) {
     using W = attn_wave<T, HDP, NR, TREE>;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4, G = s.n.G, hd = s.p.head_dim;
+    int tid = threadIdx.x;
+    if constexpr (TREE) asm volatile("" : "+v"(tid)); // nothing made of it stays in registers from one time to the other
+    const int lane = tid & 63, w = tid >> 6, i = lane & 15, g = lane >> 4, G = s.n.G, hd = s.p.head_dim;
     const int H = s.a.n_heads, h0 = kvh * G;
     const float sc = __builtin_fabsf(s.a.scale) * 1.44269504088896340736f; // exponentials are powers of two
     W x;
+    x.tid = tid;
     __shared__ uint32_t odd[2]; // trees: which of the rows have sums that are not finite
-    if (TREE && threadIdx.x < 2) odd[threadIdx.x] = 0;
+    if (TREE && tid < 2) odd[tid] = 0;
     x.far = false;
 #pragma unroll
     for (int c = 0; c < NR; c++) {
@@ -509,6 +526,11 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
 #pragma unroll 1
     for (int k = 0; k < 2; k++) {
         attn_list L = k ? own : shared;
+        if (TREE && again && L.own) { // the positions before the nodes: all rows see them
+            L.n = own.n - R / G;
+            L.to = min(L.to, L.n);
+            L.own = 0;
+        }
         int full = L.to;
 #pragma unroll
         for (int c = 0; c < NR; c++) x.lim[c] = L.n;
@@ -560,9 +582,9 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     }
     __syncthreads();
     constexpr int D4 = HDP / 4;
-    const int d = 4 * (threadIdx.x % D4); // 256 is a multiple of D4
-    if (!TREE && d >= hd) return;
-    for (int col = threadIdx.x / D4; d < hd && col < 16 * NR && row0 + col < R; col += 256 / D4) {
+    const int d = 4 * (tid % D4); // 256 is a multiple of D4
+    if (!TREE && d >= hd) return false;
+    for (int col = tid / D4; d < hd && col < 16 * NR && row0 + col < R; col += 256 / D4) {
         float m = -__builtin_inff(), l = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; k++) m = fmaxf(m, mb[k * 16 * NR + col].x);
@@ -575,6 +597,11 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
             o += *(const v4f *)(ob + (k * 16 * NR + col) * W::LDS_COL + d) * f;
         }
         const int2 th = where[col];
+        if (TREE && again) { // for attend_nodes
+            *(v4f *)(ob + col * W::LDS_COL + d) = o;
+            if (d == 0) where[col] = make_int2(__float_as_int(m), __float_as_int(l));
+            continue;
+        }
         if constexpr (TREE)
             if (!__builtin_isfinite(o[0] + o[1] + (o[2] + o[3]))) atomicOr(&odd[col >> 5], 1u << (col & 31));
         if (part < 0) {
@@ -591,11 +618,26 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     }
     if constexpr (TREE) {
         __syncthreads();
-        if (own.to > own.n - R / G && (odd[0] | odd[1])) // a chunk without nodes is seen by all
+        if (again) {
 #pragma unroll 1
-            for (int col = 0; col < 16 * NR; col++)
-                if ((odd[col >> 5] >> (col & 31)) & 1) attend_row<T>(s, lds, row0 + col, R, t0, sq, kvh, shared, own, bad, part);
+            for (int col = 0; col < 16 * NR && row0 + col < R; col++) {
+                const int2 ml = where[col];
+                const float o = ob[col * W::LDS_COL + ((int)threadIdx.x < hd ? threadIdx.x : 0)];
+                attend_nodes<T>(s, lds + W::LDS_FLOATS, __int_as_float(ml.x), __int_as_float(ml.y), o, row0 + col, R, t0, sq, kvh, own, bad, part);
+            }
+            return false;
+        }
+        return own.own && own.to > own.n - R / G && (odd[0] | odd[1]) && odd_nodes<T>(s, own.n - R / G, kvh, own);
     }
+    return false;
+}
+template <typename T, int HDP, int NR, bool TREE>
+__device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0, int R, int t0, int sq, int kvh, const attn_list &shared,
+                                       const attn_list &own, bool bad, int part) {
+    bool again = false;
+#pragma unroll 1
+    do again = attend_once<T, HDP, NR, TREE>(s, lds, row0, R, t0, sq, kvh, shared, own, bad, part, again);
+    while (TREE && again);
 }
 
 // the rows of sequences [sq, sq + n): t0 to t0 + the result, 0 where they are none
@@ -613,7 +655,7 @@ __device__ __forceinline__ int attn_rows(const attn_args &s, int sq, int n, int 
 
 template <typename T, int HDP, int NRP, int NRO, bool TREE>
 __global__ __launch_bounds__(256, 2) void k_paged_attention(const attn_args s) {
-    __shared__ __align__(16) float lds[attn_wave<T, HDP, (NRP > NRO ? NRP : NRO), TREE>::LDS_FLOATS];
+    __shared__ __align__(16) float lds[attn_wave<T, HDP, (NRP > NRO ? NRP : NRO), TREE>::LDS_FLOATS + (TREE ? NODE_FLOATS : 0)];
     const attn_plan &n = s.n;
     const int KV = s.p.n_kv_heads;
     uint32_t b = blockIdx.x;

@@ -183,7 +183,7 @@ __device__ __forceinline__ void plan_tokens(const qmh_plan_args &a, const plan_a
                 const int slot = s < n ? p.keep[s] + (t + i - p.tok[s]) : -1;
                 x[0][i] = s < n ? s : -1;
                 x[1][i] = slot;
-                x[2][i] = s < n ? (a.base ? a.base[s] : 0) + slot : -1;
+                x[2][i] = s < n ? (int)((uint32_t)(a.base ? a.base[s] : 0) + slot) : -1;
             }
             int32_t *out[3] = {a.seq + t, a.slot + t, a.pos + t};
 #pragma unroll
@@ -227,7 +227,7 @@ __device__ __forceinline__ void plan_tokens(const qmh_plan_args &a, const plan_a
         }
         a.seq[t] = s;
         a.slot[t] = keep + j;
-        a.pos[t] = base + keep + depth;
+        a.pos[t] = (int)((uint32_t)base + keep + depth);
     }
 }
 
@@ -392,10 +392,15 @@ extern "C" int qmh_launch_paged_plan(const qmh_plan_args *a, void *ws, void *str
     return (int)hipGetLastError();
 }
 
-extern "C" size_t qmh_tree_ws_bytes(const qmh_tree_args *a, int cus) { return attention_ws<true>(&a->base, a->n_rows, cus); }
+// the rows that sequences may have
+static int tree_rows(const qmh_tree_args *a) { return a->first ? a->n_rows : a->base.n_seq * a->base.q_len; }
+
+extern "C" size_t qmh_tree_ws_bytes(const qmh_tree_args *a, int cus) {
+    return attention_ws<true>(&a->base, tree_rows(a), cus);
+}
 
 extern "C" int qmh_launch_tree_attention(const qmh_tree_args *a, int cus, void *ws, void *stream) {
-    const attn_tree t = {a->n_rows, a->first, a->mask, a->mask_stride, a->mask_words};
+    const attn_tree t = {tree_rows(a), a->first, a->mask, a->mask_stride, a->mask_words};
     return run_attention<true>(&a->base, t, cus, ws, (hipStream_t)stream);
 }
 

@@ -524,6 +524,7 @@ static int check_plan(const qmh_plan_args *a, const char *me) {
         if (!a->n_tokens) return fail("%s: trees need n_tokens", me);
         if (a->tree_size < 1 || a->tree_size > 1024) return fail("%s: tree_size %d outside [1, 1024]", me, a->tree_size);
         if (a->parent_stride && a->parent_stride < a->tree_size) return fail("%s: parent_stride %d of trees of %d", me, a->parent_stride, a->tree_size);
+        if (!aligned(a->mask, 4)) return fail("%s: mask is not aligned to its words", me);
     } else if (a->mask) {
         return fail("%s: a mask needs parents", me);
     }
