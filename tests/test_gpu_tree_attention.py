@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 
 def run(q, dt, H, KV, hd, ps, groups, nodes, own, prefix=None, q_len=None, ragged=True, masks="tree", static=False, seed=0, scale=None, pad=0,
-        extra_words=0, spoil=None, touch=None, gap=0, check=True):
+        extra_words=0, spoil=None, touch=None, gap=0, more=0, check=True):
     """nodes, own: of each sequence, own with its nodes. Returns the outputs [rows, H, hd] and where each sequence's start."""
     rs = np.random.default_rng(seed)
     B, per = len(nodes), len(nodes) // groups
@@ -23,7 +23,7 @@ def run(q, dt, H, KV, hd, ps, groups, nodes, own, prefix=None, q_len=None, ragge
     tables, n_pages = o.make_tables(rs, counts, max(counts) + 1)
     pool = [rs.standard_normal((n_pages, KV, ps, hd)) for _ in range(2)]
     first = tr.starts(nodes) + gap
-    rows = (int(first[-1]) + 3) if ragged else B * q_len
+    rows = (int(first[-1]) + 3) if ragged else B * q_len + more
     if not ragged:
         assert all(n == q_len for n in nodes)
     x = o.encode(rs.standard_normal((rows, H * hd + pad)) * 1.5, dt)
@@ -163,6 +163,15 @@ def test_what_is_not_seen_has_no_effect(gpu, dtype, hd):
                         t = own[i] - n + k
                         pool[where][table[i][t // 16], :, t % 16, (3 * k) % hd] = value
             run(gpu, o.TYPES[dtype], 2, 1, hd, 16, 1, [36, 9], [70, 9], touch=touch, seed=hd)
+    # the same in pieces of a long context, trees over a piece's end; and where the context has such values, too, which all see
+    for ctx in (False, True):
+        def long(pool, table, own, nodes, see):
+            for i, n in enumerate(nodes):
+                for k in [*range(3, n, 5)] + ([-7 - n] if ctx else []):
+                    t = own[i] - n + k
+                    pool[1][table[i][t // 16], :, t % 16, (3 * abs(k)) % hd] = [np.inf, np.nan][(k + ctx) % 2]
+        run(gpu, o.TYPES[dtype], 2, 1, hd, 16, 2, [36, 100], [1304, 1100], prefix=[0, 0], touch=long, seed=hd + 1)
+        run(gpu, o.TYPES[dtype], 2, 1, hd, 16, 1, [36, 20], [700, 1100], prefix=[600], touch=long, masks="chain", seed=hd + 2)
     # the type's largest numbers are finite
     big = {"f32": 3e38, "f16": 65504.0, "bf16": 3e38}[dtype]
 
@@ -189,6 +198,11 @@ def test_bad_rows_are_left_out(gpu, first):
         at[:] = first
     got, _ = run(gpu, o.F32, 2, 2, 64, 16, 3, [4, 2, 2], [20, 20, 20], q_len=5, spoil=spoil, check=False, seed=6)
     assert got.shape[0] == 11
+
+
+def test_rows_behind_the_last_sequence_without_first(gpu):
+    run(gpu, o.F16, 4, 2, 64, 16, 2, [4, 4], [900, 20], ragged=False, more=6, seed=12)
+    run(gpu, o.F32, 4, 2, 64, 16, 2, [4, 4], [9, 20], ragged=False, more=6, seed=12)
 
 
 def test_rows_that_start_behind_others(gpu):
