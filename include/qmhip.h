@@ -25,8 +25,8 @@ extern "C" {
 
 /* tensor dtypes, same codes as the reference's qm_dtype (src/qm_base.h:11-15) */
 enum { QMH_F32 = 0, QMH_Q8_0 = 2, QMH_Q4_0 = 3 };
-/* 16-bit element types of rows, pages and logits, for the ops of "several continuations of one prompt"
- * below only: no weight and no file has them. No reference counterpart. */
+/* 16-bit element types of rows, pages and logits, for the ops of "several continuations of one prompt" and
+ * "drafted trees over pages" below only: no weight and no file has them. No reference counterpart. */
 enum { QMH_F16 = 1, QMH_BF16 = 4 };
 
 /* ------------------------------------------------------------------ runtime */
@@ -330,10 +330,10 @@ int qmh_tree_attention(const qmh_tree_args *a, void *ws, size_t ws_bytes, void *
  * not overlap it otherwise. best (NULL: not wanted) [n_rows]: the first token of the largest edited logit, before it is
  * rounded; -1 where all are -inf or NaN.
  * Sequences have at most rows_per_seq rows (first as above, or NULL).
- * history [n_seq][history_stride]: the first history_len[i] tokens (at most history_stride count), of which the first prompt_len[i]
+ * history [n_seq][history_stride] (history_stride at most 2^24): the first history_len[i] tokens (at most history_stride count), of which the first prompt_len[i]
  * (NULL: none) are the prompt's, the others outputs. Tokens outside [0, vocab) are none. history NULL: none anywhere. repetition,
  * presence, frequency: [n_seq] or NULL (1, 0, 0). A repetition that is not above 0 counts as 1.
- * bias_token, bias [n_seq][bias_stride], the first bias_len[i] of them (at most bias_stride count); of a token that is there twice the
+ * bias_token, bias [n_seq][bias_stride] (bias_stride at most 2^24), the first bias_len[i] of them (at most bias_stride count); of a token that is there twice the
  * last one counts. Tokens outside [0, vocab) are none. bias NULL: none.
  * allow [n_allow][allow_stride] words: bit t % 32 of word t / 32 of row allow_row[r] says whether token t may follow (allow_row
  * outside [0, n_allow): all may; allow_row NULL: row r of allow, n_allow >= n_rows). allow NULL: no grammar.

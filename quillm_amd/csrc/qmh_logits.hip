@@ -10,10 +10,15 @@
 namespace {
 
 // A workgroup takes a segment of the vocabulary for some rows of one sequence. First it counts the history's tokens that fall into its
-// segment, in LDS, and lists the tokens that any edit touches (the hot ones). A dense pass then goes over the rows: it copies
-// them (where they go elsewhere), puts -inf where the grammar forbids a token, and finds the best of the tokens that are
-// not hot; it is left out where there is nothing of it to do, and vectors that stay as they are, or are forbidden as a whole,
-// are not read. A sparse pass edits the hot ones: they are few, so their divisions and gathers do not weigh.
+// segment, in LDS, and lists the tokens that any edit touches (the hot ones). A dense pass then goes over pieces of the rows, a wave
+// a piece: it copies them (where they go elsewhere), puts -inf where the grammar forbids a token, and finds the best of the
+// tokens that are not hot; it is left out where there is nothing of it to do, and vectors that stay as they are, or are forbidden as a whole,
+// are not read. A sparse pass edits the hot ones: they are few, so their divisions and gathers do not weigh (in the dense pass, each lane
+// its own, they cost 24-row trees 25 us instead of 18).
+// What bounds it, measured: one row of 32000 f32 edited in place 5 us, a launch and the chain numbers, history, count, list, gather; 384
+// rows of 32003 bf16, best tokens alone, 18.7 us: two launches, and per workgroup 10 us of that chain and its 1000 VALU instructions a wave (the
+// read itself is 5 us); 160 rows of 128256 f32 written elsewhere 49 us for 166 MB, 39 of it without a history of 4000. Twice the rows
+// under way, eight waves a SIMD and a wave a whole row's segment gained nothing.
 constexpr int SEG = 4096, NT = 512;
 constexpr int ROWS = 32; // of a workgroup, at most
 constexpr uint32_t PROMPT = 1u << 31, NODE = 1u << 30; // beside a count of outputs: in the prompt; a node's token

@@ -17,6 +17,9 @@ constexpr int PLAN_TOKENS = 4096;  // tokens of a call that one workgroup does a
 constexpr int PLAN_CHUNK = 1024;   // tokens of a workgroup otherwise
 constexpr int TREE_MOST = 1024;    // nodes of a tree
 
+// Nothing here computes: a call is a chain of loads (lengths, sums, pages or parents, stores), so the work goes into as few launches and
+// dependent steps as can be. Measured: trees of 48 sequences, 870 nodes, 4.2 us, an empty launch's time; prompts of 201 sequences, 181000 rows
+// in two launches 10 us (3.4 of scan, 6 of rows, 2.2 MB).
 // What the scan finds: exclusive sums over the sequences (n + 1 of each) of tokens, pages taken and pages given, a sequence's pages
 // before and after, and the positions it keeps. For a call of one workgroup they lie in LDS, else in the workspace.
 struct plan_arrays {
@@ -290,7 +293,8 @@ bool plan_alone(const qmh_plan_args *a) { return a->n_seq <= PLAN_SEQS && a->n_t
 // A workgroup (x: piece, y: sequence) follows the path and moves its piece of what the accepted positions hold. For each node the
 // lowest of its children that the model chose is found by all threads at once, then the path is a chain of LDS reads. Positions
 // only move down and in order, so a thread that loads eight of its unit before it stores them needs no second buffer. Every
-// workgroup of a sequence follows the path for itself: a launch of its own would take longer.
+// workgroup of a sequence follows the path for itself: a launch of its own would take longer. Measured: 4 trees of 16 nodes in 6 layers of 2 x 48
+// f32 4.9 us, a launch and its chain (rows, nodes, path, pages, data); 64 trees of 61 in 4 layers of 32 x 128 f16, 27 MB, 8.9 us.
 __global__ __launch_bounds__(256) void k_tree_accept(const qmh_accept_args a, const qmh_pages pg, int row_bytes, uint32_t units) {
     __shared__ int follow[TREE_MOST], path[TREE_MOST];
     __shared__ int64_t from[TREE_MOST], to[TREE_MOST];
