@@ -260,8 +260,8 @@ int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t tabl
  * token, chosen already, its keys and values not yet in the pages. A parent that is none counts as -1.
  * Rows: sequence i's nodes are rows first[i] to first[i + 1] of the per-row arrays (first [n_seq + 1] on the device, not
  * decreasing; qmh_paged_plan writes it), or, with first NULL, rows i * q to i * q + q, q the most nodes of a sequence. A sequence
- * whose rows are outside the arrays, or more than q, is left out, and what rows that it shares with others hold is not
- * defined. Rows before the first sequence's and behind the last one's are left as they are.
+ * whose rows are outside the arrays, or more than q, is left out: what its rows hold afterwards is not defined, nor what those hold
+ * that it shares with others. Rows before the first sequence's and behind the last one's are left as they are.
  * Masks: row j of a sequence's mask says with bit k % 32 of word k / 32 whether node j sees node k of its sequence. */
 
 /* Pages and places for the positions that sequences are to hold. Sequence i holds len[i] positions, in the first ceil(len / page_size)

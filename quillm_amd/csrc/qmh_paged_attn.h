@@ -434,10 +434,12 @@ __device__ __forceinline__ void attend_nodes(const attn_args &s, float *lds, flo
         const int pos = base + tid, n = pos - ctx;
         bool sees = pos < own.to;
         if (sees) sees = s.tree.mask ? (s.tree.mask[sq * s.tree.stride + (int64_t)node * s.tree.words + (n >> 5)] >> (n & 31)) & 1 : n <= node;
-        const int page = sees ? own.tab[pos >> s.lg_ps] : -1;
-        sees = sees && page >= 0 && page < s.p.n_pages;
+        const int page = sees ? own.tab[pos >> s.lg_ps] : 0;
         float x = -__builtin_inff();
-        if (sees) {
+        if (page < 0 || page >= s.p.n_pages) {
+            x = __builtin_nanf(""); // the row's result is
+            at[tid] = 0;
+        } else if (sees) {
             const int64_t row = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (pos & (s.p.page_size - 1))) * hd;
             at[tid] = row;
             x = 0.0f;

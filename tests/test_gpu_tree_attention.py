@@ -190,6 +190,77 @@ def test_bad_lengths_and_pages_give_nan(gpu, dtype):
     run(gpu, o.TYPES[dtype], 4, 2, 64, 16, 5, [5, 5, 5, 5, 5], [20, 20, 20, 20, 20], spoil=spoil, seed=4)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_a_bad_page_of_nodes_beside_values_that_are_not_finite(gpu, dtype):
+    """Chains over two pages: rows that see the second one, which is none, are NaN, whatever the first one holds."""
+    def touch(pool, table, own, nodes, see):
+        pool[1][table[0][2], :, 4, 3] = np.inf  # node 4, at position 36
+
+    def spoil(table, own, first, bad):
+        table[0, 3] = -1  # positions 48 on: nodes 16 on
+    got, at = run(gpu, o.TYPES[dtype], 2, 1, 64, 16, 2, [20, 20], [52, 52], masks="chain", touch=touch, spoil=spoil, check=False, seed=2)
+    assert np.isnan(got[16:20]).all()
+    assert np.isfinite(got[20:40]).all()
+
+
+def test_pages_past_4_gib(gpu):
+    """Nodes and context in pages that lie more than 4 GiB into the pools, and a path moved between them."""
+    q, L, KV, hd, ps = gpu, gpu.load_library(), 16, 256, 1024
+    page = KV * ps * hd * 2  # 8 MiB
+    n_pages = 1100
+    pool = [q.DeviceBuffer(n_pages * page) for _ in range(2)]
+    rs = np.random.default_rng(0)
+    table = np.array([[1099, 1050]], np.int32)
+    own, n = 1024 + 6, 9  # nodes 0 to 2 in the first page, the others in the second
+    kv = [o.encode(rs.standard_normal((own, KV, hd)), o.F16) for _ in range(2)]
+    for b, x in zip(pool, kv):
+        for p in range(2):
+            rows = x[p * ps:(p + 1) * ps]
+            for h in range(KV):
+                part = np.ascontiguousarray(rows[:, h])
+                q._check(L.qmh_memcpy_h2d(b.ptr + int(table[0, p]) * page + h * ps * hd * 2, part.ctypes.data, part.nbytes), "rows")
+    x = o.encode(rs.standard_normal((n, KV * hd)), o.F16)
+    parent = tr.tree(rs, n)
+    parent[5] = 2
+    see = tr.ancestors(parent)
+    dev = q.DeviceBuffer.from_array
+    dx, out, tab, length, mask = dev(x), q.DeviceBuffer(x.nbytes), dev(table), dev(np.array([own], np.int32)), dev(tr.pack(see, 1))
+    pages = q.Pages(dtype=o.F16, n_kv_heads=KV, head_dim=hd, page_size=ps, n_pages=n_pages, k=pool[0].ptr, v=pool[1].ptr)
+    base = q.AttentionArgs(pages=ctypes.pointer(pages), n_heads=KV, n_seq=1, q_len=n, n_groups=1, q=dx.ptr, q_stride=KV * hd, out=out.ptr,
+                           out_stride=KV * hd, table=tab.ptr, len=length.ptr, table_stride=2, max_len=own, scale=0.0625)
+    a = q.TreeArgs(base=base, n_rows=n, mask=mask.ptr, mask_words=1)
+    need = L.qmh_tree_attention_ws(ctypes.byref(a))
+    ws = q.DeviceBuffer(max(need, 16))
+    q._check(L.qmh_tree_attention(ctypes.byref(a), ws.ptr, need, None), "attention")
+    q.sync()
+    got = o.decode(out.to_array(np.uint16), o.F16).reshape(n, KV, hd)
+    k, v = (o.decode(y, o.F16) for y in kv)
+    for j in range(n):
+        t = np.concatenate([np.ones(own - n, bool), see[j]])
+        want, mag, reach = o.attention(o.decode(x[j], o.F16).reshape(KV, hd), k[t], v[t], 0.0625)
+        tol = mag * (2 * ((hd + 4) * o.U32 * reach + 4 * o.U32) + (own + 64) * o.U32 + o.HALF[o.F16]) * 1.01 + o.HALF[o.F16] * np.abs(want)
+        o.close(got[j], want, tol + own * o.TINY[o.F16] * np.abs(v).max(), f"node {j}")
+    # the path 0, 2, 5 ...: node 5 (second page) moves to position 2 of the tree (first page)
+    token, choice = np.arange(n, dtype=np.int32), np.full(n, -1, np.int32)
+    parent[2] = 0
+    choice[0], choice[2] = 2, 5
+    d = {m: dev(y) for m, y in dict(parent=parent, token=token, choice=choice, count=np.zeros(1, np.int32), next=np.zeros(1, np.int32),
+                                    keep=np.zeros(1, np.int32)).items()}
+    a = q.AcceptArgs(n_seq=1, tree_size=n, parent=d["parent"].ptr, parent_stride=n, token=d["token"].ptr, token_stride=n, n_rows=n,
+                     choice=d["choice"].ptr, len=length.ptr, count=d["count"].ptr, next=d["next"].ptr, keep=d["keep"].ptr,
+                     pages=ctypes.pointer(pages), n_layers=1, table=tab.ptr, table_stride=2)
+    q._check(L.qmh_tree_accept(ctypes.byref(a), None), "accept")
+    q.sync()
+    assert d["count"].to_array(np.int32)[0] == 3
+    begin = own - n
+    for b, y in zip(pool, kv):
+        for h in (0, KV - 1):
+            row = np.zeros(hd, np.uint16)
+            for to, src in ((begin + 1, begin + 2), (begin + 2, begin + 5), (begin, begin)):
+                q._check(L.qmh_memcpy_d2h(row.ctypes.data, b.ptr + int(table[0, to // ps]) * page + (h * ps + to % ps) * hd * 2, row.nbytes), "row")
+                assert np.array_equal(row, y[src, h]), (to, src)
+
+
 @pytest.mark.parametrize("first", [[0, 4, 3, 8], [0, 4, 40, 8], [-1, 4, 6, 8], [0, 7, 9, 2 ** 31 - 1], [2, 4, 6, 12]])
 def test_bad_rows_are_left_out(gpu, first):
     """Rows that run backwards, behind the arrays or past the most nodes: nothing outside the arrays is touched (the guards of
