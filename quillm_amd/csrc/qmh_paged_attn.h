@@ -649,17 +649,29 @@ __device__ __forceinline__ void attend(const attn_args &s, float *lds, int row0,
     while (TREE && again);
 }
 
-// the rows of sequences [sq, sq + n): t0 to t0 + the result, 0 where they are none
+// the rows of sequence sq: t0 to t0 + the result, 0 where they are none
 template <bool TREE>
-__device__ __forceinline__ int attn_rows(const attn_args &s, int sq, int n, int &t0) {
+__device__ __forceinline__ int attn_rows(const attn_args &s, int sq, int &t0) {
     const int Q = s.a.q_len;
     if (!TREE || !s.tree.first) {
         t0 = sq * Q;
-        return n * Q;
+        return Q;
     }
     t0 = uniform(as_const(s.tree.first)[sq]);
-    const int64_t t1 = uniform(as_const(s.tree.first)[sq + n]), rows = t1 - t0;
-    return t0 < 0 || rows < 0 || t1 > s.tree.n_rows || rows > (int64_t)n * Q ? 0 : (int)rows;
+    const int64_t t1 = uniform(as_const(s.tree.first)[sq + 1]), rows = t1 - t0;
+    return t0 < 0 || rows < 0 || t1 > s.tree.n_rows || rows > Q ? 0 : (int)rows;
+}
+// the rows of a group from sequence sq on, those of sequences that are left out among them as far as q has them: the others' results
+// must not depend on them. They may be more than the group's sequences may have.
+template <bool TREE>
+__device__ __forceinline__ int group_rows(const attn_args &s, int sq, int &t0) {
+    if (!TREE || !s.tree.first) {
+        t0 = sq * s.a.q_len;
+        return s.n.per * s.a.q_len;
+    }
+    t0 = max(uniform(as_const(s.tree.first)[sq]), 0);
+    const int t1 = max(min(uniform(as_const(s.tree.first)[sq + s.n.per]), s.tree.n_rows), 0);
+    return max(t1 - t0, 0);
 }
 
 template <typename T, int HDP, int NRP, int NRO, bool TREE>
@@ -675,20 +687,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_attention(const attn_args s) {
         if (split >= n.ps) return;
         const uint32_t gk = unit - split * gks, g = gk / KV, kvh = gk - g * KV;
         int t0;
-        const int R = attn_rows<TREE>(s, g * n.per, n.per, t0) * n.G;
+        const int R = group_rows<TREE>(s, g * n.per, t0) * n.G;
         if (TREE && tile * 16 * NRP >= R) return;
         int len = uniform(as_const(s.a.prefix_len)[g]);
         const bool bad = len < 0 || len > s.a.max_prefix;
         if (bad) len = 0;
         const attn_list L = {s.a.prefix_table + (int64_t)g * s.a.prefix_stride, 0, len, split * n.pc, min(len, (split + 1) * n.pc), s.a.max_prefix - 1};
-        attend<T, HDP, NRP, TREE>(s, lds, tile * 16 * NRP, R, t0, 0, kvh, L, none, bad, split);
+        // tiles behind the last workgroup's are there only with sequences that are left out; a time's reads of LDS end before its last barrier
+        int row0 = tile * 16 * NRP;
+#pragma unroll 1
+        do attend_once<T, HDP, NRP, TREE>(s, lds, row0, R, t0, 0, kvh, L, none, bad, split, false);
+        while (TREE && (row0 += n.pt * 16 * NRP) < R);
         return;
     }
     b -= n.pre_blocks;
     const uint32_t units = (uint32_t)s.a.n_seq * KV, st = b / units, unit = b - st * units;
     const uint32_t tile = st / n.os, split = st - tile * n.os, sq = unit / KV, kvh = unit - sq * KV, g = sq / n.per;
     int t0;
-    const int R = attn_rows<TREE>(s, sq, 1, t0) * n.G;
+    const int R = attn_rows<TREE>(s, sq, t0) * n.G;
     if (TREE && (int)tile * 16 * NRO >= R) return;
     int len = s.a.max_len ? uniform(as_const(s.a.len)[sq]) : 0, plen = 0;
     bool bad = len < 0 || len > s.a.max_len || (TREE && len < R / n.G);
