@@ -310,7 +310,8 @@ int qmh_paged_plan(const qmh_plan_args *a, void *ws, size_t ws_bytes, void *stre
  * mask for all; bits of nodes that are not there have no effect). mask NULL: nodes 0 to j, a chain.
  * What a node does not see has no effect on it, whatever it holds. Values are summed with weights of up to 2^15 each before the sum of
  * these divides them: finite f32 and bf16 values above 2^112 over the number of positions may come out infinite. A node that sees nothing (or only scores of -inf) gives
- * zeros; where len is outside [n, max_len], or a page is outside the pool, rows are NaN as qmh_paged_attention says.
+ * zeros. Where a sequence's len is outside [n, max_len] all its rows are NaN, where a page is outside the pool the rows of
+ * the nodes that see a position of it: one of the context's (or of the group's prefix) is seen by all.
  * ws: qmh_tree_attention_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
 typedef struct {
     qmh_attention_args base;

@@ -410,8 +410,9 @@ struct attn_wave {
 };
 
 // Trees: a node that a row does not see must not reach it, whatever its values hold, but a product with 0 makes NaN of a value
-// that is not finite. Where sums are not finite, and some node's values are not either, a tile is made again: the positions before the nodes as
-// ever, then each row's nodes here, by the whole workgroup, from what the row sees alone: 256 nodes at a time, their scores a thread
+// that is not finite, and a page that is none makes NaN of the sums of all rows. Where sums are not finite, and some node's values are not
+// either or its page is none, a tile is made again: the positions before the nodes as ever, then each row's nodes here, by the
+// whole workgroup, from what the row sees alone: 256 nodes at a time, their scores a thread
 // each, then an output element a thread. That happens only there: looking at the values in the walk cost it registers, and 10 of 98 us of
 // 8 sequences of 4100, 32 x 128.
 constexpr int NODE_FLOATS = 256 + 256 + 512 + 4; // what it needs of LDS
@@ -479,7 +480,7 @@ __device__ __forceinline__ void attend_nodes(const attn_args &s, float *lds, flo
         s.part[to * hd + tid] = o;
     }
 }
-// whether the list's nodes, of those in its chunk, have a value that is not finite (for the whole workgroup)
+// whether the list's nodes, of those in its chunk, have a value that is not finite or a page that is none (for the whole workgroup)
 template <typename T>
 __device__ __forceinline__ bool odd_nodes(const attn_args &s, int ctx, int kvh, const attn_list &own) {
     constexpr int N = 16 / (int)sizeof(T);
@@ -487,7 +488,10 @@ __device__ __forceinline__ bool odd_nodes(const attn_args &s, int ctx, int kvh, 
     bool odd = false;
     for (int i = threadIdx.x; i < (own.to - from) * per; i += 256) {
         const int pos = from + i / per, page = own.tab[pos >> s.lg_ps];
-        if (page < 0 || page >= s.p.n_pages) continue;
+        if (page < 0 || page >= s.p.n_pages) {
+            odd = true;
+            continue;
+        }
         const int64_t row = (((int64_t)page * s.p.n_kv_heads + kvh) * s.p.page_size + (pos & (s.p.page_size - 1))) * s.p.head_dim;
         const qmh_vec<T, N> x = *(const qmh_vec<T, N> *)((const T *)s.p.v + row + i % per * N);
 #pragma unroll
@@ -612,7 +616,7 @@ __device__ __forceinline__ bool attend_once(const attn_args &s, float *lds, int 
             continue;
         }
         if constexpr (TREE)
-            if (!__builtin_isfinite(o[0] + o[1] + (o[2] + o[3]))) atomicOr(&odd[col >> 5], 1u << (col & 31));
+            if (!__builtin_isfinite(o[0] + o[1] + (o[2] + o[3]) + l)) atomicOr(&odd[col >> 5], 1u << (col & 31));
         if (part < 0) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             qmh_vec<T, 4> y;
