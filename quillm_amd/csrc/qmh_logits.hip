@@ -358,11 +358,14 @@ extern "C" int qmh_launch_logits_edit(const qmh_logits_args *a, int cus, void *w
     if (blocks > 0xffffffffll) return (int)hipErrorInvalidValue;
     qmh_for_type(a->dtype, [&](auto z) {
         using T = decltype(z);
-        for (int64_t b0 = 0; b0 < blocks; b0 += QMH_MOST_BLOCKS) { // workgroups write different places: any number of launches
-            const dim3 g((uint32_t)(blocks - b0 < QMH_MOST_BLOCKS ? blocks - b0 : QMH_MOST_BLOCKS));
+        constexpr int64_t most_blocks = qmh_most_blocks(NT);
+        for (int64_t b0 = 0; b0 < blocks; b0 += most_blocks) { // workgroups write different places: any number of launches
+            const dim3 g((uint32_t)(blocks - b0 < most_blocks ? blocks - b0 : most_blocks));
             hipLaunchKernelGGL((k_logits_edit<T>), g, dim3(NT), 0, st, *a, segs, chunks, chunk, (uint32_t)b0, (uint64_t *)ws);
         }
     });
+    const int failed = (int)hipGetLastError();
+    if (failed) return failed; // what the next one reads is not there
     if (a->best && segs > 1) hipLaunchKernelGGL(k_logits_best, dim3(a->n_seq, most < 4 * 60 ? (most + 3) / 4 : 60), dim3(256), 0, st, *a, segs, (const uint64_t *)ws);
     return (int)hipGetLastError();
 }

@@ -11,8 +11,10 @@ __device__ __forceinline__ float qmh_to_f(float x) { return x; }
 __device__ __forceinline__ float qmh_to_f(qmh_f16 x) { return (float)x; }
 __device__ __forceinline__ float qmh_to_f(qmh_bf16 x) { return (float)x; }
 
-// blocks of 256 threads in a launch: a grid holds fewer than 2^32 threads
-constexpr int64_t QMH_MOST_BLOCKS = (1 << 24) - 1;
+// blocks of so many threads in a launch: a grid holds fewer than 2^32 threads
+constexpr int64_t qmh_most_blocks(int threads) { return 0xffffffffll / threads; }
+constexpr int64_t QMH_MOST_BLOCKS = qmh_most_blocks(256);
+static_assert(QMH_MOST_BLOCKS == (1 << 24) - 1 && qmh_most_blocks(512) * 512 < 1ll << 32 && qmh_most_blocks(512) == (1 << 23) - 1);
 
 // N elements of T that are loaded and stored at once (N * sizeof(T) up to 16 bytes, aligned to it)
 template <typename T, int N>
