@@ -340,7 +340,8 @@ int qmh_tree_attention(const qmh_tree_args *a, void *ws, size_t ws_bytes, void *
  * outside [0, n_allow): all may; allow_row NULL: row r of allow, n_allow >= n_rows). allow NULL: no grammar.
  * node_token [n_seq][node_stride] (NULL: rows are no trees): row j of sequence i has the nodes that its mask's row says behind its
  * history, as outputs: itself and its ancestors (mask, mask_stride, mask_words as for qmh_tree_attention; mask NULL: nodes 0 to j).
- * vocab at most 2^24; n_seq at most 65535; rows_per_seq at most 1024 with node_token.
+ * vocab at most 2^24; n_seq at most 65535; rows_per_seq at most 1024 with node_token. With r the lower of rows_per_seq and n_rows,
+ * n_seq * ceil(r / 32) * ceil(vocab / 4096) is below 2^32 (each of these costs a look, also where a sequence has fewer rows).
  * ws: qmh_logits_edit_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
 typedef struct {
     int32_t dtype, n_rows, vocab;

@@ -260,6 +260,7 @@ int qmh_launch_paged_plan(const qmh_plan_args *a, void *ws, void *stream);
 size_t qmh_tree_ws_bytes(const qmh_tree_args *a, int cus);
 int qmh_launch_tree_attention(const qmh_tree_args *a, int cus, void *ws, void *stream);
 size_t qmh_logits_ws_bytes(const qmh_logits_args *a, int cus);
+int64_t qmh_logits_blocks(const qmh_logits_args *a); // workgroups that rows_per_seq rows of every sequence need
 int qmh_launch_logits_edit(const qmh_logits_args *a, int cus, void *ws, void *stream);
 int qmh_launch_tree_accept(const qmh_accept_args *a, void *stream);
 

@@ -335,6 +335,8 @@ __global__ __launch_bounds__(256) void k_logits_best(const qmh_logits_args a, in
 }
 
 int segments(const qmh_logits_args *a) { return (a->vocab + SEG - 1) / SEG; }
+// rows of a sequence, at most
+int most_rows(const qmh_logits_args *a) { return a->rows_per_seq < a->n_rows ? a->rows_per_seq : a->n_rows; }
 
 } // namespace
 
@@ -343,19 +345,20 @@ extern "C" size_t qmh_logits_ws_bytes(const qmh_logits_args *a, int) {
     return a->best && segs > 1 ? sizeof(uint64_t) * (size_t)a->n_rows * segs : 0;
 }
 
+extern "C" int64_t qmh_logits_blocks(const qmh_logits_args *a) { return (int64_t)a->n_seq * segments(a) * ((most_rows(a) + ROWS - 1) / ROWS); }
+
 extern "C" int qmh_launch_logits_edit(const qmh_logits_args *a, int cus, void *ws, void *stream) {
     hipStream_t st = (hipStream_t)stream;
     const int segs = segments(a);
     const int64_t units = (int64_t)a->n_seq * segs;
     // rows of a workgroup: as few as fill the chip's workgroups once (three a CU); each counts the history again
-    int most = a->rows_per_seq < a->n_rows ? a->rows_per_seq : a->n_rows;
+    const int most = most_rows(a);
     int chunks = units < 3 * cus ? (int)(3 * cus / units) : 1;
     chunks = chunks < most ? chunks : most;
     if (chunks < (most + ROWS - 1) / ROWS) chunks = (most + ROWS - 1) / ROWS;
     const int chunk = (most + chunks - 1) / chunks;
     chunks = (most + chunk - 1) / chunk;
-    const int64_t blocks = units * chunks;
-    if (blocks > 0xffffffffll) return (int)hipErrorInvalidValue;
+    const int64_t blocks = units * chunks; // below 2^32: the host code checks it
     qmh_for_type(a->dtype, [&](auto z) {
         using T = decltype(z);
         constexpr int64_t most_blocks = qmh_most_blocks(NT);

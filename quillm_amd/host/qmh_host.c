@@ -585,6 +585,8 @@ static int check_logits(const qmh_logits_args *a, const char *me) {
     if (a->rows_per_seq < 1 || a->rows_per_seq > 1 << 20) return fail("%s: rows_per_seq %d outside [1, 2^20]", me, a->rows_per_seq);
     if (!a->first && (int64_t)a->n_seq * a->rows_per_seq > a->n_rows)
         return fail("%s: %d rows for %d sequences of %d", me, a->n_rows, a->n_seq, a->rows_per_seq);
+    if (qmh_logits_blocks(a) > 0xffffffffll)
+        return fail("%s: %d sequences of up to %d rows of %d tokens are too many for a call", me, a->n_seq, a->rows_per_seq, a->vocab);
     if (check_rows(me, "logits", a->logits, a->stride, a->vocab, es)) return -1;
     if (!a->out && !a->best) return fail("%s: neither out nor best", me);
     if (a->out && check_rows(me, "out", a->out, a->out_stride, a->vocab, es)) return -1;
