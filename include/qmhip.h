@@ -304,7 +304,8 @@ size_t qmh_paged_plan_ws(const qmh_plan_args *a);
 int qmh_paged_plan(const qmh_plan_args *a, void *ws, size_t ws_bytes, void *stream);
 
 /* qmh_paged_attention with nodes of trees in place of consecutive queries. base: as there, but q_len is the most nodes of a
- * sequence, and q and out have n_rows rows (with first NULL at least n_seq * q_len). The n nodes of a sequence are the last n
+ * sequence, and q and out have n_rows rows (at most 2^20; with first NULL at least n_seq * q_len, with first n_seq and q_len are at most
+ * 2^20 each). The n nodes of a sequence are the last n
  * of its len positions; node j sees the group's prefix, the len - n positions before the nodes, and those nodes that row j
  * of the sequence's mask says: words at mask + i * mask_stride + j * mask_words (mask_words >= ceil(q_len / 32), mask_stride 0: one
  * mask for all; bits of nodes that are not there have no effect). mask NULL: nodes 0 to j, a chain.

@@ -788,6 +788,8 @@ attn_plan plan_attention(const qmh_attention_args *a, int64_t n_rows, int cus) {
     n.pt = (int)((rp + 16 * n.nrp - 1) / (16 * n.nrp));
     n.ot = (int)((ro + 16 * n.nro - 1) / (16 * n.nro));
     const int64_t up = (int64_t)a->n_groups * KV * n.pt, uo = (int64_t)a->n_seq * KV * n.ot;
+    n.blocks = up + uo;
+    if (up > QMH_MOST_BLOCKS || uo > QMH_MOST_BLOCKS) return n; // too many, however they are split
     int64_t pre = 0;
     n.os = 1;
     n.oc = a->max_len ? a->max_len : 1;

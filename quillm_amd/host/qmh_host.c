@@ -390,13 +390,14 @@ int qmh_paged_append(const qmh_append_args *a, void *stream) {
     return 0;
 }
 
-static int check_attention(const qmh_attention_args *a, const char *me) {
+/* ragged: the sequences' rows are counted elsewhere, q_len is a bound of each one's */
+static int check_attention(const qmh_attention_args *a, int ragged, const char *me) {
     if (!a) return fail("%s: NULL arguments", me);
     if (check_pages(a->pages, 1, me)) return -1;
     const qmh_pages *p = a->pages;
     if (a->n_heads < 1 || a->n_heads > 4096 || a->n_heads % p->n_kv_heads)
         return fail("%s: n_heads %d is not a multiple of n_kv_heads %d up to 4096", me, a->n_heads, p->n_kv_heads);
-    if (a->n_seq < 0 || a->q_len < 1 || (int64_t)a->n_seq * a->q_len > 1 << 20)
+    if (a->n_seq < 0 || a->q_len < 1 || a->n_seq > 1 << 20 || a->q_len > 1 << 20 || (!ragged && (int64_t)a->n_seq * a->q_len > 1 << 20))
         return fail("%s: %d sequences of %d queries (at most 2^20)", me, a->n_seq, a->q_len);
     if (a->n_groups < 1 || (a->n_seq && a->n_seq % a->n_groups))
         return fail("%s: %d sequences in %d groups", me, a->n_seq, a->n_groups);
@@ -417,13 +418,13 @@ static int check_attention(const qmh_attention_args *a, const char *me) {
 }
 
 size_t qmh_paged_attention_ws(const qmh_attention_args *a) {
-    if (check_attention(a, "paged_attention_ws") || ensure()) return 0;
+    if (check_attention(a, 0, "paged_attention_ws") || ensure()) return 0;
     return qmh_attention_ws_bytes(a, g_cus);
 }
 
 int qmh_paged_attention(const qmh_attention_args *a, void *ws, size_t ws_bytes, void *stream) {
     static const char *me = "paged_attention";
-    if (check_attention(a, me) || on_device(me)) return -1;
+    if (check_attention(a, 0, me) || on_device(me)) return -1;
     if (a->n_seq == 0) return 0;
     const size_t need = qmh_attention_ws_bytes(a, g_cus);
     if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
@@ -554,7 +555,7 @@ static int check_mask(const char *me, const uint32_t *mask, int64_t stride, int3
 
 static int check_tree(const qmh_tree_args *a, const char *me) {
     if (!a) return fail("%s: NULL arguments", me);
-    if (check_attention(&a->base, me)) return -1;
+    if (check_attention(&a->base, a->first != NULL, me)) return -1;
     if (a->n_rows < 0 || a->n_rows > 1 << 20) return fail("%s: n_rows %d outside [0, 2^20]", me, a->n_rows);
     if (!a->first && (int64_t)a->base.n_seq * a->base.q_len > a->n_rows)
         return fail("%s: %d rows for %d sequences of %d nodes", me, a->n_rows, a->base.n_seq, a->base.q_len);

@@ -13,23 +13,24 @@ pytestmark = pytest.mark.gpu
 Q, ROWS = 5, 16  # the most nodes of a sequence, rows of q and out
 
 
-def run(q, dt, H, KV, hd, first, own, prefix, groups=1):
+def run(q, dt, H, KV, hd, first, own, prefix, groups=1, Q=Q, ROWS=ROWS, static=False):
     """Outputs and tolerance-checked rows of the good sequences; bytes of the others' rows are anything."""
     rs, ps, B = np.random.default_rng(hd + len(first)), 16, len(own)
     tables, n_pages = o.make_tables(rs, [-(-n // ps) for n in prefix + own], -(-max(prefix + own) // ps) + 1)
     k, v = (o.encode(rs.standard_normal((n_pages, KV, ps, hd)), dt) for _ in range(2))
     x = o.encode(rs.standard_normal((ROWS, H * hd)) * 1.5, dt)
-    see = [tr.ancestors(tr.tree(rs, Q)) for _ in range(B)]
+    see = [tr.ancestors(tr.tree(rs, Q)) for _ in range(1 if static else B)]
+    words = -(-Q // 32)
     dk, dv, dx, out = o.Guarded(q, k), o.Guarded(q, v), o.Guarded(q, x), o.Guarded(q, np.full((ROWS, H * hd), 0x55, o.raw(dt)))
     dev = q.DeviceBuffer.from_array
     tab, ptab, n, pn, at, mask = (dev(np.ascontiguousarray(y)) for y in (
-        tables[groups:], tables[:groups], np.array(own, np.int32), np.array(prefix, np.int32), np.array(first, np.int32), tr.pack(np.array(see), 1)))
+        tables[groups:], tables[:groups], np.array(own, np.int32), np.array(prefix, np.int32), np.array(first, np.int32), tr.pack(np.array(see), words)))
     pages = q.Pages(dtype=dt, n_kv_heads=KV, head_dim=hd, page_size=ps, n_pages=n_pages, k=dk.ptr, v=dv.ptr)
     scale = float(np.float32(hd ** -0.5))
     base = q.AttentionArgs(pages=ctypes.pointer(pages), n_heads=H, n_seq=B, q_len=Q, n_groups=groups, q=dx.ptr, q_stride=H * hd, out=out.ptr,
                            out_stride=H * hd, table=tab.ptr, len=n.ptr, table_stride=tables.shape[1], max_len=max(own), prefix_table=ptab.ptr,
-                           prefix_len=pn.ptr, prefix_stride=tables.shape[1], max_prefix=max(prefix), scale=scale)
-    a = q.TreeArgs(base=base, n_rows=ROWS, first=at.ptr, mask=mask.ptr, mask_stride=Q, mask_words=1)
+                           prefix_len=pn.ptr, prefix_stride=tables.shape[1], max_prefix=max(prefix + [0]), scale=scale)
+    a = q.TreeArgs(base=base, n_rows=ROWS, first=at.ptr, mask=mask.ptr, mask_stride=0 if static else Q * words, mask_words=words)
     L = q.load_library()
     need = L.qmh_tree_attention_ws(ctypes.byref(a))
     ws = o.Guarded(q, np.full(max(need, 16), 0xFF, np.uint8))
@@ -47,7 +48,7 @@ def run(q, dt, H, KV, hd, first, own, prefix, groups=1):
         pk, pv = (o.rows_of(y, tables[i // (B // groups)], prefix[i // (B // groups)], ps) for y in kv)
         ok, ov = (o.rows_of(y, tables[groups + i], own[i], ps) for y in kv)
         for j in range(a1 - a0):
-            t = np.concatenate([np.ones(own[i] - (a1 - a0), bool), see[i][j, :a1 - a0]])
+            t = np.concatenate([np.ones(own[i] - (a1 - a0), bool), see[0 if static else i][j, :a1 - a0]])
             kk, ww = np.concatenate([pk, ok[t]]), np.concatenate([pv, ov[t]])
             want, mag, reach = o.attention(xv[a0 + j], kk, ww, scale)
             # scores of hd products, exponentials to 2 steps, sums of n terms, 16-bit probabilities rounded to the type, then the result
@@ -83,3 +84,14 @@ def test_more_rows_than_the_prefix_has_tiles_for(gpu, H, KV, hd):
     assert need > 0 and good == 2
     need, good = run(gpu, o.BF16, H, KV, hd, [0, 2, 4, 13, 16], [600, 300, 300, 600], [900, 1100], groups=2)
     assert need > 0 and good == 7
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("prefix", [0, 70, 600])
+def test_few_rows_of_many_sequences(gpu, dtype, prefix):
+    """1100 sequences of up to 1000 nodes, of which a few have some: the rows there are count, not the product."""
+    counts = np.zeros(1100, int)
+    counts[[0, 3, 500, 501, 777, 1099]] = [1, 40, 7, 3, 180, 69]
+    first = [0, *np.cumsum(counts).tolist()]
+    need, good = run(gpu, o.TYPES[dtype], 8, 2, 32, first, [int(n) + 9 for n in counts], [prefix] * 11, groups=11, Q=1000, ROWS=300, static=True)
+    assert good == 300

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from test_paged_refusals import P, refused
-from test_tree_refusals import logits_args
+from test_tree_refusals import logits_args, tree_args
 
 
 @pytest.mark.parametrize("kw", [
@@ -30,3 +30,19 @@ def test_logits_that_are_not(qmh, kw):
     a = logits_args(qmh, first=P, stride=n, out_stride=n, allow=None, node_token=None, **kw)
     assert qmh.load_library().qmh_logits_edit(ctypes.byref(a), None, 0, None) == -1
     assert "too many" not in qmh.last_error()
+
+
+@pytest.mark.parametrize("n_seq,q_len", [(1026, 1024), (1 << 20, 1 << 20), (2, 1 << 20)])
+def test_attention_counts_rows_not_sequences_times_nodes(qmh, n_seq, q_len):
+    """The rows that there are (here -1: refused for that), not n_seq * q_len, are bounded where first says whose they are."""
+    L = qmh.load_library()
+    base = dict(n_seq=n_seq, q_len=q_len)
+    for first, what in ((P, "n_rows"), (None, "queries")):
+        a = tree_args(qmh, base=base, n_rows=-1, first=first, mask=None)
+        assert L.qmh_tree_attention_ws(ctypes.byref(a)) == 0
+        refused(qmh, L.qmh_tree_attention(ctypes.byref(a), P, 1 << 40, None), "tree_attention")
+        assert what in qmh.last_error()
+    for bad in (dict(n_seq=(1 << 20) + 2), dict(q_len=(1 << 20) + 1)):
+        a = tree_args(qmh, base={**base, **bad}, mask=None)
+        refused(qmh, L.qmh_tree_attention(ctypes.byref(a), P, 1 << 40, None), "tree_attention")
+        assert "queries" in qmh.last_error()
