@@ -386,7 +386,8 @@ int qmh_logits_edit(const qmh_logits_args *a, void *ws, size_t ws_bytes, void *s
  * pages (NULL: nothing is moved): keys and values of accepted nodes move to the positions len - n on, in n_layers pools that
  * are layer_stride elements apart (pages->k and v are the first layer's; a multiple of 16 bytes), through table [n_seq][table_stride].
  * Where either place's page is outside the pool, that node is not moved. No page may be in two of the table's places.
- * count, next and keep must not overlap each other or any input. n_seq at most 65535, n_layers at most 1024. */
+ * What is written (count, path, next, keep, history, history_len) must not overlap each other or what is read (history_len is not
+ * len: workgroups of a sequence read the one while another writes the other). n_seq at most 65535, n_layers at most 1024. */
 typedef struct {
     int32_t n_seq, tree_size;
     const int32_t *parent;

@@ -635,8 +635,6 @@ int qmh_tree_accept(const qmh_accept_args *a, void *stream) {
     if (!a->first && (int64_t)a->n_seq * a->tree_size > a->n_rows)
         return fail("%s: %d rows for %d sequences of %d nodes", me, a->n_rows, a->n_seq, a->tree_size);
     if (!a->count || !a->next || !a->keep) return fail("%s: NULL count, next or keep", me);
-    if (a->keep == a->len || a->count == a->len || a->next == a->len || a->next == a->choice || a->count == a->next || a->count == a->keep || a->next == a->keep)
-        return fail("%s: outputs overlap each other or an input", me);
     if (a->history && (!a->history_len || a->history_stride < 1 || a->history_stride > 1 << 24))
         return fail("%s: history needs history_len and a stride of 1 to 2^24", me);
     if (a->pages) {
@@ -647,6 +645,15 @@ int qmh_tree_accept(const qmh_accept_args *a, void *stream) {
             return fail("%s: layer_stride %lld of pools of %lld elements", me, (long long)a->layer_stride, (long long)pool);
         if (!a->table || a->table_stride < 1 || (int64_t)a->table_stride * a->pages->page_size > 0x7fffffff)
             return fail("%s: a table of %d pages a sequence", me, a->table_stride);
+    }
+    /* workgroups of one sequence write the outputs while others still read the inputs */
+    const int32_t *const in[] = {a->parent, a->token, a->choice, a->len, a->first, a->pages ? a->table : NULL};
+    const int32_t *const out[] = {a->count, a->next, a->keep, a->path, a->history, a->history ? a->history_len : NULL};
+    for (int i = 0; i < 6; i++) {
+        for (int k = 0; k < 6; k++)
+            if (out[i] && out[i] == in[k]) return fail("%s: an output overlaps an input", me);
+        for (int k = 0; k < i; k++)
+            if (out[i] && out[i] == out[k]) return fail("%s: outputs overlap each other", me);
     }
     if (on_device(me)) return -1;
     if (a->n_seq == 0) return 0;

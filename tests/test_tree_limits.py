@@ -1,11 +1,11 @@
-"""Sizes of the ops for drafted trees that are too large together, though each is within its range: refused before anything reaches a
-device, and the largest that are not."""
+"""Sizes of the ops for drafted trees that are too large together, though each is within its range, and arrays that overlap: refused
+before anything reaches a device, and the largest sizes that are not."""
 import ctypes
 
 import pytest
 
 from test_paged_refusals import P, refused
-from test_tree_refusals import logits_args, tree_args
+from test_tree_refusals import accept_args, logits_args, tree_args
 
 
 @pytest.mark.parametrize("kw", [
@@ -46,3 +46,14 @@ def test_attention_counts_rows_not_sequences_times_nodes(qmh, n_seq, q_len):
         a = tree_args(qmh, base={**base, **bad}, mask=None)
         refused(qmh, L.qmh_tree_attention(ctypes.byref(a), P, 1 << 40, None), "tree_attention")
         assert "queries" in qmh.last_error()
+
+
+INPUTS, OUTPUTS = "parent token choice len first table".split(), "count path next keep history history_len".split()
+
+
+@pytest.mark.parametrize("out,other", [(x, y) for x in OUTPUTS for y in INPUTS + OUTPUTS if x != y])
+def test_accept_of_arrays_that_are_two_things(qmh, out, other):
+    d = {k: (10 + i) * P for i, k in enumerate(INPUTS + OUTPUTS)}
+    d[out] = d[other]
+    refused(qmh, qmh.load_library().qmh_tree_accept(ctypes.byref(accept_args(qmh, **d)), None), "tree_accept")
+    assert "overlap" in qmh.last_error()
