@@ -281,7 +281,8 @@ int qmh_paged_reorder(const qmh_pages *pages, const int32_t *table, int32_t tabl
  * more than the table row or the tree takes); 1 pages are short (it needs some and the sum of what it and the sequences before it
  * ask for is more than there are; or the ring has no room for what it gives); 2 rows are short (n_tokens, likewise).
  * Of a refused sequence nothing changes, and it has no rows.
- * n_seq at most 65535, n_seq * table_stride below 2^31, n_tokens at most 2^24. keep may be len.
+ * n_seq at most 65535, n_seq * table_stride below 2^31, n_tokens at most 2^24. keep may be len; nothing else that is written
+ * may overlap what is read or written (base is not len).
  * ws: qmh_paged_plan_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
 typedef struct {
     int32_t n_seq, page_size;

@@ -521,6 +521,7 @@ static int check_plan(const qmh_plan_args *a, const char *me) {
     if (a->free_size < 1 || a->free_size > 0x40000000) return fail("%s: free_size %d outside [1, 2^30]", me, a->free_size);
     if (a->n_tokens < 0 || a->n_tokens > 1 << 24) return fail("%s: n_tokens %d outside [0, 2^24]", me, a->n_tokens);
     if (a->n_tokens && (!a->first || !a->seq || !a->slot || !a->pos)) return fail("%s: NULL first, seq, slot or pos", me);
+    if (a->n_tokens && a->base == a->len) return fail("%s: base is len, which the call changes before it looks at base", me);
     if (a->parent) {
         if (!a->n_tokens) return fail("%s: trees need n_tokens", me);
         if (a->tree_size < 1 || a->tree_size > 1024) return fail("%s: tree_size %d outside [1, 1024]", me, a->tree_size);

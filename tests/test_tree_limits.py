@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from test_paged_refusals import P, refused
-from test_tree_refusals import accept_args, logits_args, tree_args
+from test_tree_refusals import accept_args, logits_args, plan_args, tree_args
 
 
 @pytest.mark.parametrize("kw", [
@@ -57,3 +57,11 @@ def test_accept_of_arrays_that_are_two_things(qmh, out, other):
     d[out] = d[other]
     refused(qmh, qmh.load_library().qmh_tree_accept(ctypes.byref(accept_args(qmh, **d)), None), "tree_accept")
     assert "overlap" in qmh.last_error()
+
+
+def test_plan_of_positions_that_count_from_the_length(qmh):
+    """Lengths are written before positions are: base has to be a copy."""
+    L, a = qmh.load_library(), plan_args(qmh, base=P)
+    assert L.qmh_paged_plan_ws(ctypes.byref(a)) == 0
+    refused(qmh, L.qmh_paged_plan(ctypes.byref(a), P, 1 << 40, None), "paged_plan")
+    assert "base" in qmh.last_error()
