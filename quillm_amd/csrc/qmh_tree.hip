@@ -182,7 +182,8 @@ __device__ __forceinline__ void plan_tokens(const qmh_plan_args &a, const plan_a
             int x[3][4], s = t < total ? plan_find(p.tok, n, t) : n;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                while (s < n && t + i >= p.tok[s + 1]) s++;
+                if (t + i >= total) s = n;
+                else if (t + i >= p.tok[s + 1] && t + i >= p.tok[++s + 1]) s = plan_find(p.tok, n, t + i); // past sequences without rows
                 const int slot = s < n ? p.keep[s] + (t + i - p.tok[s]) : -1;
                 x[0][i] = s < n ? s : -1;
                 x[1][i] = slot;
