@@ -18,7 +18,7 @@ constexpr int PLAN_CHUNK = 1024;   // tokens of a workgroup otherwise
 constexpr int TREE_MOST = 1024;    // nodes of a tree
 
 // Nothing here computes: a call is a chain of loads (lengths, sums, pages or parents, stores), so the work goes into as few launches and
-// dependent steps as can be. Measured: trees of 48 sequences, 870 nodes, 4.2 us, an empty launch's time; prompts of 201 sequences, 181000 rows
+// dependent steps as can be. A node's thread walks to its root, a read of LDS a step. Measured: trees of 48 sequences, 870 nodes, 4.2 us, an empty launch's time; prompts of 201 sequences, 181000 rows
 // in two launches 10 us (3.4 of scan, 6 of rows, 2.2 MB).
 // What the scan finds: exclusive sums over the sequences (n + 1 of each) of tokens, pages taken and pages given, a sequence's pages
 // before and after, and the positions it keeps. For a call of one workgroup they lie in LDS, else in the workspace.
@@ -218,11 +218,11 @@ __device__ __forceinline__ void plan_tokens(const qmh_plan_args &a, const plan_a
         const int s = plan_find(p.tok, n, t), j = t - p.tok[s], keep = p.keep[s], base = a.base ? a.base[s] : 0;
         const int16_t *up = par + (p.tok[s] - from);
         uint32_t *out = a.mask ? a.mask + ((int64_t)s * a.tree_size + j) * words : nullptr;
-        int depth = -1; // as many as there are ancestors
-        for (int w = 0; w < words; w += 2) {
+        // one walk: ancestors come in falling order, so the mask's words are done with from the last one down
+        int depth = -1, x = j;
+        for (int w = (words - 1) & ~1; w >= 0; w -= 2) {
             uint64_t bits = 0;
-            for (int x = j; x >= 0; x = up[x])
-                if (x >> 6 == w >> 1) bits |= 1ull << (x & 63);
+            for (; x >= 32 * w; x = up[x]) bits |= 1ull << (x & 63);
             depth += __popcll(bits);
             if (out) {
                 out[w] = (uint32_t)bits;

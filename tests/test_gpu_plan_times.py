@@ -6,6 +6,7 @@ import time
 import numpy as np
 import pytest
 
+import _trees as tr
 from test_gpu_plan import State, call
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,29 @@ def test_sequences_without_rows_between_others(gpu, gap, n):
     s = State(gpu, n, 16, 2, 2 * n, 2 * n, seed=gap)
     s.upload()
     call(gpu, s, None, add, max(int(add.sum()) * 2 // 3, 1))
+
+
+@pytest.mark.parametrize("mask", [False, True])
+def test_trees_with_room_for_more_nodes(gpu, mask):
+    """A chain of 256 nodes takes as long where trees may have 1024 as where they may have 256."""
+    times = []
+    for size in (256, 1024):
+        t, (seq, slot, pos) = least(gpu, [256], 256, parent=np.arange(-1, size - 1), tree=size, mask=mask)
+        times.append(t)
+        assert (seq == 0).all() and np.array_equal(slot, np.arange(256)) and np.array_equal(pos, slot)
+    assert times[1] < 2 * times[0], times
+
+
+@pytest.mark.parametrize("size", [1, 31, 32, 33, 63, 64, 65, 96, 97, 129, 1000, 1024])
+@pytest.mark.parametrize("shape", ["chain", "star", "teeth", "any"])
+def test_masks_word_by_word(gpu, size, shape):
+    """Ancestors in every word, in the first and last ones alone, and in some."""
+    j = np.arange(size)
+    rs = np.random.default_rng(size)
+    par = {"chain": j - 1, "star": np.where(j, 0, -1), "teeth": np.maximum(j - 70, -1), "any": tr.tree(rs, size, 0.2)}[shape]
+    for n, mask in ((1, True), (5, True), (5, False)):
+        s = State(gpu, n, 16, -(-size // 16), n * 64, n * 64, seed=size)
+        s.upload()
+        add = rs.integers(0, size + 1, n)
+        add[0] = size
+        call(gpu, s, None, add, int(add.sum()) + 3, parent=np.tile(par, (n, 1)).astype(np.int32), tree=size, static=True, mask=mask)
