@@ -310,9 +310,9 @@ int qmh_paged_plan(const qmh_plan_args *a, void *ws, size_t ws_bytes, void *stre
  * of its len positions; node j sees the group's prefix, the len - n positions before the nodes, and those nodes that row j
  * of the sequence's mask says: words at mask + i * mask_stride + j * mask_words (mask_words >= ceil(q_len / 32), mask_stride 0: one
  * mask for all; bits of nodes that are not there have no effect). mask NULL: nodes 0 to j, a chain.
- * What a node does not see has no effect on it, whatever it holds. Values are summed with weights of up to 2^15 each before the sum of
- * these divides them: finite f32 and bf16 values above 2^112 over the number of positions may come out infinite. A node that sees nothing (or only scores of -inf) gives
- * zeros. Where a sequence's len is outside [n, max_len] all its rows are NaN, where a page is outside the pool the rows of
+ * With 16-bit rows probabilities are rounded to their type, as there. What a node does not see has no effect on it, whatever it holds.
+ * Values are summed with weights of up to 2^15 each before the sum of these divides them: finite f32 and bf16 values above 2^112 over
+ * the number of positions may come out infinite. A node that sees nothing (or only scores of -inf) gives zeros. Where a sequence's len is outside [n, max_len] all its rows are NaN, where a page is outside the pool the rows of
  * the nodes that see a position of it: one of the context's (or of the group's prefix) is seen by all.
  * ws: qmh_tree_attention_ws(a) bytes (0: none is needed, or bad arguments), 16-byte aligned, any contents. */
 typedef struct {

@@ -37,11 +37,13 @@ namespace {
 // scores between this step's exponentials gained nothing.
 //
 // Trees: nodes in place of queries, each with the positions of a step that it sees as bits (look), which cost only the steps that some
-// row does not see all of. Measured: 8 sequences of 4100, 24 to 32 nodes, 32 x 128 bf16 82 us, the time of a copy of their keys and values.
+// row does not see all of. Measured: 8 sequences of 4100, 16 to 32 nodes, 32 x 128 bf16 82 to 88 us by device (a copy of their keys and values: 82).
 // Where many rows share the keys (64 nodes x 8 heads, 12 sequences of 6000, 64 f16: 69 us, 420 TFLOP/s) the first-level cache is the bound:
 // 16 lanes next to each other ask for 16 rows' parts of a key, 256 of a step's 430 lookups, four waves a CU at once. Without its loads a
-// step of 64 rows takes 1140 cycles, with them 1650. Copies straight into LDS halve the lookups, but their own instructions (some 100
-// a step) cost more: 78 us two steps ahead, 71 one step ahead. Two waves a SIMD are 1.6 times one.
+// step of 64 rows takes 1140 cycles, with them 1650. Copies straight into LDS, a buffer a wave, halve the lookups, but their own
+// instructions (some 100 a step) cost more: 78 us two steps ahead, 71 one step ahead. One buffer for the four waves was not tried. Two waves
+// a SIMD are 1.6 times one. Tree kernels spill, likely for what makes a tile again (attend_nodes): 46 to 73 scalar registers and 20 to 56
+// bytes of scratch a lane up to heads of 128, 156 to 204 (16 bit) and 324 (f32) past that; without trees 0 to 10, none, 116 and 252.
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -820,7 +822,8 @@ attn_plan plan_attention(const qmh_attention_args *a, int64_t n_rows, int cus) {
         if (TREE && !a->max_prefix && a->max_len) {
             // Trees without a prefix: one workgroup a CU where few rows share the keys (reading them bounds it: 8 x 32 walks of 4100 x 128 take
             // 87 us whole, 95 in two chunks each; 4 x 32 52 in two, 57 in four), two a CU where many do and their products bound it (24 tiles
-            // of 30011 x 64 35 us in 16 chunks, 31 in 21; but 256 of 6000 48 whole, 51 in two).
+            // of 30011 x 64 35 us in 16 chunks, 31 in 21; but 256 of 6000 48 whole, 51 in two). The rule looks at tiles alone: each of these was
+            // measured at one length, and many tiles of long sequences may want more parts than it gives them.
             const int64_t slots = uo * 4 >= cus * 3 ? uo : n.ot >= 4 ? 2 * cus : cus;
             const int64_t k = slots / uo < 48 ? slots / uo : 48;
             n.oc = (int)((a->max_len + k - 1) / k + unit - 1) / unit * unit;
